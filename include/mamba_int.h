@@ -508,6 +508,90 @@ mi_status mi_decode_step_static(const mi_model_params *params, int m, const int6
                                 int32_t *logits, int ld_logits, int8_t *const *conv_state,
                                 int32_t *const *h_state, void *stream);
 
+/* ------------------------------------------- float operators (forward only) */
+/* The float layer around the ternary projections, for models whose recurrence
+ * was trained in floating point: residual addition + RMS norm (float rows, or
+ * the 8-bit rows and scales that mi_bitlinear MI_OUT_FLOAT reads), the short
+ * causal convolution, the selective state space scan, and products of a few
+ * rows with 4-bit weights.  Element types below are mi_dtype values; sums,
+ * statistics and states are 32-bit floats.  Row strides (ld*) and sequence
+ * strides (bs*) count elements; a stride of an input may be 0 (one row for
+ * all).  The elements of a row are adjacent.  Outputs must not overlap inputs
+ * except where stated. */
+typedef enum { MI_F32 = 0, MI_BF16 = 1, MI_F16 = 2 } mi_dtype;
+
+/* Residual addition and root-mean-square norm of `tokens` rows of dim values:
+ *   s = residual + x,  y = s / sqrt(mean(s^2) + eps) * weight
+ * with s in 32 bits (not rounded to the residual's type first).  x of x_type;
+ * residual of res_type (x_type or MI_F32), nullable (s = x); weight fp32 [dim].
+ * Outputs, each nullable, y or q required:
+ *   res_out  s in res_type (may be residual itself);
+ *   y        in x_type (may be x itself);
+ *   q, scale int8 rows of ldq values (columns from dim on zero) and fp32
+ *            [tokens]: scale = max(max |y|, 1e-8) / 127 and q = clamp(
+ *            round_half_even(y * (127 / max(max |y|, 1e-8))), +-127), the rule
+ *            of mi_act_quant_f32.  A row with a NaN in y has a NaN scale.
+ * dim in [1, 16384]; dim <= ldq <= 32768; tokens < 2^22. */
+mi_status mi_add_rms_norm(const void *x, int x_type, int64_t ldx, const void *residual, int res_type,
+                          int64_t ldr, const float *weight, float eps, void *y, int64_t ldy, int8_t *q,
+                          int64_t ldq, float *scale, void *res_out, int64_t ldro, int tokens, int dim,
+                          void *stream);
+
+/* Depthwise causal convolution over [batch,len,dim] rows of `type`:
+ *   y[b,t,c] = act(bias[c] + sum_j w[c,j] * x[b, t - width + 1 + j, c])
+ * w fp32 [dim,width], bias fp32 [dim] nullable; act = v / (1 + exp(-v)) for
+ * silu != 0, else none.  state_in / state_out [batch,width-1,dim] of `type`,
+ * nullable, may be the same: the inputs before the sequence, oldest first
+ * (NULL: zeros), and the last ones of state_in and the sequence together.
+ * lens int32 [batch] nullable: sequence b has lens[b] tokens (clamped to
+ * [0, len]); rows of x past them are not used, rows of y past them are zero.
+ * len == 0 copies the state.  width in [1, 8]; batch * dim < 2^31. */
+mi_status mi_causal_conv(const void *x, int64_t ldx, int64_t bsx, int type, const float *w, const float *bias,
+                         int width, int silu, const void *state_in, void *state_out, const int32_t *lens,
+                         void *y, int64_t ldy, int64_t bsy, int batch, int len, int dim, void *stream);
+
+/* Selective state space scan over [batch,len,dim] rows of `type`:
+ *   d = dt[b,t,c] + dt_bias[c];  d = log(1 + exp(d)) if dt_softplus != 0
+ *   h[c,n] = exp(d * a[c,n]) * h[c,n] + d * u[b,t,c] * B[b,t,g,n]
+ *   y[b,t,c] = sum_n C[b,t,g,n] * h[c,n] + d_skip[c] * u[b,t,c]
+ *   y[b,t,c] *= z[b,t,c] / (1 + exp(-z[b,t,c]))       (with z)
+ * with g = c / (dim / groups).  a fp32 [dim,nstate]; b, c rows of groups *
+ * nstate values of `type`; d_skip, dt_bias fp32 [dim], z: nullable; h_in /
+ * h_out fp32 [batch,dim,nstate] nullable (NULL h_in: zeros), may be the same.
+ * lens as for mi_causal_conv (h_out: the state after lens[b] tokens).
+ * workspace: 16-byte aligned, mi_selective_scan_workspace_size bytes (0: may
+ * be NULL).  nstate in [1, 256]; batch * dim <= 2^25. */
+mi_status mi_selective_scan_workspace_size(int batch, int len, int dim, int nstate, size_t *bytes);
+mi_status mi_selective_scan(const void *u, int64_t ldu, int64_t bsu, const void *dt, int64_t ldt, int64_t bst,
+                            const float *a, const void *b, int64_t ldb, int64_t bsb, const void *c,
+                            int64_t ldc, int64_t bsc, const float *d_skip, const void *z, int64_t ldz,
+                            int64_t bsz, const float *dt_bias, int dt_softplus, const float *h_in,
+                            float *h_out, const int32_t *lens, void *y, int64_t ldy, int64_t bsy, int type,
+                            int batch, int len, int dim, int nstate, int groups, void *workspace,
+                            size_t workspace_bytes, void *stream);
+
+/* Lays 4-bit weights out for mi_w4_matvec.  codes uint8 [n,k] in [0, 15];
+ * scales [n, ceil(k/group)] of scale_type (MI_F16 or MI_F32); zeros uint8 [n,
+ * ceil(k/group)], nullable (8 everywhere); weight = (code - zero) * scale.
+ * group: 32, 64 or a multiple of 128.  With nb = ceil(n/16), kb = ceil(k/128):
+ *   packed     nb * kb * 1024 bytes, 16-byte aligned: blocks of 16 rows x 128
+ *              columns; 32-bit word 4 (16 g + r) + j of a block holds columns
+ *              32 j + 8 g .. + 7 of row r, column c of the eight in bits
+ *              4 (c/2) (c even) or 16 + 4 (c/2) (c odd);
+ *   scales_out, zeros_out [nb, ng, 16] (ng = kb * 128 / group for group < 128,
+ *              else ceil(k/group)).  Rows and columns past the end are 0. */
+mi_status mi_pack_w4(const uint8_t *codes, const void *scales, int scale_type, const uint8_t *zeros,
+                     uint8_t *packed, void *scales_out, uint8_t *zeros_out, int n, int k, int group,
+                     void *stream);
+/* y[m,n] = bias[n] + sum_k x[m,k] * (code[n,k] - zero[n,k/group]) *
+ * scale[n,k/group]: x and y rows of `type`, weights as mi_pack_w4 lays them
+ * out (zeros NULL: 8), bias fp32 [n] nullable.  Made for the few rows of a
+ * decode step (m up to 64 read the weights once); any m is computed.  A row
+ * with an infinite x gives NaN where the product is infinite. */
+mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const uint8_t *packed, const void *scales,
+                       int scale_type, const uint8_t *zeros, const float *bias, void *y, int64_t ldy, int m,
+                       int n, int k, int group, void *stream);
+
 /* ------------------------------------------------ integer checkpoints */
 /* The integer parameters above in a versioned file (format 2, spec
  * mi-spec-2; format-1 files of mi-spec-1, whose SSD layers have no out_proj

@@ -16,11 +16,14 @@ LIB_PATH = os.environ.get("MAMBA_INT_LIB", os.path.join(PKG_ROOT, "libmamba_int.
 
 MI_OK, MI_ERR_NULL_POINTER, MI_ERR_BAD_DIM, MI_ERR_BAD_ALIGNMENT, MI_ERR_BAD_ARG, MI_ERR_HIP = range(6)
 OUT_INT32, OUT_INT8, OUT_DECAY_MOD, OUT_RESIDUAL, OUT_FLOAT = range(5)
+F32, BF16, F16 = range(3)        # mi_dtype
 
 P = ctypes.c_void_p
 I = ctypes.c_int
 I32 = ctypes.c_int32
 F = ctypes.c_float
+I64 = ctypes.c_int64
+SZ = ctypes.c_size_t
 
 # name -> argtypes, in the order of include/mamba_int.h
 SIGNATURES = {
@@ -60,6 +63,13 @@ SIGNATURES = {
     "mi_decode_workspace_size": [P, I, P],
     "mi_decode_step": [P, I, P, P, P, I, P, P, P, ctypes.c_size_t, P],
     "mi_decode_step_static": [P, I, P, P, P, I, P, P, P],
+    "mi_add_rms_norm": [P, I, I64, P, I, I64, P, F, P, I64, P, I64, P, P, I64, I, I, P],
+    "mi_causal_conv": [P, I64, I64, I, P, P, I, I, P, P, P, P, I64, I64, I, I, I, P],
+    "mi_selective_scan_workspace_size": [I, I, I, I, P],
+    "mi_selective_scan": [P, I64, I64, P, I64, I64, P, P, I64, I64, P, I64, I64, P, P, I64, I64, P, I, P, P, P,
+                          P, I64, I64, I, I, I, I, I, I, P, SZ, P],
+    "mi_pack_w4": [P, P, I, P, P, P, P, I, I, I, P],
+    "mi_w4_matvec": [P, I64, I, P, P, I, P, P, P, I64, I, I, I, I, P],
     "mi_checkpoint_open": [ctypes.c_char_p, P],
     "mi_checkpoint_get_info": [P, P],
     "mi_checkpoint_upload": [P, P, ctypes.c_size_t, P, P, I, P],
