@@ -21,32 +21,147 @@ struct ConvArgs {
     int width, silu, batch, len, dim;
 };
 
-template <class T>
-__device__ __forceinline__ int seq_len(const int32_t *lens, int64_t b, int len) {
-    return lens ? min(max(lens[b], 0), len) : len;
+// The rows [t0, t1) of V channels of a sequence: W - 1 rows before them, then a
+// step for each, kSteps rows loaded ahead.  FULL: V channels; else the channels
+// below a.dim, element by element.
+template <class T, int W, int V, bool FULL>
+__device__ __forceinline__ void conv_rows(const ConvArgs<T> &a, int64_t b, int c, int t0, int t1, int n) {
+    constexpr int kSteps = 4;
+    const int have = FULL ? V : a.dim - c;
+    auto load = [&](const T *p) {
+        Packed<T, V> v;
+        if (FULL) {
+            v = load_packed<V>(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v.v[i] = i < have ? p[i] : (T)0.0f;
+        }
+        return v;
+    };
+    auto store = [&](T *p, const Packed<T, V> &v) {
+        if (FULL) {
+            store_packed<V>(p, v);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < have) p[i] = v.v[i];
+    };
+    // row t of the sequence, the state in front of it
+    auto row = [&](int t) {
+        Packed<T, V> v;
+        if (t >= 0) {
+            v = load(a.x.row(b, t) + c);
+        } else if (a.state_in) {
+            v = load(a.state_in + (b * (W - 1) + (W - 1 + t)) * a.dim + c);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v.v[i] = (T)0.0f;
+        }
+        return v;
+    };
+    float w[W][V], bias[V], win[W][V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int ci = FULL ? c + i : min(c + i, a.dim - 1);
+        bias[i] = a.bias ? a.bias[ci] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[j][i] = a.w[(int64_t)ci * W + j];
+    }
+    const int end = min(t1, n);
+    Packed<T, V> next[kSteps];
+    if (t0 < end) {
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) {
+            const Packed<T, V> r = row(t0 - (W - 1) + j);
+#pragma unroll
+            for (int i = 0; i < V; ++i) win[j][i] = (float)r.v[i];
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) next[s] = row(min(t0 + s, end - 1));
+    }
+    if (t0 == 0 && a.state_out) {
+        // the thread that read state_in writes state_out, so the two may be one
+        Packed<T, V> last[W];
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) last[j] = row(n - (W - 1) + j);
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) store(a.state_out + (b * (W - 1) + j) * a.dim + c, last[j]);
+    }
+    for (int t = t0; t < end; t += kSteps) {
+        Packed<T, V> now[kSteps];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) now[s] = next[s];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) next[s] = load(a.x.row(b, min(t + kSteps + s, end - 1)) + c);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            Packed<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                win[W - 1][i] = (float)now[s].v[i];
+                float y = bias[i];
+#pragma unroll
+                for (int j = 0; j < W; ++j) y = __builtin_fmaf(w[j][i], win[j][i], y);
+                o.v[i] = (T)(a.silu ? silu(y) : y);
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) win[j][i] = win[j + 1][i];
+            }
+            if (t + s < end) store(a.y.row(b, t + s) + c, o);
+        }
+    }
+    Packed<T, V> none;
+#pragma unroll
+    for (int i = 0; i < V; ++i) none.v[i] = (T)0.0f;
+    for (int t = max(t0, n); t < t1; ++t) store(a.y.row(b, t) + c, none);
 }
 
-// One thread a (sequence, channel), step after step.
+// One thread V channels (16 bytes) of `steps` rows of a sequence.
+template <class T, int W>
+__global__ __launch_bounds__(256) void causal_conv_kernel(ConvArgs<T> a, int steps, int tiles, int64_t threads) {
+    constexpr int V = 16 / sizeof(T);
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= threads) return;
+    const int cols = (a.dim + V - 1) / V;
+    const int64_t tile = id / cols;
+    const int c = (int)(id - tile * cols) * V;
+    const int64_t b = tile / tiles;
+    const int t0 = (int)(tile - b * tiles) * steps, t1 = min(a.len, t0 + steps);
+    const int n = a.lens ? min(max(a.lens[b], 0), a.len) : a.len;
+    if (c + V <= a.dim)
+        conv_rows<T, W, V, true>(a, b, c, t0, t1, n);
+    else
+        conv_rows<T, W, V, false>(a, b, c, t0, t1, n);
+}
+
+template <class T, int W>
+mi_status launch_conv(const ConvArgs<T> &a, hipStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    const int64_t cols = (a.dim + V - 1) / V, rows = (int64_t)a.batch * cols;
+    // rows a thread: the W - 1 in front of them are read twice, so as many as leave
+    // four waves a SIMD
+    int steps = 32;
+    while (steps > 4 && rows * ((a.len + steps - 1) / steps) < (int64_t)device_cus() * 4 * 4 * 64) steps /= 2;
+    const int tiles = a.len > 0 ? (a.len + steps - 1) / steps : 1;
+    const int64_t threads = rows * tiles;
+    MI_REQUIRE(threads < ((int64_t)1 << 32) - 256, MI_ERR_BAD_DIM, "mi_causal_conv: batch * len * dim is too large");
+    hipLaunchKernelGGL((causal_conv_kernel<T, W>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a, steps,
+                       tiles, threads);
+    return MI_OK;
+}
+
 template <class T>
-__global__ __launch_bounds__(64) void causal_conv_kernel(ConvArgs<T> a) {
-    const int64_t id = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (id >= (int64_t)a.batch * a.dim) return;
-    const int64_t b = id / a.dim;
-    const int c = (int)(id - b * a.dim), W = a.width;
-    const int n = seq_len<T>(a.lens, b, a.len);
-    float win[kConvMaxWidth];
-    for (int j = 0; j < W - 1; ++j) win[j] = a.state_in ? (float)a.state_in[(b * (W - 1) + j) * a.dim + c] : 0.0f;
-    const float bias = a.bias ? a.bias[c] : 0.0f;
-    for (int t = 0; t < n; ++t) {
-        win[W - 1] = (float)a.x.row(b, t)[c];
-        float s = bias;
-        for (int j = 0; j < W; ++j) s = __builtin_fmaf(a.w[(int64_t)c * W + j], win[j], s);
-        a.y.row(b, t)[c] = (T)(a.silu ? silu(s) : s);
-        for (int j = 0; j < W - 1; ++j) win[j] = win[j + 1];
+mi_status launch_width(const ConvArgs<T> &a, hipStream_t st) {
+    switch (a.width) {
+        case 1: return launch_conv<T, 1>(a, st);
+        case 2: return launch_conv<T, 2>(a, st);
+        case 3: return launch_conv<T, 3>(a, st);
+        case 4: return launch_conv<T, 4>(a, st);
+        case 5: return launch_conv<T, 5>(a, st);
+        case 6: return launch_conv<T, 6>(a, st);
+        case 7: return launch_conv<T, 7>(a, st);
+        default: return launch_conv<T, 8>(a, st);
     }
-    for (int t = n; t < a.len; ++t) a.y.row(b, t)[c] = (T)0.0f;
-    if (a.state_out)
-        for (int j = 0; j < W - 1; ++j) a.state_out[(b * (W - 1) + j) * a.dim + c] = (T)win[j];
 }
 
 }  // namespace mi
@@ -67,13 +182,13 @@ extern "C" mi_status mi_causal_conv(const void *x, int64_t ldx, int64_t bsx, int
     if (batch == 0 || dim == 0) return MI_OK;
     MI_REQUIRE(w && (len == 0 || (x && y)), MI_ERR_NULL_POINTER, "mi_causal_conv: x, w and y are required");
     const hipStream_t st = as_stream(stream);
+    mi_status status = MI_OK;
     with_type(type, [&](auto t) {
         using T = decltype(t);
         const ConvArgs<T> a{{static_cast<const T *>(x), ldx, bsx}, w, bias, static_cast<const T *>(state_in),
                             static_cast<T *>(state_out), lens, {static_cast<T *>(y), ldy, bsy}, width, silu, batch, len,
                             dim};
-        const int64_t n = (int64_t)batch * dim;
-        hipLaunchKernelGGL(causal_conv_kernel<T>, dim3((unsigned)((n + 63) / 64)), dim3(64), 0, st, a);
+        status = launch_width(a, st);
     });
-    return check_launch("mi_causal_conv");
+    return status != MI_OK ? status : check_launch("mi_causal_conv");
 }

@@ -23,6 +23,21 @@ void with_type(int type, F &&f) {
         f(f16_t{});
 }
 
+// V elements with any alignment of the type's own (global memory takes wide loads
+// and stores at every element's address).
+template <class T, int V>
+struct __attribute__((packed)) Packed {
+    T v[V];
+};
+template <int V, class T>
+__device__ __forceinline__ Packed<T, V> load_packed(const T *p) {
+    return *reinterpret_cast<const Packed<T, V> *>(p);
+}
+template <int V, class T>
+__device__ __forceinline__ void store_packed(T *p, const Packed<T, V> &v) {
+    *reinterpret_cast<Packed<T, V> *>(p) = v;
+}
+
 // A tensor of rows [batch, len, dim]: the address of row (b, t).
 template <class T>
 struct Rows {

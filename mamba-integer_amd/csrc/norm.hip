@@ -48,61 +48,155 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *red) {
     return s;
 }
 
-// One block a row, one element a thread and step.
-template <class T, class R, int THREADS, int E>
-__global__ __launch_bounds__(THREADS) void add_rms_norm_kernel(NormArgs a) {
-    __shared__ float red_s[THREADS / 64];
-    __shared__ uint32_t red_m[THREADS / 64];
-    const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x;
+// The row's 8-bit values and their scale from max |y| (its bits): y * 127 / max
+// plus 1.5 * 2^23 has the value, rounded half to even, in its low byte.  (No clamp:
+// |y| <= max, so the product rounds to 127 at most.)
+struct NormQuant {
+    float mul, scale;
+    __device__ __forceinline__ explicit NormQuant(uint32_t bits) {
+        const float amax = __builtin_bit_cast(float, bits);
+        const float top = amax < 1e-8f ? 1e-8f : amax;
+        mul = __fdiv_rn(127.0f, top);
+        scale = __fdiv_rn(top, 127.0f);
+    }
+    __device__ __forceinline__ int8_t operator()(float y) const {
+        return (int8_t)__builtin_bit_cast(int32_t, __fadd_rn(__fmul_rn(y, mul), 12582912.0f));
+    }
+};
+
+// TPR threads a row, E times V adjacent elements each: every load is issued
+// before the sum.  Rows of V elements at least; the last V of a row whose width
+// V does not divide start at dim - V (elements of two threads are summed once and
+// stored twice with one value).
+template <class T, class R, int TPR, int E>
+__global__ __launch_bounds__(256) void add_rms_norm_kernel(NormArgs a) {
+    constexpr int V = 16 / sizeof(T);
+    __shared__ float red_s[TPR / 64];
+    __shared__ uint32_t red_m[TPR / 64];
+    const int64_t row = TPR == 64 ? (int64_t)blockIdx.x * 4 + wave_id() : (int64_t)blockIdx.x;
+    const int tid = TPR == 64 ? threadIdx.x & 63 : threadIdx.x;
+    if (row >= a.rows) return;
     const T *x = static_cast<const T *>(a.x) + row * a.ldx;
-    const R *res = a.res ? static_cast<const R *>(a.res) + row * a.ldr : nullptr;
-    float v[E], ss = 0.0f;
+    const int dim = a.dim;
+    int at[E];
+    Packed<T, V> xv[E];
+    Packed<R, V> rv[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-        const int i = tid + j * THREADS;
-        v[j] = 0.0f;
-        if (i < a.dim) {
-            v[j] = (float)x[i];
-            if (res) v[j] = (float)res[i] + v[j];
-            ss += v[j] * v[j];
+        at[j] = min((tid + j * TPR) * V, dim - V);
+        xv[j] = load_packed<V>(x + at[j]);
+    }
+    if (a.res) {
+        const R *res = static_cast<const R *>(a.res) + row * a.ldr;
+#pragma unroll
+        for (int j = 0; j < E; ++j) rv[j] = load_packed<V>(res + at[j]);
+    }
+    float v[E][V], ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        const int first = (tid + j * TPR) * V;   // elements below it belong to another thread
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[j][i] = (float)xv[j].v[i];
+            if (a.res) v[j][i] += (float)rv[j].v[i];
+            ss += at[j] + i >= first ? v[j][i] * v[j][i] : 0.0f;
         }
     }
-    const float inv = 1.0f / sqrtf(block_sum<THREADS>(ss, red_s) / (float)a.dim + a.eps);
+    const float inv = 1.0f / sqrtf(block_sum<TPR>(ss, red_s) / (float)dim + a.eps);
     uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-        const int i = tid + j * THREADS;
-        if (i >= a.dim) break;
-        if (a.res_out) static_cast<R *>(a.res_out)[row * a.ldro + i] = (R)v[j];
-        v[j] = v[j] * inv * a.w[i];
-        if (a.y) static_cast<T *>(a.y)[row * a.ldy + i] = (T)v[j];
-        m = max(m, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
+        if ((tid + j * TPR) * V >= dim) break;
+        if (a.res_out) {
+            Packed<R, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = (R)v[j][i];
+            store_packed<V>(static_cast<R *>(a.res_out) + row * a.ldro + at[j], o);
+        }
+        const Packed<float, V> w = load_packed<V>(a.w + at[j]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[j][i] = v[j][i] * inv * w.v[i];
+            m = max(m, __builtin_bit_cast(uint32_t, v[j][i]) & 0x7fffffffu);
+        }
+        if (a.y) {
+            Packed<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = (T)v[j][i];
+            store_packed<V>(static_cast<T *>(a.y) + row * a.ldy + at[j], o);
+        }
     }
     if (!a.q) return;
-    m = block_max<THREADS>(m, red_m);
-    const float amax = __builtin_bit_cast(float, m);
-    const float top = amax < 1e-8f ? 1e-8f : amax;
-    const float mul = 127.0f / top;
+    const NormQuant quant(block_max<TPR>(m, red_m));
+    int8_t *q = a.q + row * a.ldq;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-        const int i = tid + j * THREADS;
-        if (i < a.dim)
-            a.q[row * a.ldq + i] = (int8_t)fminf(fmaxf(rintf(v[j] * mul), -127.0f), 127.0f);
-        else if (i < a.ldq)
-            a.q[row * a.ldq + i] = 0;
+        if ((tid + j * TPR) * V >= dim) break;
+        Packed<int8_t, V> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o.v[i] = quant(v[j][i]);
+        store_packed<V>(q + at[j], o);
     }
-    for (int64_t i = tid + E * THREADS; i < a.ldq; i += THREADS) a.q[row * a.ldq + i] = 0;
-    if (tid == 0) a.scale[row] = top / 127.0f;
+    for (int64_t i = dim + tid; i < a.ldq; i += TPR) q[i] = 0;
+    if (tid == 0) a.scale[row] = quant.scale;
 }
 
+// Rows narrower than one thread's vector: one thread a row.
+template <class T, class R>
+__global__ __launch_bounds__(64) void add_rms_norm_narrow_kernel(NormArgs a) {
+    const int64_t row = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    if (row >= a.rows) return;
+    float v[8], ss = 0.0f;
+    for (int i = 0; i < a.dim; ++i) {
+        v[i] = (float)static_cast<const T *>(a.x)[row * a.ldx + i];
+        if (a.res) v[i] += (float)static_cast<const R *>(a.res)[row * a.ldr + i];
+        ss += v[i] * v[i];
+    }
+    const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+    uint32_t m = 0;
+    for (int i = 0; i < a.dim; ++i) {
+        if (a.res_out) static_cast<R *>(a.res_out)[row * a.ldro + i] = (R)v[i];
+        v[i] = v[i] * inv * a.w[i];
+        m = max(m, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+        if (a.y) static_cast<T *>(a.y)[row * a.ldy + i] = (T)v[i];
+    }
+    if (!a.q) return;
+    const NormQuant quant(m);
+    for (int64_t i = 0; i < a.ldq; ++i) a.q[row * a.ldq + i] = i < a.dim ? quant(v[i]) : (int8_t)0;
+    a.scale[row] = quant.scale;
+}
+
+template <class T, class R, int TPR, int E>
+void launch_rows(const NormArgs &a, hipStream_t st) {
+    const int64_t blocks = TPR == 64 ? (a.rows + 3) / 4 : a.rows;
+    hipLaunchKernelGGL((add_rms_norm_kernel<T, R, TPR, E>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+}
+
+// A wave a row while a lane holds at most 32 elements, then a block a row.
 template <class T, class R>
 void launch_add_rms_norm(const NormArgs &a, hipStream_t st) {
-    const dim3 grid((unsigned)a.rows);
-    if (a.dim <= 2048)
-        hipLaunchKernelGGL((add_rms_norm_kernel<T, R, 256, 8>), grid, dim3(256), 0, st, a);
+    constexpr int V = 16 / sizeof(T);
+    const int e = (a.dim + 64 * V - 1) / (64 * V);
+    if (a.dim < V)
+        hipLaunchKernelGGL((add_rms_norm_narrow_kernel<T, R>), dim3((unsigned)((a.rows + 63) / 64)), dim3(64), 0, st, a);
+    else if (e <= 1)
+        launch_rows<T, R, 64, 1>(a, st);
+    else if (e <= 2)
+        launch_rows<T, R, 64, 2>(a, st);
+    else if (e <= 3)
+        launch_rows<T, R, 64, 3>(a, st);
+    else if (e <= 4)
+        launch_rows<T, R, 64, 4>(a, st);
+    else if (V == 4 && e <= 8)
+        launch_rows<T, R, 64, 8>(a, st);
+    else if (e <= 8)
+        launch_rows<T, R, 256, 2>(a, st);
+    else if (e <= 16)
+        launch_rows<T, R, 256, 4>(a, st);
+    else if (e <= 32)
+        launch_rows<T, R, 256, 8>(a, st);
     else
-        hipLaunchKernelGGL((add_rms_norm_kernel<T, R, 1024, 16>), grid, dim3(1024), 0, st, a);
+        launch_rows<T, R, 256, 16>(a, st);
 }
 
 }  // namespace mi

@@ -35,57 +35,79 @@ __device__ __forceinline__ float softplus(float v) {
     return v > 0.0f ? v + s : (v <= 0.0f ? s : v);
 }
 
-// LANES lanes of a wave hold a channel, four states each; step after step.
-template <class T, int LANES>
+// LANES lanes of a wave hold a channel, four states each (adjacent: 16-byte loads
+// of the state, of A and of B and C's rows where N % 4 == 0); step after step.
+template <class T, int LANES, bool QUADS>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs<T> a) {
-    const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
-    const int lane = threadIdx.x % LANES;
-    const int64_t all = (int64_t)a.batch * a.dim;
+    const uint32_t id = (blockIdx.x * 256 + threadIdx.x) / LANES, all = (uint32_t)a.batch * (uint32_t)a.dim;
+    const int lane = threadIdx.x % LANES, N = a.nstate, n0 = 4 * lane;
     const bool on = id < all;
-    const int64_t ch = on ? id : all - 1;
-    const int64_t b = ch / a.dim;
-    const int c = (int)(ch - b * a.dim), N = a.nstate;
-    const int g = c / (a.dim / a.groups);
+    const uint32_t ch = on ? id : all - 1;
+    const uint32_t b = ch / (uint32_t)a.dim;
+    const int c = (int)(ch - b * (uint32_t)a.dim);
+    const int64_t g0 = (int64_t)(c / (a.dim / a.groups)) * N + n0;
     const int len = scan_len(a.lens, b, a.len);
-    float h[4], am[4];
+    // four values from p on, those of states past N as zero
+    auto four = [&](auto *p, float (&o)[4]) {
+        if (QUADS) {
+            if (n0 < N) {
+                const auto v = load_packed<4>(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int n = 4 * lane + i;
-        am[i] = n < N ? a.a[(int64_t)c * N + n] : 0.0f;
-        h[i] = a.h_in && n < N ? a.h_in[ch * N + n] : 0.0f;
-    }
+                for (int i = 0; i < 4; ++i) o[i] = (float)v.v[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n0 + i < N) o[i] = (float)p[i];
+        }
+    };
+    float h[4] = {}, am[4] = {};
+    four(a.a + (int64_t)c * N + n0, am);
+    if (a.h_in) four(a.h_in + (int64_t)ch * N + n0, h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) am[i] *= 1.44269504f;
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.0f, skip = a.d_skip ? a.d_skip[c] : 0.0f;
     for (int t = 0; t < len; ++t) {
+        float bn[4] = {}, cn[4] = {};
+        four(a.b.row(b, t) + g0, bn);
+        four(a.c.row(b, t) + g0, cn);
+        const float u = (float)a.u.row(b, t)[c];
         float dt = (float)a.dt.row(b, t)[c] + bias;
         if (a.softplus) dt = softplus(dt);
-        const float u = (float)a.u.row(b, t)[c];
+        const float du = dt * u;
         float y = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int n = 4 * lane + i;
-            if (n < N) {
-                const float bn = (float)a.b.row(b, t)[(int64_t)g * N + n], cn = (float)a.c.row(b, t)[(int64_t)g * N + n];
-                h[i] = expf(dt * am[i]) * h[i] + dt * u * bn;
-                y += cn * h[i];
-            }
+            h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * am[i]), h[i], du * bn[i]);
+            if (n0 + i < N) y = __builtin_fmaf(cn[i], h[i], y);
         }
+#pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) y += __shfl_xor(y, o);
-        y += skip * u;
+        y = __builtin_fmaf(skip, u, y);
         if (a.z.p) y *= silu((float)a.z.row(b, t)[c]);
         if (on && lane == 0) a.y.row(b, t)[c] = (T)y;
     }
     if (!on) return;
     if (lane == 0)
         for (int t = len; t < a.len; ++t) a.y.row(b, t)[c] = (T)0.0f;
-    if (a.h_out)
+    if (!a.h_out) return;
+    float *h_out = a.h_out + (int64_t)ch * N + n0;
+    if (QUADS) {
+        if (n0 < N) store_packed<4>(h_out, Packed<float, 4>{{h[0], h[1], h[2], h[3]}});
+    } else {
+#pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (4 * lane + i < N) a.h_out[ch * N + 4 * lane + i] = h[i];
+            if (n0 + i < N) h_out[i] = h[i];
+    }
 }
 
 template <class T, int LANES>
 void launch_scan_step(const ScanArgs<T> &a, hipStream_t st) {
-    const int64_t n = (int64_t)a.batch * a.dim * LANES;
-    hipLaunchKernelGGL((scan_step_kernel<T, LANES>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)(((int64_t)a.batch * a.dim * LANES + 255) / 256));
+    if (a.nstate % 4 == 0)
+        hipLaunchKernelGGL((scan_step_kernel<T, LANES, true>), grid, dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((scan_step_kernel<T, LANES, false>), grid, dim3(256), 0, st, a);
 }
 
 template <class T>

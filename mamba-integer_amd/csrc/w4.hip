@@ -55,24 +55,148 @@ struct W4Args {
     int m, n, k, group, ng;
 };
 
-// One thread an output.
-template <class T, class S>
-__global__ __launch_bounds__(64) void w4_kernel(W4Args<T, S> a) {
-    const int64_t id = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (id >= (int64_t)a.m * a.n) return;
-    const int64_t m = id / a.n;
-    const int n = (int)(id - m * a.n), r = n % kW4Rows;
-    const int64_t nb = n / kW4Rows;
-    const int kb = (a.k + kW4Cols - 1) / kW4Cols;
-    float acc = 0.0f;
-    for (int k = 0; k < a.k; ++k) {
-        const int in = k % kW4Cols, c = in & 7;
-        const uint32_t w = a.packed[(nb * kb + k / kW4Cols) * 256 + 4 * (16 * ((in & 31) >> 3) + r) + (in >> 5)];
-        const int64_t at = (nb * a.ng + k / a.group) * kW4Rows + r;
-        const int zero = a.zeros ? a.zeros[at] : 8;
-        acc += (float)a.x[m * a.ldx + k] * ((float)((int)((w >> w4_shift(c)) & 15) - zero) * (float)a.scales[at]);
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef bf16_t v8b __attribute__((ext_vector_type(8)));
+typedef f16_t v8h __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ v4f mfma(v8b a, v8b b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// Operands of the matrix instruction by the type of x.  A weight enters as 16 + q,
+// exact in 16 bits and built by a shift and a bit select for two of them (q are the
+// top bits of the mantissa of 2^4); 16 + zero times the row's sum of x is taken off
+// after the product.  float32 rows enter as three bf16 parts whose sum is the value.
+template <class T>
+struct W4Type;
+template <>
+struct W4Type<bf16_t> {
+    typedef v8b Vec;
+    static constexpr int kParts = 1;
+    static __device__ __forceinline__ Vec weights(uint32_t w) {
+        const v4u r = {((w << 3) & 0x00780078u) | 0x41804180u, ((w >> 1) & 0x00780078u) | 0x41804180u,
+                       ((w >> 5) & 0x00780078u) | 0x41804180u, ((w >> 9) & 0x00780078u) | 0x41804180u};
+        return __builtin_bit_cast(Vec, r);
     }
-    a.y[m * a.ldy + n] = (T)(acc + (a.bias ? a.bias[n] : 0.0f));
+    static __device__ __forceinline__ void split(const Packed<bf16_t, 8> &x, Vec (&o)[1]) {
+        o[0] = __builtin_bit_cast(Vec, x);
+    }
+};
+template <>
+struct W4Type<f16_t> {
+    typedef v8h Vec;
+    static constexpr int kParts = 1;
+    static __device__ __forceinline__ Vec weights(uint32_t w) {
+        const v4u r = {((w << 6) & 0x03c003c0u) | 0x4c004c00u, ((w << 2) & 0x03c003c0u) | 0x4c004c00u,
+                       ((w >> 2) & 0x03c003c0u) | 0x4c004c00u, ((w >> 6) & 0x03c003c0u) | 0x4c004c00u};
+        return __builtin_bit_cast(Vec, r);
+    }
+    static __device__ __forceinline__ void split(const Packed<f16_t, 8> &x, Vec (&o)[1]) {
+        o[0] = __builtin_bit_cast(Vec, x);
+    }
+};
+template <>
+struct W4Type<float> {
+    typedef v8b Vec;
+    static constexpr int kParts = 3;
+    static __device__ __forceinline__ Vec weights(uint32_t w) { return W4Type<bf16_t>::weights(w); }
+    // each part the leading 8 bits of what the ones before it leave (cut off, not
+    // rounded: no part overflows, and the third holds the rest exactly)
+    static __device__ __forceinline__ void split(const Packed<float, 8> &x, Vec (&o)[3]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float v = x.v[i];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                const uint32_t top = __builtin_bit_cast(uint32_t, v) >> 16;
+                o[p][i] = __builtin_bit_cast(bf16_t, (uint16_t)top);
+                v -= __builtin_bit_cast(float, top << 16);
+            }
+        }
+    }
+};
+
+// A block: KS waves, 16 weight rows, MT x 16 rows of x; wave w takes the column
+// blocks w, w + KS, ...  In the matrix instruction x is operand A (lane: row l & 15,
+// columns 8 (l >> 4) .. + 7 of 32) and the weights B (lane: weight row l & 15), so a
+// lane's results belong to one weight row and its scale.
+template <class T, class S, int MT, int KS>
+__global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
+    using W = W4Type<T>;
+    using Vec = typename W::Vec;
+    constexpr int P = W::kParts;
+    __shared__ v4f part[KS][MT][64];
+    const int wave = wave_id(), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int64_t nb = blockIdx.x;
+    const int m0 = blockIdx.y * 16 * MT, kb_all = (a.k + kW4Cols - 1) / kW4Cols;
+    const v4u *words = reinterpret_cast<const v4u *>(a.packed) + nb * kb_all * 64 + lane;
+    const S *scales = a.scales + nb * a.ng * kW4Rows + r;
+    const uint8_t *zeros = a.zeros ? a.zeros + nb * a.ng * kW4Rows + r : nullptr;
+    const Vec ones = W::weights(0);   // 16 in every place
+    v4f acc[MT] = {};
+    for (int kb = wave; kb < kb_all; kb += KS) {
+        const v4u w = words[(int64_t)kb * 64];
+        v4f d[MT], s16[MT];   // sums of x (16 + q) and of 16 x of the group so far
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = kb * kW4Cols + 32 * j;
+            const bool first = a.group == 32 || j == 0 || (a.group == 64 && j == 2);
+            const Vec wj = W::weights(w[j]);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const int m = m0 + 16 * mt + r, k0 = k + 8 * g;
+                Packed<T, 8> xv;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) xv.v[i] = (T)0.0f;
+                if (m < a.m) {
+                    const T *x = a.x + (int64_t)m * a.ldx + k0;
+                    if (k0 + 8 <= a.k) {
+                        xv = load_packed<8>(x);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (k0 + i < a.k) xv.v[i] = x[i];
+                    }
+                }
+                Vec parts[P];
+                W::split(xv, parts);
+                if (first) d[mt] = s16[mt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int p = P - 1; p >= 0; --p) {
+                    d[mt] = mfma(parts[p], wj, d[mt]);
+                    s16[mt] = mfma(parts[p], ones, s16[mt]);
+                }
+            }
+            const bool last = a.group == 32 || j == 3 || (a.group == 64 && j == 1);
+            if (last) {
+                const int64_t at = (int64_t)(k / a.group) * kW4Rows;
+                const float s = (float)scales[at], z = 1.0f + 0.0625f * (zeros ? (float)zeros[at] : 8.0f);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) acc[mt] += s * (d[mt] - z * s16[mt]);
+            }
+        }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) part[wave][mt][lane] = acc[mt];
+    __syncthreads();
+    const int n = (int)nb * kW4Rows + r;
+    for (int mt = wave; mt < MT; mt += KS) {
+        v4f sum = part[0][mt][lane];
+#pragma unroll
+        for (int w = 1; w < KS; ++w) sum += part[w][mt][lane];
+        const float bias = a.bias && n < a.n ? a.bias[n] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int m = m0 + 16 * mt + 4 * g + i;
+            if (m < a.m && n < a.n) a.y[(int64_t)m * a.ldy + n] = (T)(sum[i] + bias);
+        }
+    }
+}
+
+template <class T, class S, int MT>
+void launch_w4(const W4Args<T, S> &a, hipStream_t st) {
+    const dim3 grid((unsigned)((a.n + kW4Rows - 1) / kW4Rows), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
+    hipLaunchKernelGGL((w4_kernel<T, S, MT, 4>), grid, dim3(256), 0, st, a);
 }
 
 // Groups of one packed row block: whole column blocks of them.
@@ -129,7 +253,8 @@ extern "C" mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const ui
     if (m == 0 || n == 0) return MI_OK;
     MI_REQUIRE(x && packed && scales && y, MI_ERR_NULL_POINTER, "mi_w4_matvec: x, packed, scales and y are required");
     MI_REQUIRE(aligned(packed, 16), MI_ERR_BAD_ALIGNMENT, "mi_w4_matvec: packed must be 16-byte aligned");
-    MI_REQUIRE((int64_t)m * n < ((int64_t)1 << 31), MI_ERR_BAD_DIM, "mi_w4_matvec: m * n must be below 2^31");
+    MI_REQUIRE((int64_t)m * n < ((int64_t)1 << 31) && m <= 64 * 65535, MI_ERR_BAD_DIM,
+               "mi_w4_matvec: m * n must be below 2^31, and m at most 64 * 65535");
     const hipStream_t st = as_stream(stream);
     with_type(type, [&](auto t) {
         using T = decltype(t);
@@ -138,7 +263,12 @@ extern "C" mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const ui
             const W4Args<T, S> a{static_cast<const T *>(x), ldx, reinterpret_cast<const uint32_t *>(packed),
                                  static_cast<const S *>(scales), zeros, bias, static_cast<T *>(y), ldy, m, n, k, group,
                                  w4_groups(k, group)};
-            hipLaunchKernelGGL((w4_kernel<T, S>), dim3((unsigned)(((int64_t)m * n + 63) / 64)), dim3(64), 0, st, a);
+            if (m <= 16)
+                launch_w4<T, S, 1>(a, st);
+            else if (m <= 32)
+                launch_w4<T, S, 2>(a, st);
+            else
+                launch_w4<T, S, 4>(a, st);
         };
         if (scale_type == MI_F32)
             go(float{});
