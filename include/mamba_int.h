@@ -561,7 +561,8 @@ mi_status mi_causal_conv(const void *x, int64_t ldx, int64_t bsx, int type, cons
  * lens as for mi_causal_conv (h_out: the state after lens[b] tokens).
  * workspace: 16-byte aligned, mi_selective_scan_workspace_size bytes (0: may
  * be NULL).  nstate in [1, 256]; batch * dim <= 2^25. */
-mi_status mi_selective_scan_workspace_size(int batch, int len, int dim, int nstate, size_t *bytes);
+mi_status mi_selective_scan_workspace_size(int batch, int len, int dim, int nstate, int groups,
+                                           size_t *bytes);
 mi_status mi_selective_scan(const void *u, int64_t ldu, int64_t bsu, const void *dt, int64_t ldt, int64_t bst,
                             const float *a, const void *b, int64_t ldb, int64_t bsb, const void *c,
                             int64_t ldc, int64_t bsc, const float *d_skip, const void *z, int64_t ldz,

@@ -65,7 +65,7 @@ SIGNATURES = {
     "mi_decode_step_static": [P, I, P, P, P, I, P, P, P],
     "mi_add_rms_norm": [P, I, I64, P, I, I64, P, F, P, I64, P, I64, P, P, I64, I, I, P],
     "mi_causal_conv": [P, I64, I64, I, P, P, I, I, P, P, P, P, I64, I64, I, I, I, P],
-    "mi_selective_scan_workspace_size": [I, I, I, I, P],
+    "mi_selective_scan_workspace_size": [I, I, I, I, I, P],
     "mi_selective_scan": [P, I64, I64, P, I64, I64, P, P, I64, I64, P, I64, I64, P, P, I64, I64, P, I, P, P, P,
                           P, I64, I64, I, I, I, I, I, I, P, SZ, P],
     "mi_pack_w4": [P, P, I, P, P, P, P, I, I, I, P],

@@ -608,9 +608,9 @@ def causal_conv(x, weight, bias=None, activation: Optional[str] = "silu", state_
 
 
 @functools.lru_cache(maxsize=256)
-def _scan_workspace(B: int, L: int, D: int, N: int) -> int:
+def _scan_workspace(B: int, L: int, D: int, N: int, G: int) -> int:
     n = ctypes.c_size_t()
-    _lib.call("mi_selective_scan_workspace_size", B, L, D, N, ctypes.byref(n))
+    _lib.call("mi_selective_scan_workspace_size", B, L, D, N, G, ctypes.byref(n))
     return n.value
 
 
@@ -644,7 +644,7 @@ def selective_scan(u, dt, a, b, c, d_skip=None, z=None, dt_bias=None, dt_softplu
         rows.append(_rows(t, (B, L, G * N), typ, name))
     y = out if out is not None else torch.empty(shape, dtype=typ, device=u.device)
     st = (B, D, N)
-    size = _scan_workspace(B, L, D, N)
+    size = _scan_workspace(B, L, D, N, G)
     ws = torch.empty(size, dtype=torch.uint8, device=u.device).data_ptr() if size else None
     _lib.call("mi_selective_scan", *_rows(u, shape, typ, "u"), *_rows(dt, shape, typ, "dt"),
               _vec(a, (D, N), torch.float32, "a"), *rows[0], *rows[1], _vec(d_skip, (D,), torch.float32, "d_skip"),

@@ -71,11 +71,11 @@ def test_zero_sizes_are_noops():
 def test_workspace_size():
     from mamba_int import _lib
     n = ctypes.c_size_t(99)
-    assert _lib.raw("mi_selective_scan_workspace_size", 1, 1, 64, 16, ctypes.byref(n)) == 0 and n.value == 0
-    assert _lib.raw("mi_selective_scan_workspace_size", 1, 1, 64, 0, ctypes.byref(n)) == 2
-    assert _lib.raw("mi_selective_scan_workspace_size", 1, 1, 64, 16, None) == 1
+    assert _lib.raw("mi_selective_scan_workspace_size", 1, 1, 64, 16, 1, ctypes.byref(n)) == 0 and n.value == 0
+    assert _lib.raw("mi_selective_scan_workspace_size", 1, 1, 64, 0, 1, ctypes.byref(n)) == 2
+    assert _lib.raw("mi_selective_scan_workspace_size", 1, 1, 64, 16, 1, None) == 1
     # a call that needs a workspace is refused without one
-    assert _lib.raw("mi_selective_scan_workspace_size", 1, 65536, 64, 16, ctypes.byref(n)) == 0
+    assert _lib.raw("mi_selective_scan_workspace_size", 1, 65536, 64, 16, 1, ctypes.byref(n)) == 0
     if n.value:
         assert _lib.raw(*scan(L=65536, D=64, ldy=64, ld=64)) == 4
         assert "workspace" in _lib.last_error()
