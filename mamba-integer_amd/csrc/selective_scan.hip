@@ -12,7 +12,8 @@
 
 namespace mi {
 
-constexpr int kScanMaxStates = 256;
+constexpr int kScanMaxStates = 256, kScanStepLen = 4;
+constexpr int64_t kScanMaxLd = (int64_t)1 << 25;   // 16 rows' offsets in 32 bits
 
 template <class T>
 struct ScanArgs {
@@ -116,22 +117,48 @@ void launch_scan_step(const ScanArgs<T> &a, hipStream_t st) {
 // ------------------------------------------------------------- prompts
 // A block holds 64 channels of a sequence (a lane each) and NW * S states (S a
 // wave), and walks the steps in tiles of TT.  Per state and step: the decay's
-// product, its exponential, its product with h, and two matrix instructions of
-// 4 x 1 by 1 x 4 in 16 blocks (block = four channels): one adds the outer product
-// of four states' B with the channels' d * u to four states, one adds C * h of a
-// state to the channels' y.  They take their B and C from any one lane group of a
-// register (cbsz 4, abid), so a register holds 64 values of B, or 16 of C, and no
-// lane moves a value to another.  (The other three rows of y's product are not
-// used: a row of its own for each of four steps would carry a NaN of a later step
-// into an earlier one.)
+// product, its exponential (two issue slots), d u B, the multiply-add of h and that
+// of y.  B and C are the same for all lanes: a register holds 16 of their values in
+// each row of 16 lanes, and the multiplications read one of them by a DPP row
+// broadcast, so they cost no instruction, no LDS and no scalar load of their own.
+// (Both products on 4x4x1 matrix instructions, with the same broadcast by cbsz and
+// abid: one takes 9 to 12 issue cycles and blocks the SIMD meanwhile, a
+// multiply-add 4; 8 x 2048 x 1536 x 16 took 319 us.)
 //
 // The decays are kept in log2: d is softplus in units of log 2, so exp(d a) is one
 // exp2 of the product with a as it is.
-typedef float v4f __attribute__((ext_vector_type(4)));
+template <int LANE>
+__device__ __forceinline__ float bcast(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + LANE, 0xf, 0xf, true));
+}
 
-template <int ABID>
-__device__ __forceinline__ v4f outer(float a, float b, v4f c) {
-    return __builtin_amdgcn_mfma_f32_4x4x1f32(a, b, c, 4, ABID, 0);
+// One step of four states: p = a * next (the next step's exponents), h = e * h + x,
+// y += C * h with C in lanes LANE .. + 3 of every row of c.  In assembly, since the
+// compiler does not fold a broadcast into a multiply-add.  The four products in
+// front are the wait states that a broadcast of a register just written, and the
+// use of an exponential just taken, ask for.
+template <int LANE>
+__device__ __forceinline__ void scan_quad(const float (&a)[4], float next, const float (&e)[4], float (&x)[4], float c,
+                                          float (&p)[4], float (&h)[4], float &y) {
+    asm("v_mul_f32 %0, %9, %13\n\tv_mul_f32 %1, %10, %13\n\tv_mul_f32 %2, %11, %13\n\tv_mul_f32 %3, %12, %13\n\t"
+        "v_fmac_f32 %4, %14, %18\n\tv_fmac_f32 %5, %15, %19\n\tv_fmac_f32 %6, %16, %20\n\tv_fmac_f32 %7, %17, %21\n\t"
+        "v_fmac_f32_dpp %8, %22, %4 row_newbcast:%23 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %8, %22, %5 row_newbcast:%24 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %8, %22, %6 row_newbcast:%25 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %8, %22, %7 row_newbcast:%26 row_mask:0xf bank_mask:0xf"
+        : "=&v"(p[0]), "=&v"(p[1]), "=&v"(p[2]), "=&v"(p[3]), "+&v"(x[0]), "+&v"(x[1]), "+&v"(x[2]), "+&v"(x[3]), "+&v"(y)
+        : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(next), "v"(e[0]), "v"(e[1]), "v"(e[2]), "v"(e[3]), "v"(h[0]),
+          "v"(h[1]), "v"(h[2]), "v"(h[3]), "v"(c), "n"(LANE), "n"(LANE + 1), "n"(LANE + 2), "n"(LANE + 3));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = x[i];
+}
+
+// A barrier for what the block shares through LDS: __syncthreads would also wait for
+// the next tile's loads.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 // Calls f with integral_constant 0 .. N - 1.
@@ -157,169 +184,232 @@ struct ScanSplit {
 
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f, kMaxFloat = 3.402823466e38f;
 
+// kHelpers waves of a block turn rows into a tile's d, d u, B and C in LDS and the
+// recurring waves' parts of y into output rows, one tile ahead and one behind.
+constexpr int kHelpers = 4;
+
 template <class T, int S, int NW, int TT, int PASS>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
-    constexpr int kRows = TT / NW;               // of a tile, a wave's share
-    constexpr int kB = TT * S / 64, kC = TT * S / 16;
-    static_assert(kRows * NW == TT && kB * 64 == TT * S, "tile");
-    constexpr bool kShare = NW > 1, kY = PASS != kEnds;
-    __shared__ float2 steps[kShare ? TT : 1][64];
-    __shared__ float parts[kShare && kY ? NW : 1][kShare && kY ? TT : 1][64];
-    const int wave = NW > 1 ? wave_id() : 0, lane = threadIdx.x & 63;
+__global__ __launch_bounds__(64 * (NW + kHelpers)) __attribute__((amdgpu_waves_per_eu(S <= 8 ? 4 : 2))) void
+scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
+    constexpr bool kY = PASS != kEnds;
+    constexpr int kStates = S * NW, kRows = TT / kHelpers;     // a helper wave's rows of a tile
+    constexpr int kBC = TT * S / 16;                           // registers of B, and of C, of a tile
+    constexpr int kLoadBC = (TT * kStates + 64 * kHelpers - 1) / (64 * kHelpers);
+    static_assert(kRows * kHelpers == TT && kBC * 16 == TT * S, "tile");
+    __shared__ float2 steps[2][TT][64];                        // d, d u
+    __shared__ float parts[2][kY ? NW : 1][kY ? TT : 1][64];
+    __shared__ float bs[2][TT * kStates], cs[2][kY ? TT * kStates : 1];
+    const int wave = wave_id(), lane = threadIdx.x & 63;
     const int group_dim = a.dim / a.groups, N = a.nstate;
     const int64_t b = blockIdx.x / (a.groups * sp.blocks);
     const int rest = blockIdx.x % (a.groups * sp.blocks), g = rest / sp.blocks;
     const int in_group = rest % sp.blocks * 64 + lane;
     const bool on = in_group < group_dim;
     const int c = g * group_dim + min(in_group, group_dim - 1);
-    const int n0 = wave * S, k = PASS == kWhole ? 0 : blockIdx.y;
+    const int k = PASS == kWhole ? 0 : blockIdx.y;
     const int len = scan_len(a.lens, b, a.len);
     const int from = k * sp.chunk, to = PASS == kWhole ? a.len : min(a.len, from + sp.chunk);
-    const int end = min(to, len);                // steps of this part that are computed
+    const int end = min(to, len);                              // steps of this part that are computed
 
-    float am[S];
-    v4f h[S / 4];
+    if (wave < NW) {
+        // ---- the recurrence: the states n0 .. + S - 1
+        const int n0 = wave * S;
+        float am[S / 4][4], h[S / 4][4];
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-        const int n = n0 + i;
-        float v = n < N ? a.a[(int64_t)c * N + n] : 0.0f;
-        am[i] = v < -kMaxFloat ? -kMaxFloat : v;  // (a step of 0 then keeps the state whatever a is)
-        h[i / 4][i % 4] = PASS != kEnds && a.h_in && n < N ? a.h_in[(b * a.dim + c) * N + n] : 0.0f;
-    }
-    if (PASS == kParts) {
-        const float *e = sp.ends + b * sp.chunks * (N + 1) * a.dim + c;
-        for (int j = 0; j < k; ++j, e += (int64_t)(N + 1) * a.dim) {
-            const float sum = e[(int64_t)N * a.dim];
+        for (int i = 0; i < S; ++i) {
+            const int n = n0 + i;
+            float v = n < N ? a.a[(int64_t)c * N + n] : 0.0f;
+            am[i / 4][i % 4] = v < -kMaxFloat ? -kMaxFloat : v;  // (a step of 0 then keeps the state whatever a is)
+            h[i / 4][i % 4] = PASS != kEnds && a.h_in && n < N ? a.h_in[(b * a.dim + c) * N + n] : 0.0f;
+        }
+        if (PASS == kParts) {
+            const float *e = sp.ends + b * sp.chunks * (N + 1) * a.dim + c;
+            for (int j = 0; j < k; ++j, e += (int64_t)(N + 1) * a.dim) {
+                const float sum = e[(int64_t)N * a.dim];
 #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const float last = n0 + i < N ? e[(int64_t)(n0 + i) * a.dim] : 0.0f, was = h[i / 4][i % 4];
-                h[i / 4][i % 4] = was != 0.0f ? __builtin_fmaf(__builtin_amdgcn_exp2f(am[i] * sum), was, last) : last;
+                for (int i = 0; i < S; ++i) {
+                    const float last = n0 + i < N ? e[(int64_t)(n0 + i) * a.dim] : 0.0f;
+                    float &hi = h[i / 4][i % 4];
+                    hi = hi != 0.0f ? __builtin_fmaf(__builtin_amdgcn_exp2f(am[i / 4][i % 4] * sum), hi, last) : last;
+                }
             }
         }
+        float sum = 0.0f;
+        int buf = 0;
+        if (from < end) lds_barrier();
+        for (int t = from; t < end; t += TT, buf ^= 1) {
+            float bv[kBC], cv[kBC];
+#pragma unroll
+            for (int i = 0; i < kBC; ++i) {
+                const int e = i * 16 + (lane & 15), at = e / S * kStates + n0 + e % S;
+                bv[i] = bs[buf][at];
+                cv[i] = kY ? cs[buf][at] : 0.0f;
+            }
+            float2 dx[TT];
+#pragma unroll
+            for (int s = 0; s < TT; ++s) dx[s] = steps[buf][s][lane];
+            float p[S / 4][4];
+#pragma unroll
+            for (int i = 0; i < S; ++i) p[i / 4][i % 4] = am[i / 4][i % 4] * dx[0].x;
+            static_for<TT>([&](auto step) {
+                constexpr int s = decltype(step)::value;
+                const float next = dx[s + 1 < TT ? s + 1 : s].x;
+                if (PASS == kEnds) sum += dx[s].x;
+                float acc = 0.0f;
+                static_for<S / 4>([&](auto quad) {
+                    constexpr int q = decltype(quad)::value, k0 = s * S + 4 * q;
+                    float e[4], x[4];
+                    static_for<4>([&](auto state) {
+                        constexpr int i = decltype(state)::value;
+                        e[i] = __builtin_amdgcn_exp2f(p[q][i]);
+                        x[i] = bcast<(k0 + i) % 16>(bv[k0 / 16]) * dx[s].y;
+                    });
+                    if constexpr (kY) {
+                        scan_quad<k0 % 16>(am[q], next, e, x, cv[k0 / 16], p[q], h[q], acc);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            h[q][i] = __builtin_fmaf(e[i], h[q][i], x[i]);
+                            p[q][i] = am[q][i] * next;
+                        }
+                    }
+                });
+                if (kY) parts[buf][wave][s][lane] = acc;
+            });
+            lds_barrier();
+        }
+        if (!on) return;
+        if (PASS == kEnds) {
+            float *e = sp.ends + (b * sp.chunks + k) * (N + 1) * a.dim + c;
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+                if (n0 + i < N) e[(int64_t)(n0 + i) * a.dim] = h[i / 4][i % 4];
+            if (wave == 0) e[(int64_t)N * a.dim] = sum;
+        } else if (a.h_out && (PASS == kWhole || k == sp.chunks - 1)) {
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+                if (n0 + i < N) a.h_out[(b * a.dim + c) * N + n0 + i] = h[i / 4][i % 4];
+        }
+        return;
     }
+
+    // ---- a helper wave, in front of the others: they wait for it at the barrier
+    // (151 us instead of 156 at 8 x 2048 x 1536 x 16)
+    __builtin_amdgcn_s_setprio(2);
+    const int hw = wave - NW, r0 = hw * kRows, tid = hw * 64 + lane;
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.0f, skip = a.d_skip ? a.d_skip[c] : 0.0f;
     const bool gate = kY && a.z.p != nullptr;
-
-    // the rows of the tile at t: this wave's share of dt, u and z, and B and C of its states
-    T dt_next[kRows], u_next[kRows], z_next[kRows], b_next[kB], c_next[kC];
-    auto load = [&](int t) {
+    // Rows are read from the tile's first row, whose address every lane shares, by
+    // 32-bit offsets that stay the same from tile to tile.
+    uint32_t dt_off[kRows], u_off[kRows], z_off[kRows], y_off[kRows], b_off[kLoadBC], c_off[kLoadBC];
+    auto offsets = [&](int last) {                             // last: the last row of the tile that is read
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const int row = min(t + wave * kRows + i, end - 1);
-            dt_next[i] = a.dt.row(b, row)[c];
-            u_next[i] = a.u.row(b, row)[c];
-            if (gate) z_next[i] = a.z.row(b, row)[c];
+            const uint32_t row = min(r0 + i, last);
+            dt_off[i] = (row * (uint32_t)a.dt.ld + c) * sizeof(T);
+            u_off[i] = (row * (uint32_t)a.u.ld + c) * sizeof(T);
+            z_off[i] = gate ? (row * (uint32_t)a.z.ld + c) * sizeof(T) : u_off[i];
+            y_off[i] = ((r0 + i) * (uint32_t)a.y.ld + c) * sizeof(T);
         }
 #pragma unroll
-        for (int i = 0; i < kB; ++i) {
-            const int at = i * 64 + lane;
-            b_next[i] = a.b.row(b, min(t + at / S, end - 1))[(int64_t)g * N + min(n0 + at % S, N - 1)];
-        }
-        if (kY) {
-#pragma unroll
-            for (int i = 0; i < kC; ++i) {
-                const int at = i * 16 + lane / 4;
-                c_next[i] = a.c.row(b, min(t + at / S, end - 1))[(int64_t)g * N + min(n0 + at % S, N - 1)];
-            }
+        for (int i = 0; i < kLoadBC; ++i) {
+            const int e = min(tid + i * 64 * kHelpers, TT * kStates - 1);
+            const uint32_t row = min(e / kStates, last), col = g * N + min(e % kStates, N - 1);
+            b_off[i] = (row * (uint32_t)a.b.ld + col) * sizeof(T);
+            c_off[i] = (row * (uint32_t)a.c.ld + col) * sizeof(T);
         }
     };
-
-    float sum = 0.0f;
-    if (from < end) load(from);
-    for (int t = from; t < end; t += TT) {
-        float u[kRows], z[kRows], bv[kB], cv[kC], d[kRows], du[kRows], y[kShare ? 1 : TT];
+    auto at = [](const T *base, uint32_t off) {
+        return *reinterpret_cast<const T *>(reinterpret_cast<const char *>(base) + off);
+    };
+    const T *dt_p = a.dt.row(b, from), *u_p = a.u.row(b, from), *z_p = gate ? a.z.row(b, from) : u_p;
+    const T *b_p = a.b.row(b, from), *c_p = a.c.row(b, from);
+    const int64_t z_ld = gate ? a.z.ld : a.u.ld;
+    T *y_p = kY ? a.y.row(b, from) : nullptr;
+    T dt_next[kRows], u_next[kRows], z_next[kRows], b_next[kLoadBC], c_next[kLoadBC];
+    auto load = [&]() {
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const bool in = t + wave * kRows + i < end;
-            u[i] = (float)u_next[i];
-            z[i] = gate ? (float)z_next[i] : 0.0f;
+            dt_next[i] = at(dt_p, dt_off[i]);
+            u_next[i] = at(u_p, u_off[i]);
+            if (kY) z_next[i] = at(z_p, z_off[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kLoadBC; ++i) {
+            b_next[i] = at(b_p, b_off[i]);
+            if (kY) c_next[i] = at(c_p, c_off[i]);
+        }
+    };
+    // the loads of the tile at t, the one after the last that was loaded
+    auto fetch = [&](int t) {
+        if (t >= end) return;
+        if (end - t < TT) offsets(end - t - 1);
+        dt_p += TT * a.dt.ld;
+        u_p += TT * a.u.ld;
+        z_p += TT * z_ld;
+        b_p += TT * a.b.ld;
+        c_p += TT * a.c.ld;
+        load();
+    };
+    float u[3][kRows], z[3][kRows];                            // of the tile staged, the one before it, ...
+    auto stage = [&](int t, int buf) {
+        const int rows = end - t;                              // steps past the end: a step of 0 that adds nothing
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            u[2][i] = u[1][i];
+            z[2][i] = z[1][i];
+            u[1][i] = u[0][i];
+            z[1][i] = z[0][i];
+            u[0][i] = (float)u_next[i];
+            z[0][i] = kY ? (float)z_next[i] : 0.0f;
             const float raw = (float)dt_next[i] + bias;
-            float s = kLog2e * raw, v = raw * u[i];
+            float d = kLog2e * raw, du = raw * u[0][i];
             if (a.softplus) {
-                const float e = __builtin_amdgcn_exp2f(-fabsf(s)), w = 1.0f + e;
-                const float low = __builtin_amdgcn_logf(w) + kLog2e * (e - (w - 1.0f));
-                s = s > 0.0f ? s + low : (s <= 0.0f ? low : s);
-                v = s * (kLn2 * u[i]);
+                const float e = __builtin_amdgcn_exp2f(-fabsf(d)), w = 1.0f + e;
+                d = fmaxf(d, 0.0f) + (__builtin_amdgcn_logf(w) + kLog2e * (e - (w - 1.0f)));
+                du = d * (kLn2 * u[0][i]);
             }
-            d[i] = in ? s : 0.0f;
-            du[i] = in ? v : 0.0f;
-            if (kShare) steps[wave * kRows + i][lane] = float2{d[i], du[i]};
+            steps[buf][r0 + i][lane] = r0 + i < rows ? float2{d, du} : float2{0.0f, 0.0f};
         }
 #pragma unroll
-        for (int i = 0; i < kB; ++i) {
-            const int at = i * 64 + lane;
-            bv[i] = t + at / S < end && n0 + at % S < N ? (float)b_next[i] : 0.0f;
+        for (int i = 0; i < kLoadBC; ++i) {
+            const int e = min(tid + i * 64 * kHelpers, TT * kStates - 1);
+            const bool real = e % kStates < N;
+            bs[buf][e] = real && e / kStates < rows ? (float)b_next[i] : 0.0f;
+            if (kY) cs[buf][e] = real ? (float)c_next[i] : 0.0f;
         }
-        if (kY) {
+    };
+    auto finish = [&](int t, int buf, const float (&uf)[kRows], const float (&zf)[kRows]) {
 #pragma unroll
-            for (int i = 0; i < kC; ++i) cv[i] = n0 + (i * 16 + lane / 4) % S < N ? (float)c_next[i] : 0.0f;
+        for (int i = 0; i < kRows; ++i) {
+            float v = skip * uf[i];
+#pragma unroll
+            for (int w = 0; w < NW; ++w) v += parts[buf][w][r0 + i][lane];
+            const float gated = v * silu(zf[i]);
+            if (on && t + r0 + i < end)
+                *reinterpret_cast<T *>(reinterpret_cast<char *>(y_p) + y_off[i]) = (T)(gate ? gated : v);
         }
-        if (t + TT < end) load(t + TT);
-        if (kShare) __syncthreads();
-        static_for<TT>([&](auto step) {
-            constexpr int s = decltype(step)::value;
-            float ds, dus;
-            if constexpr (kShare) {
-                const float2 v = steps[s][lane];
-                ds = v.x;
-                dus = v.y;
-            } else {
-                ds = d[s];
-                dus = du[s];
-            }
-            if (PASS == kEnds) sum += ds;
-            v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-            static_for<S / 4>([&](auto quad) {
-                constexpr int q = decltype(quad)::value, at = s * S + 4 * q;
-                v4f p;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(am[4 * q + i] * ds) * h[q][i];
-                h[q] = outer<at % 64 / 4>(bv[at / 64], dus, p);
-                if constexpr (kY)
-                    static_for<4>([&](auto state) {
-                        constexpr int n = at + decltype(state)::value;
-                        acc = outer<n % 16>(cv[n / 16], h[q][decltype(state)::value], acc);
-                    });
-            });
-            if constexpr (kY) {
-                if constexpr (kShare)
-                    parts[wave][s][lane] = acc[0];
-                else
-                    y[s] = acc[0];
-            }
-        });
-        if (kShare) __syncthreads();
-        if (kY) {
-#pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                const int s = wave * kRows + i;
-                float v = skip * u[i];
-                if (kShare) {
-#pragma unroll
-                    for (int w = 0; w < NW; ++w) v += parts[w][s][lane];
-                } else {
-                    v += y[i];
-                }
-                if (gate) v *= silu(z[i]);
-                if (on && t + s < end) a.y.row(b, t + s)[c] = (T)v;
-            }
+        y_p += TT * a.y.ld;
+    };
+    if (from < end) {
+        offsets(min(TT, end - from) - 1);
+        load();
+        stage(from, 0);
+        fetch(from + TT);
+        lds_barrier();
+        int buf = 0, t = from;
+        for (; t + TT < end; t += TT, buf ^= 1) {
+            stage(t + TT, buf ^ 1);
+            fetch(t + 2 * TT);
+            if (kY && t > from) finish(t - TT, buf ^ 1, u[2], z[2]);
+            lds_barrier();
         }
+        if (kY && t > from) finish(t - TT, buf ^ 1, u[1], z[1]);
+        lds_barrier();
+        if (kY) finish(t, buf, u[0], z[0]);
     }
-    if (kY)
-        for (int t = max(from, end) + wave; t < to; t += NW)
-            if (on) a.y.row(b, t)[c] = (T)0.0f;
-    if (!on) return;
-    if (PASS == kEnds) {
-        float *e = sp.ends + (b * sp.chunks + k) * (N + 1) * a.dim + c;
-#pragma unroll
-        for (int i = 0; i < S; ++i)
-            if (n0 + i < N) e[(int64_t)(n0 + i) * a.dim] = h[i / 4][i % 4];
-        if (wave == 0) e[(int64_t)N * a.dim] = sum;
-    } else if (a.h_out && (PASS == kWhole || k == sp.chunks - 1)) {
-#pragma unroll
-        for (int i = 0; i < S; ++i)
-            if (n0 + i < N) a.h_out[(b * a.dim + c) * N + n0 + i] = h[i / 4][i % 4];
-    }
+    if (kY && on)
+        for (int t = max(from, end) + hw; t < to; t += kHelpers) a.y.row(b, t)[c] = (T)0.0f;
 }
 
 // How a scan is split: states a wave, waves a block, parts of the sequence (0: the
@@ -330,20 +420,24 @@ struct ScanPlan {
 
 inline ScanPlan scan_plan(int batch, int len, int dim, int nstate, int groups) {
     ScanPlan p{};
-    if (len <= 4) return p;
+    if (len <= kScanStepLen) return p;
     p.blocks = (dim / groups + 63) / 64;
+    // four waves of the states where that is 4 to 16 a wave (64 states, 256 blocks of 512
+    // steps: 16 x 4 110 us, 8 x 8 120; 32 states: 8 x 4 67, 4 x 8 75)
+    p.states = nstate <= 16 ? 4 : nstate <= 32 ? 8 : nstate <= 128 ? 16 : 32;
+    p.waves = nstate <= 4 ? 1 : nstate <= 8 ? 2 : nstate <= 64 ? 4 : 8;
+    // Parts: a first pass over them costs about two thirds of the second, so only where
+    // blocks are few, and then about three blocks a CU; and parts of 2 sqrt(len) steps
+    // at least, since each walks over those in front of it.  16 states, one part and the
+    // split in us: 4096 steps, 24 blocks 283 and 63; 96 blocks 284 and 176; 128 blocks 284
+    // and 229; 192 blocks 290 and 331.  256 steps: 24 blocks 22 and 14, 128 blocks 23 and 26.
     const int64_t blocks = (int64_t)batch * groups * p.blocks;
-    const int64_t simds = (int64_t)device_cus() * 4;
-    p.states = nstate > 64 || blocks >= 2 * simds ? 16 : 4;
-    p.waves = 1;
-    while (p.waves * p.states < nstate) p.waves *= 2;
-    // a second pass over the sequence costs as much as the first one saves until the
-    // waves are few
+    const int cus = device_cus();
     int64_t chunks = 1;
-    if (blocks * p.waves * 2 <= simds) chunks = 2 * simds / (blocks * p.waves);
-    const int64_t most = (len + 63) / 64;
-    if (chunks > most) chunks = most;
-    if (chunks > 64) chunks = 64;
+    if (blocks <= (len < 512 ? cus * 3 / 8 : cus / 2)) {
+        chunks = 3 * cus / blocks;
+        while (chunks * chunks * 4 > len) --chunks;
+    }
     if (chunks < 3) chunks = 1;
     p.chunk = (int)(((len + chunks - 1) / chunks + 15) / 16 * 16);
     p.chunks = (len + p.chunk - 1) / p.chunk;
@@ -355,10 +449,10 @@ void launch_scan_tiles(const ScanArgs<T> &a, const ScanPlan &p, float *ends, hip
     const ScanSplit sp{ends, p.chunks, p.chunk, p.blocks};
     const dim3 grid((unsigned)(a.batch * a.groups * p.blocks), (unsigned)p.chunks);
     if (p.chunks == 1) {
-        hipLaunchKernelGGL((scan_tile_kernel<T, S, NW, TT, kWhole>), grid, dim3(64 * NW), 0, st, a, sp);
+        hipLaunchKernelGGL((scan_tile_kernel<T, S, NW, TT, kWhole>), grid, dim3(64 * (NW + kHelpers)), 0, st, a, sp);
     } else {
-        hipLaunchKernelGGL((scan_tile_kernel<T, S, NW, TT, kEnds>), dim3(grid.x, grid.y - 1), dim3(64 * NW), 0, st, a, sp);
-        hipLaunchKernelGGL((scan_tile_kernel<T, S, NW, TT, kParts>), grid, dim3(64 * NW), 0, st, a, sp);
+        hipLaunchKernelGGL((scan_tile_kernel<T, S, NW, TT, kEnds>), dim3(grid.x, grid.y - 1), dim3(64 * (NW + kHelpers)), 0, st, a, sp);
+        hipLaunchKernelGGL((scan_tile_kernel<T, S, NW, TT, kParts>), grid, dim3(64 * (NW + kHelpers)), 0, st, a, sp);
     }
 }
 
@@ -387,13 +481,10 @@ void launch_scan(const ScanArgs<T> &a, const ScanPlan &p, float *ends, hipStream
         case 401: return launch_scan_tiles<T, 4, 1, 16>(a, p, ends, st);
         case 402: return launch_scan_tiles<T, 4, 2, 16>(a, p, ends, st);
         case 404: return launch_scan_tiles<T, 4, 4, 16>(a, p, ends, st);
-        case 408: return launch_scan_tiles<T, 4, 8, 16>(a, p, ends, st);
-        case 416: return launch_scan_tiles<T, 4, 16, 16>(a, p, ends, st);
-        case 1601: return launch_scan_tiles<T, 16, 1, 8>(a, p, ends, st);
-        case 1602: return launch_scan_tiles<T, 16, 2, 16>(a, p, ends, st);
+        case 804: return launch_scan_tiles<T, 8, 4, 16>(a, p, ends, st);
         case 1604: return launch_scan_tiles<T, 16, 4, 16>(a, p, ends, st);
-        case 1608: return launch_scan_tiles<T, 16, 8, 16>(a, p, ends, st);
-        default: return launch_scan_tiles<T, 16, 16, 16>(a, p, ends, st);
+        case 1608: return launch_scan_tiles<T, 16, 8, 8>(a, p, ends, st);
+        default: return launch_scan_tiles<T, 32, 8, 8>(a, p, ends, st);
     }
 }
 
@@ -438,8 +529,11 @@ extern "C" mi_status mi_selective_scan(const void *u, int64_t ldu, int64_t bsu, 
     MI_REQUIRE(a && (len == 0 || (u && dt && b && c && y)), MI_ERR_NULL_POINTER,
                "mi_selective_scan: u, dt, a, b, c and y are required");
     const ScanPlan plan = scan_plan(batch, len, dim, nstate, groups);
-    MI_REQUIRE((int64_t)batch * groups * plan.blocks * plan.waves * 64 < ((int64_t)1 << 32), MI_ERR_BAD_DIM,
+    MI_REQUIRE((int64_t)batch * groups * plan.blocks * (plan.waves + kHelpers) * 64 < ((int64_t)1 << 32), MI_ERR_BAD_DIM,
                "mi_selective_scan: too many groups of few channels for one launch");
+    MI_REQUIRE(plan.chunks == 0 || (ldu <= kScanMaxLd && ldt <= kScanMaxLd && ldb <= kScanMaxLd && ldc <= kScanMaxLd &&
+                                    ldz <= kScanMaxLd && ldy <= kScanMaxLd),
+               MI_ERR_BAD_DIM, "mi_selective_scan: a row stride is above %lld", (long long)kScanMaxLd);
     const size_t need = plan.chunks > 1 ? (size_t)batch * plan.chunks * (nstate + 1) * dim * sizeof(float) : 0;
     MI_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), MI_ERR_BAD_ARG,
                "mi_selective_scan: workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : 0, need);
