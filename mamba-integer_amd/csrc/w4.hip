@@ -9,6 +9,8 @@
 // eight in bits 4 (c / 2) for an even c, 16 + 4 (c / 2) for an odd one (the two
 // columns of a 16-bit pair lie 16 bits apart).  Scales and zero points lie as
 // [row block, group, 16].
+#include <type_traits>
+
 #include "float_ops.hpp"
 
 namespace mi {
@@ -116,87 +118,178 @@ struct W4Type<float> {
     }
 };
 
-// A block: KS waves, 16 weight rows, MT x 16 rows of x; wave w takes the column
-// blocks w, w + KS, ...  In the matrix instruction x is operand A (lane: row l & 15,
-// columns 8 (l >> 4) .. + 7 of 32) and the weights B (lane: weight row l & 15), so a
-// lane's results belong to one weight row and its scale.
-template <class T, class S, int MT, int KS>
+// A block: NT x 16 weight rows and MT x 16 rows of x; its KS waves take every KS-th
+// column block and join their sums in LDS, so the block reads each of its weights and
+// its rows of x once and no wave waits for another before the end.  A wave issues all
+// loads of U column blocks (weights, scales, x) before it uses the first: the call is
+// a few memory latencies long.  In the matrix instruction x is operand A (lane: row
+// l & 15, columns 8 (l >> 4) .. + 7 of 32) and the weights B (lane: weight row l & 15),
+// so a lane's results belong to one weight row and its scale.  16 times the row sums of
+// x come from a product with a constant operand.
+// The whole column blocks go without a branch (one past a wave's last is one of its
+// own again, scaled by 0), since a load in a branch is waited for where the branch
+// ends; the columns past them are a last step of their own.
+template <class T, class S, int MT, int NT, int KS, int U>
 __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
     using W = W4Type<T>;
     using Vec = typename W::Vec;
     constexpr int P = W::kParts;
-    __shared__ v4f part[KS][MT][64];
+    __shared__ v4f part[KS][MT * NT][64];
     const int wave = wave_id(), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int64_t nb = blockIdx.x;
-    const int m0 = blockIdx.y * 16 * MT, kb_all = (a.k + kW4Cols - 1) / kW4Cols;
-    const v4u *words = reinterpret_cast<const v4u *>(a.packed) + nb * kb_all * 64 + lane;
-    const S *scales = a.scales + nb * a.ng * kW4Rows + r;
-    const uint8_t *zeros = a.zeros ? a.zeros + nb * a.ng * kW4Rows + r : nullptr;
+    const int nb_all = (a.n + kW4Rows - 1) / kW4Rows, kb_all = (a.k + kW4Cols - 1) / kW4Cols, kb_whole = a.k / kW4Cols;
+    const int m0 = blockIdx.y * 16 * MT;
+    const int per = a.group < kW4Cols ? kW4Cols / a.group : 1;             // groups of a column block
+    const int each = a.group < kW4Cols ? 1 : a.group / kW4Cols;            // column blocks of a group
+    const v4u *words[NT];
+    const S *scales[NT];
+    const uint8_t *zeros[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int64_t nb = min((int)blockIdx.x * NT + nt, nb_all - 1);     // past the last: not stored
+        words[nt] = reinterpret_cast<const v4u *>(a.packed) + nb * kb_all * 64 + lane;
+        // a lane loads one of the column block's (group, row) values, and gets those it needs from other lanes
+        const int64_t at = nb * a.ng * kW4Rows + (lane & (16 * per - 1));
+        scales[nt] = a.scales + at;
+        zeros[nt] = a.zeros ? a.zeros + at : reinterpret_cast<const uint8_t *>(scales[nt]);
+    }
+    const T *x[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) x[mt] = a.x + (int64_t)min(m0 + 16 * mt + r, a.m - 1) * a.ldx + 8 * g;
     const Vec ones = W::weights(0);   // 16 in every place
-    v4f acc[MT] = {};
-    for (int kb = wave; kb < kb_all; kb += KS) {
-        const v4u w = words[(int64_t)kb * 64];
-        v4f d[MT], s16[MT];   // sums of x (16 + q) and of 16 x of the group so far
+    v4f acc[MT][NT] = {};
+    // the sums of a column block: x (16 + q) by groups, less (16 + zero) of x
+    auto compute = [&](const v4u (&w)[NT], const Packed<T, 8> (&xv)[MT][4], const float (&s)[NT], const float (&z)[NT]) {
+        v4f d[MT][NT] = {}, s16[MT] = {};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int k = kb * kW4Cols + 32 * j;
-            const bool first = a.group == 32 || j == 0 || (a.group == 64 && j == 2);
-            const Vec wj = W::weights(w[j]);
+            Vec wj[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) wj[nt] = W::weights(w[nt][j]);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const int m = m0 + 16 * mt + r, k0 = k + 8 * g;
-                Packed<T, 8> xv;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) xv.v[i] = (T)0.0f;
-                if (m < a.m) {
-                    const T *x = a.x + (int64_t)m * a.ldx + k0;
-                    if (k0 + 8 <= a.k) {
-                        xv = load_packed<8>(x);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (k0 + i < a.k) xv.v[i] = x[i];
-                    }
-                }
                 Vec parts[P];
-                W::split(xv, parts);
-                if (first) d[mt] = s16[mt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                W::split(xv[mt][j], parts);
 #pragma unroll
                 for (int p = P - 1; p >= 0; --p) {
-                    d[mt] = mfma(parts[p], wj, d[mt]);
                     s16[mt] = mfma(parts[p], ones, s16[mt]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) d[mt][nt] = mfma(parts[p], wj[nt], d[mt][nt]);
                 }
             }
-            const bool last = a.group == 32 || j == 3 || (a.group == 64 && j == 1);
-            if (last) {
-                const int64_t at = (int64_t)(k / a.group) * kW4Rows;
-                const float s = (float)scales[at], z = 1.0f + 0.0625f * (zeros ? (float)zeros[at] : 8.0f);
+            if (per == 4 || j == 3 || (per == 2 && j == 1)) {
+                const int from = per == 4 ? 16 * j : per == 2 ? 16 * (j / 2) : 0;
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) acc[mt] += s * (d[mt] - z * s16[mt]);
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float sj = per == 1 ? s[nt] : __shfl(s[nt], from + r), zj = per == 1 ? z[nt] : __shfl(z[nt], from + r);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        acc[mt][nt] += sj * (d[mt][nt] - zj * s16[mt]);
+                        d[mt][nt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                    }
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s16[mt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
             }
         }
+    };
+    auto zero_of = [&](uint8_t z) { return 1.0f + 0.0625f * (a.zeros ? (float)z : 8.0f); };
+    for (int kb0 = wave; kb0 < kb_whole; kb0 += KS * U) {
+        v4u w[U][NT];
+        S s[U][NT];
+        uint8_t z[U][NT];
+        Packed<T, 8> xv[U][MT][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int kb = kb0 + u * KS < kb_whole ? kb0 + u * KS : kb0;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                w[u][nt] = words[nt][(int64_t)kb * 64];
+                s[u][nt] = scales[nt][(int64_t)(kb / each) * (16 * per)];
+                z[u][nt] = zeros[nt][(int64_t)(kb / each) * (16 * per)];
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) xv[u][mt][j] = load_packed<8>(x[mt] + kb * kW4Cols + 32 * j);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float sf[NT], zf[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                sf[nt] = kb0 + u * KS < kb_whole ? (float)s[u][nt] : 0.0f;
+                zf[nt] = zero_of(z[u][nt]);
+            }
+            compute(w[u], xv[u], sf, zf);
+        }
+    }
+    if (kb_whole < kb_all && wave == kb_whole % KS) {
+        v4u w[NT];
+        float s[NT], z[NT];
+        Packed<T, 8> xv[MT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            w[nt] = words[nt][(int64_t)kb_whole * 64];
+            s[nt] = (float)scales[nt][(int64_t)(kb_whole / each) * (16 * per)];
+            z[nt] = zero_of(zeros[nt][(int64_t)(kb_whole / each) * (16 * per)]);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int k = kb_whole * kW4Cols + 32 * j + i;
+                    xv[mt][j].v[i] = k + 8 * g < a.k ? x[mt][k] : (T)0.0f;
+                }
+        compute(w, xv, s, z);
     }
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) part[wave][mt][lane] = acc[mt];
+    for (int i = 0; i < MT * NT; ++i) part[wave][i][lane] = acc[i / NT][i % NT];
     __syncthreads();
-    const int n = (int)nb * kW4Rows + r;
-    for (int mt = wave; mt < MT; mt += KS) {
-        v4f sum = part[0][mt][lane];
+    for (int i = wave; i < MT * NT; i += KS) {
+        v4f sum = part[0][i][lane];
 #pragma unroll
-        for (int w = 1; w < KS; ++w) sum += part[w][mt][lane];
-        const float bias = a.bias && n < a.n ? a.bias[n] : 0.0f;
+        for (int w = 1; w < KS; ++w) sum += part[w][i][lane];
+        const int n = (int)(blockIdx.x * NT + i % NT) * kW4Rows + r;
+        if (n >= a.n) continue;
+        const float bias = a.bias ? a.bias[n] : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int m = m0 + 16 * mt + 4 * g + i;
-            if (m < a.m && n < a.n) a.y[(int64_t)m * a.ldy + n] = (T)(sum[i] + bias);
+        for (int e = 0; e < 4; ++e) {
+            const int m = m0 + 16 * (i / NT) + 4 * g + e;
+            if (m < a.m) a.y[(int64_t)m * a.ldy + n] = (T)(sum[e] + bias);
         }
     }
 }
 
-template <class T, class S, int MT>
+template <class T, class S, int MT, int NT, int KS, int U>
 void launch_w4(const W4Args<T, S> &a, hipStream_t st) {
-    const dim3 grid((unsigned)((a.n + kW4Rows - 1) / kW4Rows), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
-    hipLaunchKernelGGL((w4_kernel<T, S, MT, 4>), grid, dim3(256), 0, st, a);
+    const dim3 grid((unsigned)((a.n + 16 * NT - 1) / (16 * NT)), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
+    hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, KS, U>), grid, dim3(64 * KS), 0, st, a);
+}
+
+// By the rows of x, and by the number of row blocks: more weight rows a block read x
+// fewer times, more waves a block share a column's blocks where there are few blocks.
+template <class T, class S>
+void launch_w4_shape(const W4Args<T, S> &a, hipStream_t st) {
+    constexpr bool f32 = std::is_same<T, float>::value;
+    const int nb = (a.n + kW4Rows - 1) / kW4Rows, cus = device_cus();
+    if (a.m <= 16) {
+        if (nb >= 3 * cus)
+            launch_w4<T, S, 1, 1, 4, f32 ? 2 : 4>(a, st);
+        else
+            launch_w4<T, S, 1, 1, 8, 2>(a, st);
+    } else if (a.m <= 32 || f32) {
+        if (nb >= 2 * cus)
+            launch_w4<T, S, 2, 2, 8, f32 ? 1 : 2>(a, st);
+        else
+            launch_w4<T, S, 2, 1, 8, f32 ? 1 : 2>(a, st);
+    } else {
+        if (nb >= 2 * cus)
+            launch_w4<T, S, f32 ? 2 : 4, 2, 8, f32 ? 1 : 2>(a, st);
+        else
+            launch_w4<T, S, f32 ? 2 : 4, 1, 8, f32 ? 1 : 2>(a, st);
+    }
 }
 
 // Groups of one packed row block: whole column blocks of them.
@@ -253,8 +346,8 @@ extern "C" mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const ui
     if (m == 0 || n == 0) return MI_OK;
     MI_REQUIRE(x && packed && scales && y, MI_ERR_NULL_POINTER, "mi_w4_matvec: x, packed, scales and y are required");
     MI_REQUIRE(aligned(packed, 16), MI_ERR_BAD_ALIGNMENT, "mi_w4_matvec: packed must be 16-byte aligned");
-    MI_REQUIRE((int64_t)m * n < ((int64_t)1 << 31) && m <= 64 * 65535, MI_ERR_BAD_DIM,
-               "mi_w4_matvec: m * n must be below 2^31, and m at most 64 * 65535");
+    MI_REQUIRE((int64_t)m * n < ((int64_t)1 << 31) && m <= 32 * 65535, MI_ERR_BAD_DIM,
+               "mi_w4_matvec: m * n must be below 2^31, and m at most 32 * 65535");
     const hipStream_t st = as_stream(stream);
     with_type(type, [&](auto t) {
         using T = decltype(t);
@@ -263,12 +356,7 @@ extern "C" mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const ui
             const W4Args<T, S> a{static_cast<const T *>(x), ldx, reinterpret_cast<const uint32_t *>(packed),
                                  static_cast<const S *>(scales), zeros, bias, static_cast<T *>(y), ldy, m, n, k, group,
                                  w4_groups(k, group)};
-            if (m <= 16)
-                launch_w4<T, S, 1>(a, st);
-            else if (m <= 32)
-                launch_w4<T, S, 2>(a, st);
-            else
-                launch_w4<T, S, 4>(a, st);
+            launch_w4_shape<T, S>(a, st);
         };
         if (scale_type == MI_F32)
             go(float{});

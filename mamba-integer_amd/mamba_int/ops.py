@@ -491,42 +491,53 @@ def _float_type(t: torch.Tensor, name: str) -> int:
 def _rows(t: torch.Tensor, shape, dtype: torch.dtype, name: str, out: bool = False):
     """A tensor of rows as (address, row stride[, sequence stride]); the leading
     dimensions may have any strides, the elements of a row are adjacent."""
+    _like(t, shape, dtype, name)
+    st = t.stride()
+    if st[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name}: the elements of a row must be adjacent (strides {st})")
+    if not out:
+        return (t.data_ptr(), st[1], st[0]) if len(st) == 3 else (t.data_ptr(), st[0])
+    # rows that overlap would be written twice: each must end before the next begins
+    span = shape[-1]
+    for size, stride in zip(reversed(shape[:-1]), reversed(st[:-1])):
+        if size > 1 and stride < span:
+            raise ValueError(f"{name}: output rows overlap (strides {st})")
+        span = max(span, stride * size)
+    # (the stride of a dimension of one element is free: the library asks for a row's length)
+    ld = st[-2] if shape[-2] > 1 else shape[-1]
+    return (t.data_ptr(), ld, st[0] if shape[0] > 1 else 0) if len(st) == 3 else (t.data_ptr(), ld)
+
+
+def _like(t: torch.Tensor, shape, dtype: torch.dtype, name: str) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a device tensor (libmamba_int has no host path)")
-    st = t.stride()
-    if st[-1] != 1 and shape[-1] > 1:
-        raise ValueError(f"{name}: the elements of a row must be adjacent (strides {st})")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient; the float operators are forward only")
-    if out:
-        # rows that overlap would be written twice: each must end before the next begins
-        span = shape[-1]
-        for size, stride in zip(reversed(shape[:-1]), reversed(st[:-1])):
-            if size > 1 and stride < span:
-                raise ValueError(f"{name}: output rows overlap (strides {st})")
-            span = max(span, stride * size)
-        # (the stride of a dimension of one element is free: the library asks for a row's length)
-        ld = st[-2] if shape[-2] > 1 else shape[-1]
-        return (t.data_ptr(), ld) + ((st[0] if shape[0] > 1 else 0,) if len(shape) == 3 else ())
-    return (t.data_ptr(), st[-2]) + ((st[0],) if len(shape) == 3 else ())
 
 
 def _vec(t: Optional[torch.Tensor], shape, dtype: torch.dtype, name: str):
     """Address of a contiguous tensor of this shape (None: NULL)."""
     if t is None:
         return None
-    _req(t, dtype, name)
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient; the float operators are forward only")
+    _like(t, shape, dtype, name)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
+
+
+def _address(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream() -> int:
+    """The current stream's handle, without a stream object around it (2.8 us less)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _norm(x, weight, residual, eps, residual_out, y, q, scale):
@@ -544,7 +555,7 @@ def _norm(x, weight, residual, eps, residual_out, y, q, scale):
     yp, ldy = _rows(y, shape, x.dtype, "out", True) if y is not None else (None, 0)
     qp, ldq, sp = (q.data_ptr(), q.stride(0), scale.data_ptr()) if q is not None else (None, 0, None)
     _lib.call("mi_add_rms_norm", xp, code, ldx, rp, rcode, ldr, _vec(weight, shape[1:], torch.float32, "weight"),
-              eps, yp, ldy, qp, ldq, sp, op, ldo, shape[0], shape[1], _stream())
+              eps, yp, ldy, qp, ldq, sp, op, ldo, shape[0], shape[1], _raw_stream())
 
 
 def add_rms_norm(x, weight, residual=None, eps: float = 1e-5, residual_out=None, out=None):
@@ -553,9 +564,9 @@ def add_rms_norm(x, weight, residual=None, eps: float = 1e-5, residual_out=None,
     has x's type or float32 (None: s = x, returned only if ``residual_out`` is passed, else
     None).  ``residual_out`` may be the residual itself, ``out`` may be x.  Forward only."""
     _float_type(x, "x")
-    y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = out if out is not None else x.new_empty(x.shape)
     if residual is not None and residual_out is None:
-        residual_out = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+        residual_out = residual.new_empty(residual.shape)
     _norm(x, weight, residual, eps, residual_out, y, None, None)
     return y, residual_out
 
@@ -569,10 +580,10 @@ def add_rms_norm_quant(x, weight, residual=None, eps: float = 1e-5, residual_out
     if unit < 1:
         raise ValueError(f"unit={unit} must be at least 1")
     T, d = x.shape
-    q = torch.empty((T, -(-d // unit) * unit), dtype=torch.int8, device=x.device)
-    scale = torch.empty((T,), dtype=torch.float32, device=x.device)
+    q = x.new_empty((T, -(-d // unit) * unit), dtype=torch.int8)
+    scale = x.new_empty((T,), dtype=torch.float32)
     if residual is not None and residual_out is None:
-        residual_out = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+        residual_out = residual.new_empty(residual.shape)
     _norm(x, weight, residual, eps, residual_out, None, q, scale)
     return q, scale, residual_out
 
@@ -596,14 +607,14 @@ def causal_conv(x, weight, bias=None, activation: Optional[str] = "silu", state_
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight must be a tensor [dim, width]")
     W = weight.shape[1]
-    y = out if out is not None else torch.empty(shape, dtype=x.dtype, device=x.device)
+    y = out if out is not None else x.new_empty(shape)
     xp, ldx, bsx = _rows(x, shape, x.dtype, "x")
     yp, ldy, bsy = _rows(y, shape, x.dtype, "out", True)
     st = (B, W - 1, D)
     _lib.call("mi_causal_conv", xp, ldx, bsx, code, _vec(weight, (D, W), torch.float32, "weight"),
               _vec(bias, (D,), torch.float32, "bias"), W, _ACTIVATIONS[activation],
               _vec(state_in, st, x.dtype, "state_in"), _vec(state_out, st, x.dtype, "state_out"),
-              _vec(lens, (B,), torch.int32, "lens"), yp, ldy, bsy, B, L, D, _stream())
+              _vec(lens, (B,), torch.int32, "lens"), yp, ldy, bsy, B, L, D, _raw_stream())
     return y
 
 
@@ -642,16 +653,16 @@ def selective_scan(u, dt, a, b, c, d_skip=None, z=None, dt_bias=None, dt_softplu
                 raise ValueError(f"{name}: the groups of a row must be adjacent (strides {t.stride()})")
             t = t[:, :, 0] if G == 1 else t.as_strided((B, L, G * N), (t.stride(0), t.stride(1), 1))
         rows.append(_rows(t, (B, L, G * N), typ, name))
-    y = out if out is not None else torch.empty(shape, dtype=typ, device=u.device)
+    y = out if out is not None else u.new_empty(shape)
     st = (B, D, N)
     size = _scan_workspace(B, L, D, N, G)
-    ws = torch.empty(size, dtype=torch.uint8, device=u.device).data_ptr() if size else None
+    ws = u.new_empty(size, dtype=torch.uint8) if size else None
     _lib.call("mi_selective_scan", *_rows(u, shape, typ, "u"), *_rows(dt, shape, typ, "dt"),
               _vec(a, (D, N), torch.float32, "a"), *rows[0], *rows[1], _vec(d_skip, (D,), torch.float32, "d_skip"),
               *(_rows(z, shape, typ, "z") if z is not None else (None, 0, 0)),
               _vec(dt_bias, (D,), torch.float32, "dt_bias"), int(dt_softplus), _vec(h_in, st, torch.float32, "h_in"),
               _vec(h_out, st, torch.float32, "h_out"), _vec(lens, (B,), torch.int32, "lens"),
-              *_rows(y, shape, typ, "out", True), code, B, L, D, N, G, ws, size, _stream())
+              *_rows(y, shape, typ, "out", True), code, B, L, D, N, G, _address(ws), size, _raw_stream())
     return y
 
 
@@ -681,7 +692,7 @@ def pack_w4(codes, scales, group: int, zeros=None):
     z_out = torch.empty((nb, ng, 16), dtype=torch.uint8, device=codes.device) if zeros is not None else None
     _lib.call("mi_pack_w4", codes.data_ptr(), _vec(scales, (n, have), st, "scales"), _FLOAT[st],
               _vec(zeros, (n, have), torch.uint8, "zeros"), packed.data_ptr(), s_out.data_ptr(), _ptr(z_out), n, k, group,
-              _stream())
+              _raw_stream())
     return packed, s_out, z_out
 
 
@@ -697,9 +708,9 @@ def w4_matvec(x, packed, scales, n: int, group: int, zeros=None, bias=None, out=
     if st is not torch.float16 and st is not torch.float32:
         raise TypeError(f"scales must be a float16 or float32 tensor, got {st}")
     vals = (nb, _w4_groups(k, group), 16)
-    y = out if out is not None else torch.empty((M, n), dtype=x.dtype, device=x.device)
+    y = out if out is not None else x.new_empty((M, n))
     _lib.call("mi_w4_matvec", *_rows(x, x.shape, x.dtype, "x"), code,
               _vec(packed, (nb, -(-k // 128), 1024), torch.uint8, "packed"), _vec(scales, vals, st, "scales"), _FLOAT[st],
               _vec(zeros, vals, torch.uint8, "zeros"), _vec(bias, (n,), torch.float32, "bias"),
-              *_rows(y, (M, n), x.dtype, "out", True), M, n, k, group, _stream())
+              *_rows(y, (M, n), x.dtype, "out", True), M, n, k, group, _raw_stream())
     return y
