@@ -587,8 +587,8 @@ mi_status mi_pack_w4(const uint8_t *codes, const void *scales, int scale_type, c
 /* y[m,n] = bias[n] + sum_k x[m,k] * (code[n,k] - zero[n,k/group]) *
  * scale[n,k/group]: x and y rows of `type`, weights as mi_pack_w4 lays them
  * out (zeros NULL: 8), bias fp32 [n] nullable.  Made for the few rows of a
- * decode step (m up to 64 read the weights once); any m is computed.  A row
- * with an infinite x gives NaN where the product is infinite. */
+ * decode step (m up to 64 read the weights once); any m is computed.  A float32
+ * or bf16 row with an infinite x gives NaN where the product is infinite. */
 mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const uint8_t *packed, const void *scales,
                        int scale_type, const uint8_t *zeros, const float *bias, void *y, int64_t ldy, int m,
                        int n, int k, int group, void *stream);

@@ -65,21 +65,25 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ v4f mfma(v8b a, v8b b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// Operands of the matrix instruction by the type of x.  A weight enters as 16 + q,
-// exact in 16 bits and built by a shift and a bit select for two of them (q are the
-// top bits of the mantissa of 2^4); 16 + zero times the row's sum of x is taken off
-// after the product.  float32 rows enter as three bf16 parts whose sum is the value.
+// Operands of the matrix instruction by the type of x.  A weight is made as 16 + q,
+// exact in 16 bits by a shift and a bit select for two of them (q are the top bits of
+// the mantissa of 2^4).  f16 then takes 16 + zero off in one packed addition of two,
+// exactly; bf16 has none, so the product is made with 16 + q and 16 + zero times the
+// row's sum of x is taken off it (its 2^-8 rounding of y hides the bits this costs);
+// float32 rows, which keep theirs, enter as three bf16 parts whose sum is the value,
+// and their weights are subtracted one by one.
 template <class T>
 struct W4Type;
 template <>
 struct W4Type<bf16_t> {
     typedef v8b Vec;
     static constexpr int kParts = 1;
-    static __device__ __forceinline__ Vec weights(uint32_t w) {
-        const v4u r = {((w << 3) & 0x00780078u) | 0x41804180u, ((w >> 1) & 0x00780078u) | 0x41804180u,
-                       ((w >> 5) & 0x00780078u) | 0x41804180u, ((w >> 9) & 0x00780078u) | 0x41804180u};
-        return __builtin_bit_cast(Vec, r);
+    static constexpr bool kOffset = true;
+    static __device__ __forceinline__ v4u pairs(uint32_t w) {
+        return v4u{((w << 3) & 0x00780078u) | 0x41804180u, ((w >> 1) & 0x00780078u) | 0x41804180u,
+                   ((w >> 5) & 0x00780078u) | 0x41804180u, ((w >> 9) & 0x00780078u) | 0x41804180u};
     }
+    static __device__ __forceinline__ Vec weights(uint32_t w, float) { return __builtin_bit_cast(Vec, pairs(w)); }
     static __device__ __forceinline__ void split(const Packed<bf16_t, 8> &x, Vec (&o)[1]) {
         o[0] = __builtin_bit_cast(Vec, x);
     }
@@ -88,10 +92,11 @@ template <>
 struct W4Type<f16_t> {
     typedef v8h Vec;
     static constexpr int kParts = 1;
-    static __device__ __forceinline__ Vec weights(uint32_t w) {
+    static constexpr bool kOffset = false;
+    static __device__ __forceinline__ Vec weights(uint32_t w, float zero) {
         const v4u r = {((w << 6) & 0x03c003c0u) | 0x4c004c00u, ((w << 2) & 0x03c003c0u) | 0x4c004c00u,
                        ((w >> 2) & 0x03c003c0u) | 0x4c004c00u, ((w >> 6) & 0x03c003c0u) | 0x4c004c00u};
-        return __builtin_bit_cast(Vec, r);
+        return __builtin_bit_cast(Vec, r) - (f16_t)(16.0f + zero);
     }
     static __device__ __forceinline__ void split(const Packed<f16_t, 8> &x, Vec (&o)[1]) {
         o[0] = __builtin_bit_cast(Vec, x);
@@ -101,7 +106,18 @@ template <>
 struct W4Type<float> {
     typedef v8b Vec;
     static constexpr int kParts = 3;
-    static __device__ __forceinline__ Vec weights(uint32_t w) { return W4Type<bf16_t>::weights(w); }
+    static constexpr bool kOffset = false;
+    // bf16 is the upper half of float32, and q - zero needs no bits below it
+    static __device__ __forceinline__ Vec weights(uint32_t w, float zero) {
+        v4u r = W4Type<bf16_t>::pairs(w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float lo = __builtin_bit_cast(float, r[i] << 16) - (16.0f + zero);
+            const float hi = __builtin_bit_cast(float, r[i] & 0xffff0000u) - (16.0f + zero);
+            r[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
+        }
+        return __builtin_bit_cast(Vec, r);
+    }
     // each part the leading 8 bits of what the ones before it leave (cut off, not
     // rounded: no part overflows, and the third holds the rest exactly)
     static __device__ __forceinline__ void split(const Packed<float, 8> &x, Vec (&o)[3]) {
@@ -120,20 +136,19 @@ struct W4Type<float> {
 
 // A block: NT x 16 weight rows and MT x 16 rows of x; its KS waves take every KS-th
 // column block and join their sums in LDS, so the block reads each of its weights and
-// its rows of x once and no wave waits for another before the end.  A wave issues all
-// loads of U column blocks (weights, scales, x) before it uses the first: the call is
-// a few memory latencies long.  In the matrix instruction x is operand A (lane: row
+// its rows of x once and no wave waits for another before the end: a call is a few
+// memory latencies long.  In the matrix instruction x is operand A (lane: row
 // l & 15, columns 8 (l >> 4) .. + 7 of 32) and the weights B (lane: weight row l & 15),
-// so a lane's results belong to one weight row and its scale.  16 times the row sums of
-// x come from a product with a constant operand.
-// The whole column blocks go without a branch (one past a wave's last is one of its
-// own again, scaled by 0), since a load in a branch is waited for where the branch
-// ends; the columns past them are a last step of their own.
-template <class T, class S, int MT, int NT, int KS, int U>
+// so a lane's results belong to one weight row and its scale.  Row sums of x (bf16)
+// come from a product with ones.
+// The loads of a whole column block stand in no branch (one in a branch is waited for
+// where it ends); the columns past the whole blocks are a last step of their own.
+template <class T, class S, int MT, int NT, int KS>
 __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
     using W = W4Type<T>;
     using Vec = typename W::Vec;
     constexpr int P = W::kParts;
+    const v4u kOnes = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};    // 1 in bf16
     __shared__ v4f part[KS][MT * NT][64];
     const int wave = wave_id(), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int nb_all = (a.n + kW4Rows - 1) / kW4Rows, kb_all = (a.k + kW4Cols - 1) / kW4Cols, kb_whole = a.k / kW4Cols;
@@ -155,73 +170,72 @@ __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
     const T *x[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) x[mt] = a.x + (int64_t)min(m0 + 16 * mt + r, a.m - 1) * a.ldx + 8 * g;
-    const Vec ones = W::weights(0);   // 16 in every place
     v4f acc[MT][NT] = {};
-    // the sums of a column block: x (16 + q) by groups, less (16 + zero) of x
     auto compute = [&](const v4u (&w)[NT], const Packed<T, 8> (&xv)[MT][4], const float (&s)[NT], const float (&z)[NT]) {
-        v4f d[MT][NT] = {}, s16[MT] = {};
+        v4f d[MT][NT], sx[MT];                   // of the group so far; sx: the rows' sums of x
+        float sj[NT], zj[NT];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            if (j == 0 || per == 4 || (per == 2 && j == 2)) {
+                const int from = (per == 4 ? 16 * j : per == 2 ? 16 * (j / 2) : 0) + r;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    sj[nt] = per == 1 ? s[nt] : __shfl(s[nt], from);
+                    zj[nt] = per == 1 ? z[nt] : __shfl(z[nt], from);
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    sx[mt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) d[mt][nt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+            }
             Vec wj[NT];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) wj[nt] = W::weights(w[nt][j]);
+            for (int nt = 0; nt < NT; ++nt) wj[nt] = W::weights(w[nt][j], zj[nt]);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 Vec parts[P];
                 W::split(xv[mt][j], parts);
 #pragma unroll
                 for (int p = P - 1; p >= 0; --p) {
-                    s16[mt] = mfma(parts[p], ones, s16[mt]);
+                    if constexpr (W::kOffset) sx[mt] = mfma(parts[p], __builtin_bit_cast(Vec, kOnes), sx[mt]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) d[mt][nt] = mfma(parts[p], wj[nt], d[mt][nt]);
                 }
             }
-            if (per == 4 || j == 3 || (per == 2 && j == 1)) {
-                const int from = per == 4 ? 16 * j : per == 2 ? 16 * (j / 2) : 0;
+            if (j == 3 || per == 4 || (per == 2 && j == 1)) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const float sj = per == 1 ? s[nt] : __shfl(s[nt], from + r), zj = per == 1 ? z[nt] : __shfl(z[nt], from + r);
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        acc[mt][nt] += sj * (d[mt][nt] - zj * s16[mt]);
-                        d[mt][nt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-                    }
-                }
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) s16[mt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int mt = 0; mt < MT; ++mt)
+                        acc[mt][nt] += sj[nt] * (W::kOffset ? d[mt][nt] - (16.0f + zj[nt]) * sx[mt] : d[mt][nt]);
             }
         }
     };
-    auto zero_of = [&](uint8_t z) { return 1.0f + 0.0625f * (a.zeros ? (float)z : 8.0f); };
-    for (int kb0 = wave; kb0 < kb_whole; kb0 += KS * U) {
-        v4u w[U][NT];
-        S s[U][NT];
-        uint8_t z[U][NT];
-        Packed<T, 8> xv[U][MT][4];
+    auto zero_of = [&](uint8_t z) { return a.zeros ? (float)z : 8.0f; };
+    for (int kb = wave; kb < kb_whole; kb += KS) {
+        v4u w[NT];
+        S s[NT];
+        uint8_t z[NT];
+        Packed<T, 8> xv[MT][4];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int kb = kb0 + u * KS < kb_whole ? kb0 + u * KS : kb0;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                w[u][nt] = words[nt][(int64_t)kb * 64];
-                s[u][nt] = scales[nt][(int64_t)(kb / each) * (16 * per)];
-                z[u][nt] = zeros[nt][(int64_t)(kb / each) * (16 * per)];
-            }
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) xv[u][mt][j] = load_packed<8>(x[mt] + kb * kW4Cols + 32 * j);
+        for (int nt = 0; nt < NT; ++nt) {
+            w[nt] = words[nt][(int64_t)kb * 64];
+            s[nt] = scales[nt][(int64_t)(kb / each) * (16 * per)];
+            z[nt] = zeros[nt][(int64_t)(kb / each) * (16 * per)];
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float sf[NT], zf[NT];
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                sf[nt] = kb0 + u * KS < kb_whole ? (float)s[u][nt] : 0.0f;
-                zf[nt] = zero_of(z[u][nt]);
-            }
-            compute(w[u], xv[u], sf, zf);
+            for (int j = 0; j < 4; ++j) xv[mt][j] = load_packed<8>(x[mt] + kb * kW4Cols + 32 * j);
+        float sf[NT], zf[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            sf[nt] = (float)s[nt];
+            zf[nt] = zero_of(z[nt]);
         }
+        compute(w, xv, sf, zf);
     }
     if (kb_whole < kb_all && wave == kb_whole % KS) {
         v4u w[NT];
@@ -262,33 +276,31 @@ __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
     }
 }
 
-template <class T, class S, int MT, int NT, int KS, int U>
+template <class T, class S, int MT, int NT, int KS>
 void launch_w4(const W4Args<T, S> &a, hipStream_t st) {
     const dim3 grid((unsigned)((a.n + 16 * NT - 1) / (16 * NT)), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
-    hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, KS, U>), grid, dim3(64 * KS), 0, st, a);
+    hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, KS>), grid, dim3(64 * KS), 0, st, a);
 }
 
-// By the rows of x, and by the number of row blocks: more weight rows a block read x
-// fewer times, more waves a block share a column's blocks where there are few blocks.
+// More weight rows a block read x fewer times; fewer leave more blocks.  Measured (us;
+// 16-bit rows, weights of three sets in turn): 1 x 2048 -> 32000 NT 4, 2, 1: 9.4, 9.4,
+// 10.1 (8 rows 10.4, 11.7, 14.7; 32-bit rows 13.4 with four waves, 14.7, 19.8); 64 x
+// 2048 -> 8192 10.6, 11.8, 19.3; 64 x 2048 -> 2048 8.6, 7.1, 7.2.  64 rows as one tile of
+// x 64 x 2048 -> 8192 12.3, as two of 32 rows, which read the weights twice, 10.6.
 template <class T, class S>
 void launch_w4_shape(const W4Args<T, S> &a, hipStream_t st) {
-    constexpr bool f32 = std::is_same<T, float>::value;
     const int nb = (a.n + kW4Rows - 1) / kW4Rows, cus = device_cus();
     if (a.m <= 16) {
-        if (nb >= 3 * cus)
-            launch_w4<T, S, 1, 1, 4, f32 ? 2 : 4>(a, st);
+        if (nb >= 4 * cus)
+            launch_w4<T, S, 1, 4, std::is_same<T, float>::value ? 4 : 8>(a, st);
+        else if (nb >= 2 * cus)
+            launch_w4<T, S, 1, 2, 8>(a, st);
         else
-            launch_w4<T, S, 1, 1, 8, 2>(a, st);
-    } else if (a.m <= 32 || f32) {
-        if (nb >= 2 * cus)
-            launch_w4<T, S, 2, 2, 8, f32 ? 1 : 2>(a, st);
-        else
-            launch_w4<T, S, 2, 1, 8, f32 ? 1 : 2>(a, st);
+            launch_w4<T, S, 1, 1, 8>(a, st);
+    } else if (a.m <= 32 || nb < 2 * cus) {
+        launch_w4<T, S, 2, 2, 8>(a, st);
     } else {
-        if (nb >= 2 * cus)
-            launch_w4<T, S, f32 ? 2 : 4, 2, 8, f32 ? 1 : 2>(a, st);
-        else
-            launch_w4<T, S, f32 ? 2 : 4, 1, 8, f32 ? 1 : 2>(a, st);
+        launch_w4<T, S, 2, 4, 8>(a, st);
     }
 }
 
