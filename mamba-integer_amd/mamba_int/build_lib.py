@@ -1,11 +1,14 @@
-"""Builds libmamba_int.so (hipcc, gfx950) in-tree, next to this package."""
+"""Builds libmamba_int.so (hipcc, gfx950) in-tree, next to this package, and the module
+of the float operators' calls (host C++ against torch) in it."""
 from __future__ import annotations
 
 import concurrent.futures
 import glob
 import os
+import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 
 PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -14,6 +17,8 @@ CSRC = os.path.join(PKG_ROOT, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB_PATH = os.path.join(PKG_ROOT, "libmamba_int.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+CALLS_PATH = os.path.join(PKG_ROOT, "mamba_int", "_float_calls.so")
+CXX = os.environ.get("CXX", "g++")
 ARCH = "gfx950"
 
 FLAGS = [
@@ -40,18 +45,34 @@ def _run(cmd: list, verbose: bool) -> None:
         print(errs, file=sys.stderr)
 
 
+def calls_command(out: str) -> list:
+    """g++ of csrc/float_calls.cpp, a Python module that takes torch's tensors."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc, lib = os.path.join(root, "include"), os.path.join(root, "lib")
+    return [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", f"-I{inc}",
+            f"-I{os.path.join(inc, 'torch', 'csrc', 'api', 'include')}", f"-I{sysconfig.get_paths()['include']}",
+            os.path.join(CSRC, "float_calls.cpp"), "-o", out, f"-L{lib}", f"-Wl,-rpath,{lib}", "-ltorch_python",
+            "-ltorch_cpu", "-lc10"]
+
+
 def build(verbose: bool = False) -> str:
     """Compiles every source to an object in parallel (each file's kernels are
-    self-contained: no relocatable device code), then links the library."""
+    self-contained: no relocatable device code), then links the library; beside
+    them, the calls' module."""
     srcs = sources()
     with tempfile.TemporaryDirectory(prefix="mamba_int_build_") as tmp:
         objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in srcs]
         jobs = [[HIPCC, *FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", s, "-o", o] for s, o in zip(srcs, objs)]
+        jobs.append(calls_command(os.path.join(tmp, "calls.so")))
         workers = max(1, min(len(jobs), os.cpu_count() or 1, 8))
         with concurrent.futures.ThreadPoolExecutor(max_workers=workers) as pool:
             for f in [pool.submit(_run, j, verbose) for j in jobs]:
                 f.result()
         _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", LIB_PATH + ".tmp"], verbose)
+        shutil.copyfile(os.path.join(tmp, "calls.so"), CALLS_PATH + ".tmp")
+    os.replace(CALLS_PATH + ".tmp", CALLS_PATH)
     os.replace(LIB_PATH + ".tmp", LIB_PATH)
     return LIB_PATH
 

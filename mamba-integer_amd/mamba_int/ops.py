@@ -474,88 +474,27 @@ def embed_argmax(keys, ids_out, emb, r, row_stats) -> None:
 
 # -------------------------------------------- float operators (forward only)
 # Rows may be strided views (a half of in_proj's rows, slices of x_proj's): only
-# the elements of a row must be adjacent.  A call on inputs that require
-# gradients is refused while autograd records: these operators have no backward.
+# the elements of a row must be adjacent.  Inputs that require gradients are
+# refused while autograd records: these operators have no backward.  The tensors'
+# checks, the outputs and the call are csrc/float_calls.cpp's.
 _FLOAT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_ACTIVATIONS = {None: 0, "none": 0, "silu": 1}
 
 
-def _float_type(t: torch.Tensor, name: str) -> int:
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    code = _FLOAT.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    return code
-
-
-def _rows(t: torch.Tensor, shape, dtype: torch.dtype, name: str, out: bool = False):
-    """A tensor of rows as (address, row stride[, sequence stride]); the leading
-    dimensions may have any strides, the elements of a row are adjacent."""
-    _like(t, shape, dtype, name)
-    st = t.stride()
-    if st[-1] != 1 and shape[-1] > 1:
-        raise ValueError(f"{name}: the elements of a row must be adjacent (strides {st})")
-    if not out:
-        return (t.data_ptr(), st[1], st[0]) if len(st) == 3 else (t.data_ptr(), st[0])
-    # rows that overlap would be written twice: each must end before the next begins
-    span = shape[-1]
-    for size, stride in zip(reversed(shape[:-1]), reversed(st[:-1])):
-        if size > 1 and stride < span:
-            raise ValueError(f"{name}: output rows overlap (strides {st})")
-        span = max(span, stride * size)
-    # (the stride of a dimension of one element is free: the library asks for a row's length)
-    ld = st[-2] if shape[-2] > 1 else shape[-1]
-    return (t.data_ptr(), ld, st[0] if shape[0] > 1 else 0) if len(st) == 3 else (t.data_ptr(), ld)
-
-
-def _like(t: torch.Tensor, shape, dtype: torch.dtype, name: str) -> None:
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype is not dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a device tensor (libmamba_int has no host path)")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient; the float operators are forward only")
-
-
-def _vec(t: Optional[torch.Tensor], shape, dtype: torch.dtype, name: str):
-    """Address of a contiguous tensor of this shape (None: NULL)."""
-    if t is None:
-        return None
-    _like(t, shape, dtype, name)
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
-
-
-def _address(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+@functools.lru_cache(maxsize=None)
+def _calls():
+    lib = _lib.load()
+    from . import _float_calls     # built with the library: its absence is an error
+    entries = ("mi_add_rms_norm", "mi_causal_conv", "mi_selective_scan_workspace_size", "mi_selective_scan",
+               "mi_w4_matvec", "mi_last_error_string")
+    _float_calls.init(_lib.MIError, *(ctypes.cast(getattr(lib, e), ctypes.c_void_p).value for e in entries))
+    return _float_calls
 
 
 def _raw_stream() -> int:
-    """The current stream's handle, without a stream object around it (2.8 us less)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
-
-
-def _norm(x, weight, residual, eps, residual_out, y, q, scale):
-    code = _float_type(x, "x")
-    shape = x.shape
-    if len(shape) != 2:
-        raise ValueError(f"x must be [tokens, dim], got {tuple(shape)}")
-    rtype = residual.dtype if residual is not None else residual_out.dtype if residual_out is not None else x.dtype
-    rcode = _FLOAT.get(rtype, -1)
-    if rtype is not x.dtype and rtype is not torch.float32:
-        raise TypeError(f"the residual must be {x.dtype} or float32, got {rtype}")
-    xp, ldx = _rows(x, shape, x.dtype, "x")
-    rp, ldr = _rows(residual, shape, rtype, "residual") if residual is not None else (None, 0)
-    op, ldo = _rows(residual_out, shape, rtype, "residual_out", True) if residual_out is not None else (None, 0)
-    yp, ldy = _rows(y, shape, x.dtype, "out", True) if y is not None else (None, 0)
-    qp, ldq, sp = (q.data_ptr(), q.stride(0), scale.data_ptr()) if q is not None else (None, 0, None)
-    _lib.call("mi_add_rms_norm", xp, code, ldx, rp, rcode, ldr, _vec(weight, shape[1:], torch.float32, "weight"),
-              eps, yp, ldy, qp, ldq, sp, op, ldo, shape[0], shape[1], _raw_stream())
+    """The current stream's handle, without a stream object around it (2.8 us less);
+    0 where there is no device (every call then refuses its tensors)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) if torch.cuda.is_initialized() else 0
 
 
 def add_rms_norm(x, weight, residual=None, eps: float = 1e-5, residual_out=None, out=None):
@@ -563,32 +502,16 @@ def add_rms_norm(x, weight, residual=None, eps: float = 1e-5, residual_out=None,
     (normed rows in x's type, s in the residual's type).  weight float32 [d]; the residual
     has x's type or float32 (None: s = x, returned only if ``residual_out`` is passed, else
     None).  ``residual_out`` may be the residual itself, ``out`` may be x.  Forward only."""
-    _float_type(x, "x")
-    y = out if out is not None else x.new_empty(x.shape)
-    if residual is not None and residual_out is None:
-        residual_out = residual.new_empty(residual.shape)
-    _norm(x, weight, residual, eps, residual_out, y, None, None)
-    return y, residual_out
+    return _calls().add_rms_norm(_raw_stream(), x, weight, residual, eps, residual_out, out, 0)
 
 
 def add_rms_norm_quant(x, weight, residual=None, eps: float = 1e-5, residual_out=None, unit: int = 64):
     """``add_rms_norm`` with the normed rows in 8 bits: returns (q int8 [T, dp], scale float32
     [T], s), dp = d rounded up to ``unit`` (zeros from d on): the rows ``bitlinear`` OUT_FLOAT
     reads with ``x_scale=scale``, bit-identical to ``act_quant`` of the float32 norm."""
-    if not isinstance(x, torch.Tensor) or x.dim() != 2:
-        raise ValueError("x must be a tensor [tokens, dim]")
     if unit < 1:
         raise ValueError(f"unit={unit} must be at least 1")
-    T, d = x.shape
-    q = x.new_empty((T, -(-d // unit) * unit), dtype=torch.int8)
-    scale = x.new_empty((T,), dtype=torch.float32)
-    if residual is not None and residual_out is None:
-        residual_out = residual.new_empty(residual.shape)
-    _norm(x, weight, residual, eps, residual_out, None, q, scale)
-    return q, scale, residual_out
-
-
-_ACTIVATIONS = {None: 0, "none": 0, "silu": 1}
+    return _calls().add_rms_norm(_raw_stream(), x, weight, residual, eps, residual_out, None, unit)
 
 
 def causal_conv(x, weight, bias=None, activation: Optional[str] = "silu", state_in=None, state_out=None, lens=None,
@@ -598,31 +521,9 @@ def causal_conv(x, weight, bias=None, activation: Optional[str] = "silu", state_
     [B, W-1, D] of x's type: the inputs before x (None: zeros) and the last ones after it
     (may be the same tensor); L = 1 is a decode step.  lens int32 [B]: tokens of each
     sequence, the rows of the output past them are zero.  Forward only."""
-    code = _float_type(x, "x")
-    if x.dim() != 3:
-        raise ValueError(f"x must be [batch, len, dim], got {tuple(x.shape)}")
-    B, L, D = shape = x.shape
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be 'silu' or None, got {activation!r}")
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
-        raise ValueError("weight must be a tensor [dim, width]")
-    W = weight.shape[1]
-    y = out if out is not None else x.new_empty(shape)
-    xp, ldx, bsx = _rows(x, shape, x.dtype, "x")
-    yp, ldy, bsy = _rows(y, shape, x.dtype, "out", True)
-    st = (B, W - 1, D)
-    _lib.call("mi_causal_conv", xp, ldx, bsx, code, _vec(weight, (D, W), torch.float32, "weight"),
-              _vec(bias, (D,), torch.float32, "bias"), W, _ACTIVATIONS[activation],
-              _vec(state_in, st, x.dtype, "state_in"), _vec(state_out, st, x.dtype, "state_out"),
-              _vec(lens, (B,), torch.int32, "lens"), yp, ldy, bsy, B, L, D, _raw_stream())
-    return y
-
-
-@functools.lru_cache(maxsize=256)
-def _scan_workspace(B: int, L: int, D: int, N: int, G: int) -> int:
-    n = ctypes.c_size_t()
-    _lib.call("mi_selective_scan_workspace_size", B, L, D, N, G, ctypes.byref(n))
-    return n.value
+    return _calls().causal_conv(_raw_stream(), x, weight, bias, _ACTIVATIONS[activation], state_in, state_out, lens, out)
 
 
 def selective_scan(u, dt, a, b, c, d_skip=None, z=None, dt_bias=None, dt_softplus: bool = True, h_in=None, h_out=None,
@@ -633,43 +534,7 @@ def selective_scan(u, dt, a, b, c, d_skip=None, z=None, dt_bias=None, dt_softplu
     a float32 [D, N], d_skip, dt_bias float32 [D]; h_in / h_out float32 [B, D, N] (None: zeros;
     may be the same tensor); L = 1 is a decode step.  lens int32 [B]: tokens of each sequence
     (h_out: the state after them; rows of the output past them are zero).  Forward only."""
-    code = _float_type(u, "u")
-    if u.dim() != 3:
-        raise ValueError(f"u must be [batch, len, dim], got {tuple(u.shape)}")
-    typ = u.dtype
-    B, L, D = shape = u.shape
-    if not isinstance(a, torch.Tensor) or a.dim() != 2:
-        raise ValueError("a must be a tensor [dim, states]")
-    N = a.shape[1]
-    G = 1
-    if isinstance(b, torch.Tensor) and b.dim() == 4:
-        G = b.shape[2]
-    rows = []
-    for name, t in (("b", b), ("c", c)):
-        if isinstance(t, torch.Tensor) and t.dim() == 4:
-            if t.shape != (B, L, G, N):
-                raise ValueError(f"{name} must be {(B, L, G, N)}, got {tuple(t.shape)}")
-            if G > 1 and t.stride(2) != N or N > 1 and t.stride(3) != 1:
-                raise ValueError(f"{name}: the groups of a row must be adjacent (strides {t.stride()})")
-            t = t[:, :, 0] if G == 1 else t.as_strided((B, L, G * N), (t.stride(0), t.stride(1), 1))
-        rows.append(_rows(t, (B, L, G * N), typ, name))
-    y = out if out is not None else u.new_empty(shape)
-    st = (B, D, N)
-    size = _scan_workspace(B, L, D, N, G)
-    ws = u.new_empty(size, dtype=torch.uint8) if size else None
-    _lib.call("mi_selective_scan", *_rows(u, shape, typ, "u"), *_rows(dt, shape, typ, "dt"),
-              _vec(a, (D, N), torch.float32, "a"), *rows[0], *rows[1], _vec(d_skip, (D,), torch.float32, "d_skip"),
-              *(_rows(z, shape, typ, "z") if z is not None else (None, 0, 0)),
-              _vec(dt_bias, (D,), torch.float32, "dt_bias"), int(dt_softplus), _vec(h_in, st, torch.float32, "h_in"),
-              _vec(h_out, st, torch.float32, "h_out"), _vec(lens, (B,), torch.int32, "lens"),
-              *_rows(y, shape, typ, "out", True), code, B, L, D, N, G, _address(ws), size, _raw_stream())
-    return y
-
-
-def _w4_groups(k: int, group: int) -> int:
-    if not (group in (32, 64) or group > 0 and group % 128 == 0):
-        raise ValueError(f"group={group} must be 32, 64 or a multiple of 128")
-    return -(-k // 128) * 128 // group if group < 128 else -(-k // group)
+    return _calls().selective_scan(_raw_stream(), u, dt, a, b, c, d_skip, z, dt_bias, dt_softplus, h_in, h_out, lens, out)
 
 
 def pack_w4(codes, scales, group: int, zeros=None):
@@ -680,37 +545,28 @@ def pack_w4(codes, scales, group: int, zeros=None):
     _req(codes, torch.uint8, "codes")
     if codes.dim() != 2:
         raise ValueError(f"codes must be [n, k], got {tuple(codes.shape)}")
+    if not (group in (32, 64) or group > 0 and group % 128 == 0):
+        raise ValueError(f"group={group} must be 32, 64 or a multiple of 128")
+    if not isinstance(scales, torch.Tensor) or scales.dtype not in _FLOAT:
+        raise TypeError("scales must be a float32, bfloat16 or float16 tensor")
     n, k = codes.shape
-    ng, have = _w4_groups(k, group), -(-k // group)
-    _float_type(scales, "scales")
+    nb, kb, have = -(-n // 16), -(-k // 128), -(-k // group)
+    ng = kb * 128 // group if group < 128 else have
     if scales.dtype != torch.float16:
         scales = scales.float()
     st = scales.dtype
-    nb, kb = -(-n // 16), -(-k // 128)
+    for name, t, dtype in (("scales", scales, st), ("zeros", zeros, torch.uint8)):
+        if t is not None and _req(t, dtype, name).shape != (n, have):
+            raise ValueError(f"{name} must be {(n, have)}, got {tuple(t.shape)}")
     packed = torch.empty((nb, kb, 1024), dtype=torch.uint8, device=codes.device)
     s_out = torch.empty((nb, ng, 16), dtype=st, device=codes.device)
     z_out = torch.empty((nb, ng, 16), dtype=torch.uint8, device=codes.device) if zeros is not None else None
-    _lib.call("mi_pack_w4", codes.data_ptr(), _vec(scales, (n, have), st, "scales"), _FLOAT[st],
-              _vec(zeros, (n, have), torch.uint8, "zeros"), packed.data_ptr(), s_out.data_ptr(), _ptr(z_out), n, k, group,
-              _raw_stream())
+    _lib.call("mi_pack_w4", _ptr(codes), _ptr(scales), _FLOAT[st], _ptr(zeros), _ptr(packed), _ptr(s_out), _ptr(z_out), n,
+              k, group, _stream())
     return packed, s_out, z_out
 
 
 def w4_matvec(x, packed, scales, n: int, group: int, zeros=None, bias=None, out=None):
     """y [M, n] = x [M, K] @ W^T (+ bias float32 [n]) for the 4-bit weights of ``pack_w4``:
     made for the rows of a decode step (1..64; more are computed too).  Forward only."""
-    code = _float_type(x, "x")
-    if x.dim() != 2:
-        raise ValueError(f"x must be [rows, k], got {tuple(x.shape)}")
-    M, k = x.shape
-    nb = -(-n // 16)
-    st = scales.dtype if isinstance(scales, torch.Tensor) else None
-    if st is not torch.float16 and st is not torch.float32:
-        raise TypeError(f"scales must be a float16 or float32 tensor, got {st}")
-    vals = (nb, _w4_groups(k, group), 16)
-    y = out if out is not None else x.new_empty((M, n))
-    _lib.call("mi_w4_matvec", *_rows(x, x.shape, x.dtype, "x"), code,
-              _vec(packed, (nb, -(-k // 128), 1024), torch.uint8, "packed"), _vec(scales, vals, st, "scales"), _FLOAT[st],
-              _vec(zeros, vals, torch.uint8, "zeros"), _vec(bias, (n,), torch.float32, "bias"),
-              *_rows(y, (M, n), x.dtype, "out", True), M, n, k, group, _raw_stream())
-    return y
+    return _calls().w4_matvec(_raw_stream(), x, packed, scales, n, group, zeros, bias, out)

@@ -107,38 +107,14 @@ def test_host_tensors_and_wrong_types_are_refused():
         ops.selective_scan(x[None], x[None], w, x[None], x[None])
     with pytest.raises(ValueError, match="b must be"):
         ops.selective_scan(x[None], x[None], torch.zeros(8, 4), torch.zeros(1, 2, 1, 5), torch.zeros(1, 2, 4))
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        ops.causal_conv([1.0], torch.zeros(8, 4))
     with pytest.raises(TypeError, match="scales"):
         ops.w4_matvec(x, None, w.double(), 4, 32)
     with pytest.raises(ValueError, match="group"):
         ops.w4_matvec(x, None, w, 4, 48)
     with pytest.raises(ValueError, match="device"):
         ops.pack_w4(torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 2), 32)
-
-
-def test_row_strides():
-    """Which views are rows: adjacent elements, outputs that do not overlap."""
-    from mamba_int import ops
-
-    class Dev(torch.Tensor):
-        is_cuda = True
-
-    def rows(t, **k):
-        return ops._rows(t.as_subclass(Dev), t.shape, t.dtype, "t", **k)[1:]
-    x = torch.zeros(3, 4, 10)
-    assert rows(x) == (10, 40) and rows(x[..., :4], out=True) == (10, 40) and rows(x[:, 1:3], out=True) == (10, 40)
-    assert rows(x[:1], out=True) == (10, 0) and rows(x[:, :1], out=True) == (10, 40)
-    assert rows(x[0, :1].expand(4, 10)) == (0,)
-    for bad in (x.transpose(1, 2), x[..., ::2]):
-        with pytest.raises(ValueError, match="adjacent"):
-            rows(bad)
-    for bad in (x[:, :1].expand(3, 4, 10), x[:1].expand(3, 4, 10), x.as_strided((3, 4, 10), (10, 10, 1))):
-        with pytest.raises(ValueError, match="overlap"):
-            rows(bad, out=True)
-    w = torch.zeros(3, 4, requires_grad=True)
-    with pytest.raises(ValueError, match="forward only"):
-        rows(w)
-    with torch.no_grad():
-        assert rows(w) == (4,)
 
 
 def test_oracle_against_brute_force():
