@@ -358,8 +358,8 @@ extern "C" mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const ui
     if (m == 0 || n == 0) return MI_OK;
     MI_REQUIRE(x && packed && scales && y, MI_ERR_NULL_POINTER, "mi_w4_matvec: x, packed, scales and y are required");
     MI_REQUIRE(aligned(packed, 16), MI_ERR_BAD_ALIGNMENT, "mi_w4_matvec: packed must be 16-byte aligned");
-    MI_REQUIRE((int64_t)m * n < ((int64_t)1 << 31) && m <= 32 * 65535, MI_ERR_BAD_DIM,
-               "mi_w4_matvec: m * n must be below 2^31, and m at most 32 * 65535");
+    MI_REQUIRE((int64_t)m * n < ((int64_t)1 << 31) && m <= 32 * 65535 && n <= 1 << 28, MI_ERR_BAD_DIM,
+               "mi_w4_matvec: m * n must be below 2^31, m at most 32 * 65535 and n at most 2^28");
     const hipStream_t st = as_stream(stream);
     with_type(type, [&](auto t) {
         using T = decltype(t);

@@ -50,7 +50,8 @@ def pack(c=A, s=A, st=2, z=None, p=A, so=A, zo=None, n=16, k=128, g=128):
     (scan(B=1 << 23, D=8), 2, "2^25"), (scan(a=None), 1, "required"), (scan(u=None), 1, "required"),
     (w4(k=0), 2, "k=0"), (w4(g=48), 4, "group"), (w4(g=192), 4, "group"), (w4(g=0), 4, "group"), (w4(g=-128), 4, "group"),
     (w4(t=7), 4, "type"), (w4(st=1), 4, "scales"), (w4(ldy=15), 2, "ldy"), (w4(p=X), 3, "aligned"), (w4(p=None), 1, "required"),
-    (w4(y=None), 1, "required"), (w4(m=1 << 20, n=1 << 11, ldy=1 << 11), 2, "2^31"),
+    (w4(y=None), 1, "required"), (w4(m=1 << 20, n=1 << 11, ldy=1 << 11), 2, "2^31"), (w4(n=(1 << 28) + 1, ldy=1 << 30), 2, "2^28"),
+    (w4(m=32 * 65535 + 1), 2, "65535"),
     (pack(n=-1), 2, "negative"), (pack(g=16), 4, "group"), (pack(st=1), 4, "scales"), (pack(c=None), 1, "required"),
     (pack(z=A), 1, "zeros"), (pack(p=X), 3, "aligned"),
 ])
