@@ -61,12 +61,25 @@ __device__ __forceinline__ void conv_rows(const ConvArgs<T> &a, int64_t b, int c
         return v;
     };
     float w[W][V], bias[V], win[W][V];
+    if (FULL) {
+        // the channels' taps are adjacent: one run of 16-byte loads
+        const Packed<float, V * W> wp = load_packed<V * W>(a.w + (int64_t)c * W);
+        Packed<float, V> bp;
+        if (a.bias) bp = load_packed<V>(a.bias + c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int ci = FULL ? c + i : min(c + i, a.dim - 1);
-        bias[i] = a.bias ? a.bias[ci] : 0.0f;
+        for (int i = 0; i < V; ++i) {
+            bias[i] = a.bias ? bp.v[i] : 0.0f;
 #pragma unroll
-        for (int j = 0; j < W; ++j) w[j][i] = a.w[(int64_t)ci * W + j];
+            for (int j = 0; j < W; ++j) w[j][i] = wp.v[i * W + j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int ci = min(c + i, a.dim - 1);
+            bias[i] = a.bias ? a.bias[ci] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < W; ++j) w[j][i] = a.w[(int64_t)ci * W + j];
+        }
     }
     const int end = min(t1, n);
     Packed<T, V> next[kSteps];

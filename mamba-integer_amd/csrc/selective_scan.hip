@@ -15,6 +15,8 @@ namespace mi {
 constexpr int kScanMaxStates = 256, kScanStepLen = 4;
 constexpr int64_t kScanMaxLd = (int64_t)1 << 25;   // 16 rows' offsets in 32 bits
 
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f, kMaxFloat = 3.402823466e38f;
+
 template <class T>
 struct ScanArgs {
     Rows<const T> u, dt, b, c, z;
@@ -105,10 +107,73 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs<T> a) {
     }
 }
 
+// One token: as above, over kSeqs sequences a thread, which share the channel's A, bias
+// and skip, and whose states' loads are all in flight together.  Bound by the states,
+// read and written once.
+constexpr int kSeqs = 2;
+
+template <class T, int LANES>
+__global__ __launch_bounds__(256) void scan_token_kernel(ScanArgs<T> a) {
+    const uint32_t id = (blockIdx.x * 256 + threadIdx.x) / LANES, all = (uint32_t)a.dim * (uint32_t)((a.batch + kSeqs - 1) / kSeqs);
+    const int lane = threadIdx.x % LANES, N = a.nstate, n0 = min(4 * lane, N - 4);
+    const bool on = id < all, mine = 4 * lane < N;
+    const uint32_t ch = on ? id : all - 1;
+    const uint32_t b0 = ch / (uint32_t)a.dim * kSeqs;
+    const int c = (int)(ch % (uint32_t)a.dim);
+    const int64_t g0 = (int64_t)(c / (a.dim / a.groups)) * N + n0;
+    Packed<float, 4> h[kSeqs];
+    Packed<T, 4> bn[kSeqs], cn[kSeqs];
+    T u[kSeqs], dt[kSeqs], z[kSeqs];
+    int64_t b[kSeqs], at[kSeqs];
+#pragma unroll
+    for (int s = 0; s < kSeqs; ++s) {
+        b[s] = min((int)b0 + s, a.batch - 1);
+        at[s] = (b[s] * a.dim + c) * N + n0;
+        if (a.h_in) h[s] = load_packed<4>(a.h_in + at[s]);
+        u[s] = a.u.row(b[s], 0)[c];
+        dt[s] = a.dt.row(b[s], 0)[c];
+        bn[s] = load_packed<4>(a.b.row(b[s], 0) + g0);
+        cn[s] = load_packed<4>(a.c.row(b[s], 0) + g0);
+        if (a.z.p) z[s] = a.z.row(b[s], 0)[c];
+    }
+    const Packed<float, 4> am = load_packed<4>(a.a + (int64_t)c * N + n0);
+    const float bias = a.dt_bias ? a.dt_bias[c] : 0.0f, skip = a.d_skip ? a.d_skip[c] : 0.0f;
+#pragma unroll
+    for (int s = 0; s < kSeqs; ++s) {
+        const bool run = scan_len(a.lens, b[s], 1) != 0;
+        const float uf = (float)u[s];
+        float d = (float)dt[s] + bias;
+        if (a.softplus) d = softplus(d);
+        const float du = d * uf;
+        float y = 0.0f;
+        Packed<float, 4> next;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float was = a.h_in ? h[s].v[i] : 0.0f;
+            const float now = __builtin_fmaf(__builtin_amdgcn_exp2f(kLog2e * (d * am.v[i])), was, du * (float)bn[s].v[i]);
+            y = __builtin_fmaf((float)cn[s].v[i], now, y);
+            next.v[i] = run ? now : was;
+        }
+        if (!mine) y = 0.0f;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) y += __shfl_xor(y, o);
+        if (!on || (int)b0 + s >= a.batch) continue;
+        if (a.h_out && mine) store_packed<4>(a.h_out + at[s], next);
+        if (lane == 0) {
+            y = __builtin_fmaf(skip, uf, y);
+            if (a.z.p) y *= silu((float)z[s]);
+            a.y.row(b[s], 0)[c] = (T)(run ? y : 0.0f);
+        }
+    }
+}
+
 template <class T, int LANES>
 void launch_scan_step(const ScanArgs<T> &a, hipStream_t st) {
     const dim3 grid((unsigned)(((int64_t)a.batch * a.dim * LANES + 255) / 256));
-    if (a.nstate % 4 == 0)
+    if (a.len == 1 && a.nstate % 4 == 0)
+        hipLaunchKernelGGL((scan_token_kernel<T, LANES>),
+                           dim3((unsigned)(((int64_t)((a.batch + kSeqs - 1) / kSeqs) * a.dim * LANES + 255) / 256)), dim3(256), 0, st, a);
+    else if (a.nstate % 4 == 0)
         hipLaunchKernelGGL((scan_step_kernel<T, LANES, true>), grid, dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((scan_step_kernel<T, LANES, false>), grid, dim3(256), 0, st, a);
@@ -181,8 +246,6 @@ struct ScanSplit {
     float *ends;
     int chunks, chunk, blocks;   // blocks: of 64 channels, a group
 };
-
-constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f, kMaxFloat = 3.402823466e38f;
 
 // kHelpers waves of a block turn rows into a tile's d, d u, B and C in LDS and the
 // recurring waves' parts of y into output rows, one tile ahead and one behind.
