@@ -242,8 +242,8 @@ __device__ __forceinline__ void static_for(F &&f) {
 
 // The steps of a sequence in `chunks` parts of `chunk` steps: kWhole is one part;
 // kEnds computes each part's last state from zero and its sum of d (into ends,
-// [batch, chunks, nstate + 1, dim]); kParts starts each part from the states in
-// front of it, joined from those.
+// [batch, chunks, nstate + 1, dim], the last part's place holding the sequence's first
+// state); kParts starts each part from the states in front of it, joined from those.
 enum ScanPass { kWhole, kEnds, kParts };
 
 struct ScanSplit {
@@ -287,10 +287,23 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
             const int n = n0 + i;
             float v = n < N ? a.a[(int64_t)c * N + n] : 0.0f;
             am[i / 4][i % 4] = v < -kMaxFloat ? -kMaxFloat : v;  // (a step of 0 then keeps the state whatever a is)
-            h[i / 4][i % 4] = PASS != kEnds && a.h_in && n < N ? a.h_in[(b * a.dim + c) * N + n] : 0.0f;
+            h[i / 4][i % 4] = 0.0f;
+            if (PASS != kParts && k == 0 && a.h_in && n < N) h[i / 4][i % 4] = a.h_in[(b * a.dim + c) * N + n];
+        }
+        if (PASS == kEnds && k == 0) {
+            // the second pass reads the first state here: h_out, which it writes, may be h_in
+            float *e = sp.ends + (b * sp.chunks + sp.chunks - 1) * (N + 1) * a.dim + c;
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                if (on && n0 + i < N) e[(int64_t)(n0 + i) * a.dim] = h[i / 4][i % 4];
+                h[i / 4][i % 4] = 0.0f;
+            }
         }
         if (PASS == kParts) {
             const float *e = sp.ends + b * sp.chunks * (N + 1) * a.dim + c;
+            const float *first = e + (int64_t)(sp.chunks - 1) * (N + 1) * a.dim;
+#pragma unroll
+            for (int i = 0; i < S; ++i) h[i / 4][i % 4] = n0 + i < N ? first[(int64_t)(n0 + i) * a.dim] : 0.0f;
             for (int j = 0; j < k; ++j, e += (int64_t)(N + 1) * a.dim) {
                 const float sum = e[(int64_t)N * a.dim];
 #pragma unroll
@@ -564,6 +577,7 @@ extern "C" mi_status mi_selective_scan_workspace_size(int batch, int len, int di
     MI_REQUIRE(bytes, MI_ERR_NULL_POINTER, "mi_selective_scan_workspace_size: bytes is required");
     MI_REQUIRE(batch >= 0 && len >= 0 && dim >= 0 && nstate >= 1 && nstate <= kScanMaxStates, MI_ERR_BAD_DIM,
                "mi_selective_scan_workspace_size: a size is negative, or nstate=%d not in [1, %d]", nstate, kScanMaxStates);
+    MI_REQUIRE(len <= 1 << 30, MI_ERR_BAD_DIM, "mi_selective_scan_workspace_size: len must be at most 2^30");
     MI_REQUIRE(groups >= 1 && dim % groups == 0, MI_ERR_BAD_DIM, "mi_selective_scan_workspace_size: groups=%d must divide dim=%d",
                groups, dim);
     *bytes = 0;
@@ -592,6 +606,8 @@ extern "C" mi_status mi_selective_scan(const void *u, int64_t ldu, int64_t bsu, 
                MI_ERR_BAD_DIM, "mi_selective_scan: a stride is negative, or ldy is less than dim");
     MI_REQUIRE((int64_t)batch * dim <= ((int64_t)1 << 25), MI_ERR_BAD_DIM,
                "mi_selective_scan: batch * dim must be at most 2^25");
+    MI_REQUIRE(len <= 1 << 30 && (int64_t)groups * nstate <= kScanMaxLd, MI_ERR_BAD_DIM,
+               "mi_selective_scan: len must be at most 2^30, groups * nstate at most %lld", (long long)kScanMaxLd);
     if (batch == 0 || dim == 0) return MI_OK;
     MI_REQUIRE(a && (len == 0 || (u && dt && b && c && y)), MI_ERR_NULL_POINTER,
                "mi_selective_scan: u, dt, a, b, c and y are required");

@@ -83,6 +83,18 @@ def test_long(cuda, B, L, D, N):
     check(s, got, h, torch.float32)
 
 
+def test_long_state_in_place(cuda):
+    """The state in place where the sequence is split: its parts read the first state, the
+    last one writes the new one."""
+    s = make(1, 2000, 200, 16, 1, torch.float32, 8)
+    want, h = run(s, cuda)
+    check(s, want, h, torch.float32)
+    for _ in range(5):
+        state = s["h_in"].to(cuda)
+        got, _ = run(s, cuda, h_in=state, h_out=state)
+        assert torch.equal(got, want) and torch.equal(state, h)
+
+
 def test_parts_and_steps(cuda):
     """A prompt in parts and then token by token, the state in place, is the prompt at once."""
     from mamba_int import ops
