@@ -152,9 +152,10 @@ mi_status launch_conv(const ConvArgs<T> &a, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);
     const int64_t cols = (a.dim + V - 1) / V, rows = (int64_t)a.batch * cols;
     // rows a thread: the W - 1 in front of them are read twice, so as many as leave
-    // four waves a SIMD
+    // four waves a SIMD; at least W - 1, so that only the first rows' thread, which writes
+    // state_out, reads state_in
     int steps = 32;
-    while (steps > 4 && rows * ((a.len + steps - 1) / steps) < (int64_t)device_cus() * 4 * 4 * 64) steps /= 2;
+    while (steps > (W <= 5 ? 4 : 8) && rows * ((a.len + steps - 1) / steps) < (int64_t)device_cus() * 4 * 4 * 64) steps /= 2;
     const int tiles = a.len > 0 ? (a.len + steps - 1) / steps : 1;
     const int64_t threads = rows * tiles;
     MI_REQUIRE(threads < ((int64_t)1 << 32) - 256, MI_ERR_BAD_DIM, "mi_causal_conv: batch * len * dim is too large");
@@ -191,7 +192,8 @@ extern "C" mi_status mi_causal_conv(const void *x, int64_t ldx, int64_t bsx, int
     MI_REQUIRE(known_type(type), MI_ERR_BAD_ARG, "mi_causal_conv: unknown element type %d", type);
     MI_REQUIRE(ldx >= 0 && bsx >= 0 && ldy >= dim && bsy >= 0, MI_ERR_BAD_DIM,
                "mi_causal_conv: a stride is negative, or ldy is less than dim");
-    MI_REQUIRE((int64_t)batch * dim < ((int64_t)1 << 31), MI_ERR_BAD_DIM, "mi_causal_conv: batch * dim must be below 2^31");
+    MI_REQUIRE((int64_t)batch * dim < ((int64_t)1 << 31) && len <= 1 << 30, MI_ERR_BAD_DIM,
+               "mi_causal_conv: batch * dim must be below 2^31, and len at most 2^30");
     if (batch == 0 || dim == 0) return MI_OK;
     MI_REQUIRE(w && (len == 0 || (x && y)), MI_ERR_NULL_POINTER, "mi_causal_conv: x, w and y are required");
     const hipStream_t st = as_stream(stream);

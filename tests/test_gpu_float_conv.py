@@ -87,6 +87,19 @@ def test_state_in_place_and_steps(cuda, L):
     assert torch.equal(st.cpu(), last)
 
 
+@pytest.mark.parametrize("W", [5, 6, 8])
+def test_wide_state_in_place(cuda, W):
+    """As many rows of state as a thread walks: only the thread that writes it reads it."""
+    from mamba_int import ops
+    x, w, bias, st, _ = make(2, 61, 72, W, torch.float32, W)
+    y, err, last = R.conv(x, w, bias, True, st, None)
+    for _ in range(5):
+        state = st.to(cuda)
+        R.close(ops.causal_conv(x.to(cuda), w.to(cuda), bias=bias.to(cuda), state_in=state, state_out=state), y, err,
+                torch.float32)
+        assert torch.equal(state.cpu(), last)
+
+
 def test_masked_rows_are_not_read_as_values(cuda):
     from mamba_int import ops
     x, w, bias, st, _ = make(3, 20, 64, 4, torch.float32, 2)
