@@ -545,7 +545,8 @@ mi_status mi_add_rms_norm(const void *x, int x_type, int64_t ldx, const void *re
  * (NULL: zeros), and the last ones of state_in and the sequence together.
  * lens int32 [batch] nullable: sequence b has lens[b] tokens (clamped to
  * [0, len]); rows of x past them are not used, rows of y past them are zero.
- * len == 0 copies the state.  width in [1, 8]; batch * dim < 2^31. */
+ * len == 0 copies the state.  width in [1, 8]; batch * dim < 2^31, len <=
+ * 2^30. */
 mi_status mi_causal_conv(const void *x, int64_t ldx, int64_t bsx, int type, const float *w, const float *bias,
                          int width, int silu, const void *state_in, void *state_out, const int32_t *lens,
                          void *y, int64_t ldy, int64_t bsy, int batch, int len, int dim, void *stream);
@@ -560,7 +561,8 @@ mi_status mi_causal_conv(const void *x, int64_t ldx, int64_t bsx, int type, cons
  * h_out fp32 [batch,dim,nstate] nullable (NULL h_in: zeros), may be the same.
  * lens as for mi_causal_conv (h_out: the state after lens[b] tokens).
  * workspace: 16-byte aligned, mi_selective_scan_workspace_size bytes (0: may
- * be NULL).  nstate in [1, 256]; batch * dim <= 2^25. */
+ * be NULL).  nstate in [1, 256]; batch * dim, groups * nstate and, for more
+ * than 8 steps, row strides <= 2^25; len <= 2^30. */
 mi_status mi_selective_scan_workspace_size(int batch, int len, int dim, int nstate, int groups,
                                            size_t *bytes);
 mi_status mi_selective_scan(const void *u, int64_t ldu, int64_t bsu, const void *dt, int64_t ldt, int64_t bst,
@@ -585,7 +587,7 @@ mi_status mi_pack_w4(const uint8_t *codes, const void *scales, int scale_type, c
                      uint8_t *packed, void *scales_out, uint8_t *zeros_out, int n, int k, int group,
                      void *stream);
 /* y[m,n] = bias[n] + sum_k x[m,k] * (code[n,k] - zero[n,k/group]) *
- * scale[n,k/group]: x and y rows of `type`, weights as mi_pack_w4 lays them
+ * scale[n,k/group] (n <= 2^28, k <= 2^30): x and y rows of `type`, weights as mi_pack_w4 lays them
  * out (zeros NULL: 8), bias fp32 [n] nullable.  Made for the few rows of a
  * decode step (m up to 64 read the weights once); any m is computed.  A float32
  * or bf16 row with an infinite x gives NaN where the product is infinite. */

@@ -29,6 +29,8 @@ decltype(&mi_w4_matvec) g_w4;
 decltype(&mi_last_error_string) g_last_error;
 PyObject *g_mi_error;   // _lib.MIError
 
+thread_local c10::DeviceIndex t_device;   // of the call's first tensor
+
 struct Raised {};       // a Python error is set
 
 [[noreturn]] void raise(PyObject *type, const char *fmt, ...) {
@@ -85,6 +87,7 @@ const Tensor &like(PyObject *o, at::IntArrayRef shape, at::ScalarType type, cons
     if (t.scalar_type() != type) raise(PyExc_TypeError, "%s must be %s, got %s", name, type_name(type), type_name(t.scalar_type()));
     if (t.sizes() != shape) raise(PyExc_ValueError, "%s must be %s, got %s", name, text(shape).c_str(), text(t.sizes()).c_str());
     if (!t.is_cuda()) raise(PyExc_ValueError, "%s must be a device tensor (libmamba_int has no host path)", name);
+    if (t.device().index() != t_device) raise(PyExc_ValueError, "%s must be on the device of the other tensors", name);
     if (t.requires_grad() && c10::GradMode::is_enabled())
         raise(PyExc_ValueError, "%s requires a gradient; the float operators are forward only", name);
     return t;
@@ -172,6 +175,7 @@ PyObject *add_rms_norm(PyObject *const *a, Py_ssize_t n) {
     count(n, 8, "add_rms_norm");
     const Tensor &x = tensor(a[1], "x");
     const int code = float_type(x, "x");
+    t_device = x.device().index();
     if (x.dim() != 2) raise(PyExc_ValueError, "x must be [tokens, dim], got %s", text(x.sizes()).c_str());
     const int64_t T = x.size(0), d = x.size(1), unit = int_of(a[7]);
     const auto shape = x.sizes();
@@ -214,6 +218,7 @@ PyObject *causal_conv(PyObject *const *a, Py_ssize_t n) {
     count(n, 9, "causal_conv");
     const Tensor &x = tensor(a[1], "x");
     const int code = float_type(x, "x");
+    t_device = x.device().index();
     if (x.dim() != 3) raise(PyExc_ValueError, "x must be [batch, len, dim], got %s", text(x.sizes()).c_str());
     const at::ScalarType type = x.scalar_type();
     const auto shape = x.sizes();
@@ -250,6 +255,7 @@ PyObject *selective_scan(PyObject *const *a, Py_ssize_t n) {
     count(n, 14, "selective_scan");
     const Tensor &u = tensor(a[1], "u");
     const int code = float_type(u, "u");
+    t_device = u.device().index();
     if (u.dim() != 3) raise(PyExc_ValueError, "u must be [batch, len, dim], got %s", text(u.sizes()).c_str());
     const at::ScalarType type = u.scalar_type();
     const auto shape = u.sizes();
@@ -287,6 +293,7 @@ PyObject *w4_matvec(PyObject *const *a, Py_ssize_t n_args) {
     count(n_args, 9, "w4_matvec");
     const Tensor &x = tensor(a[1], "x");
     const int code = float_type(x, "x");
+    t_device = x.device().index();
     if (x.dim() != 2) raise(PyExc_ValueError, "x must be [rows, k], got %s", text(x.sizes()).c_str());
     const int64_t M = x.size(0), k = x.size(1), n = int_of(a[4]), group = int_of(a[5]);
     if (group != 32 && group != 64 && (group <= 0 || group % 128))

@@ -320,6 +320,7 @@ extern "C" mi_status mi_pack_w4(const uint8_t *codes, const void *scales, int sc
                                 void *stream) {
     clear_error();
     MI_REQUIRE(n >= 0 && k >= 0, MI_ERR_BAD_DIM, "mi_pack_w4: negative size");
+    MI_REQUIRE(n <= 1 << 28 && k <= 1 << 30, MI_ERR_BAD_DIM, "mi_pack_w4: n must be at most 2^28, k at most 2^30");
     MI_REQUIRE(w4_group_ok(group), MI_ERR_BAD_ARG, "mi_pack_w4: group=%d must be 32, 64 or a multiple of 128", group);
     MI_REQUIRE(scale_type == MI_F32 || scale_type == MI_F16, MI_ERR_BAD_ARG, "mi_pack_w4: scales are MI_F32 or MI_F16");
     if (n == 0 || k == 0) return MI_OK;
@@ -351,6 +352,7 @@ extern "C" mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const ui
                                   int n, int k, int group, void *stream) {
     clear_error();
     MI_REQUIRE(m >= 0 && n >= 0 && k >= 1, MI_ERR_BAD_DIM, "mi_w4_matvec: a size is negative, or k=%d not positive", k);
+    MI_REQUIRE(k <= 1 << 30, MI_ERR_BAD_DIM, "mi_w4_matvec: k must be at most 2^30");
     MI_REQUIRE(w4_group_ok(group), MI_ERR_BAD_ARG, "mi_w4_matvec: group=%d must be 32, 64 or a multiple of 128", group);
     MI_REQUIRE(known_type(type), MI_ERR_BAD_ARG, "mi_w4_matvec: unknown element type %d", type);
     MI_REQUIRE(scale_type == MI_F32 || scale_type == MI_F16, MI_ERR_BAD_ARG, "mi_w4_matvec: scales are MI_F32 or MI_F16");

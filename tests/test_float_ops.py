@@ -45,6 +45,8 @@ def pack(c=A, s=A, st=2, z=None, p=A, so=A, zo=None, n=16, k=128, g=128):
     (conv(B=-1), 2, "negative"), (conv(width=0), 4, "width"), (conv(width=9), 4, "width"), (conv(t=5), 4, "type"),
     (conv(ldy=7), 2, "ldy"), (conv(bsx=-8), 2, "stride"), (conv(x=None), 1, "required"), (conv(w=None), 1, "required"),
     (conv(B=1 << 20, D=1 << 11, ldx=1 << 11, ldy=1 << 11), 2, "2^31"),
+    (conv(L=(1 << 30) + 1), 2, "2^30"), (scan(L=(1 << 30) + 1), 2, "2^30"), (scan(D=1 << 18, G=1 << 18, N=256, ld=1 << 18, ldy=1 << 18), 2, "groups"),
+    (w4(k=(1 << 30) + 1), 2, "2^30"), (pack(n=(1 << 28) + 1), 2, "2^28"), (scan(ld=1 << 26, L=64), 2, "row stride"),
     (scan(L=-1), 2, "negative"), (scan(N=0), 2, "nstate"), (scan(N=257), 2, "nstate"), (scan(G=3), 2, "groups"),
     (scan(G=0), 2, "groups"), (scan(t=-1), 4, "type"), (scan(ldy=4), 2, "ldy"), (scan(ldz=-1), 2, "stride"),
     (scan(B=1 << 23, D=8), 2, "2^25"), (scan(a=None), 1, "required"), (scan(u=None), 1, "required"),
