@@ -22,30 +22,31 @@ struct ConvArgs {
 };
 
 // The rows [t0, t1) of V channels of a sequence: W - 1 rows before them, then a
-// step for each, kSteps rows loaded ahead.  FULL: V channels; else the channels
-// below a.dim, element by element.
-template <class T, int W, int V, bool FULL>
-__device__ __forceinline__ void conv_rows(const ConvArgs<T> &a, int64_t b, int c, int t0, int t1, int n) {
+// step for each, kSteps rows loaded ahead.  The first `skip` channels belong to the
+// thread before (the last V of a row whose width V does not divide): read and computed
+// with the others (their state may be overwritten meanwhile), not stored.  NARROW: rows
+// of fewer than V channels, element by element.
+template <class T, int W, int V, bool NARROW>
+__device__ __forceinline__ void conv_rows(const ConvArgs<T> &a, int64_t b, int c, int skip, int t0, int t1, int n) {
     constexpr int kSteps = 4;
-    const int have = FULL ? V : a.dim - c;
     auto load = [&](const T *p) {
         Packed<T, V> v;
-        if (FULL) {
+        if (!NARROW) {
             v = load_packed<V>(p);
         } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) v.v[i] = i < have ? p[i] : (T)0.0f;
+            for (int i = 0; i < V; ++i) v.v[i] = i < a.dim ? p[i] : (T)0.0f;
         }
         return v;
     };
     auto store = [&](T *p, const Packed<T, V> &v) {
-        if (FULL) {
+        if (!NARROW && skip == 0) {
             store_packed<V>(p, v);
             return;
         }
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (i < have) p[i] = v.v[i];
+            if (i >= skip && (!NARROW || i < a.dim)) p[i] = v.v[i];
     };
     // row t of the sequence, the state in front of it
     auto row = [&](int t) {
@@ -61,7 +62,7 @@ __device__ __forceinline__ void conv_rows(const ConvArgs<T> &a, int64_t b, int c
         return v;
     };
     float w[W][V], bias[V], win[W][V];
-    if (FULL) {
+    if (!NARROW) {
         // the channels' taps are adjacent: one run of 16-byte loads
         const Packed<float, V * W> wp = load_packed<V * W>(a.w + (int64_t)c * W);
         Packed<float, V> bp;
@@ -75,7 +76,7 @@ __device__ __forceinline__ void conv_rows(const ConvArgs<T> &a, int64_t b, int c
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int ci = min(c + i, a.dim - 1);
+            const int ci = min(i, a.dim - 1);
             bias[i] = a.bias ? a.bias[ci] : 0.0f;
 #pragma unroll
             for (int j = 0; j < W; ++j) w[j][i] = a.w[(int64_t)ci * W + j];
@@ -130,21 +131,18 @@ __device__ __forceinline__ void conv_rows(const ConvArgs<T> &a, int64_t b, int c
 }
 
 // One thread V channels (16 bytes) of `steps` rows of a sequence.
-template <class T, int W>
+template <class T, int W, bool NARROW>
 __global__ __launch_bounds__(256) void causal_conv_kernel(ConvArgs<T> a, int steps, int tiles, int64_t threads) {
     constexpr int V = 16 / sizeof(T);
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= threads) return;
     const int cols = (a.dim + V - 1) / V;
     const int64_t tile = id / cols;
-    const int c = (int)(id - tile * cols) * V;
+    const int first = (int)(id - tile * cols) * V, c = NARROW ? 0 : min(first, a.dim - V);
     const int64_t b = tile / tiles;
     const int t0 = (int)(tile - b * tiles) * steps, t1 = min(a.len, t0 + steps);
     const int n = a.lens ? min(max(a.lens[b], 0), a.len) : a.len;
-    if (c + V <= a.dim)
-        conv_rows<T, W, V, true>(a, b, c, t0, t1, n);
-    else
-        conv_rows<T, W, V, false>(a, b, c, t0, t1, n);
+    conv_rows<T, W, V, NARROW>(a, b, c, first - c, t0, t1, n);
 }
 
 template <class T, int W>
@@ -159,8 +157,11 @@ mi_status launch_conv(const ConvArgs<T> &a, hipStream_t st) {
     const int tiles = a.len > 0 ? (a.len + steps - 1) / steps : 1;
     const int64_t threads = rows * tiles;
     MI_REQUIRE(threads < ((int64_t)1 << 32) - 256, MI_ERR_BAD_DIM, "mi_causal_conv: batch * len * dim is too large");
-    hipLaunchKernelGGL((causal_conv_kernel<T, W>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a, steps,
-                       tiles, threads);
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    if (a.dim < V)
+        hipLaunchKernelGGL((causal_conv_kernel<T, W, true>), grid, dim3(256), 0, st, a, steps, tiles, threads);
+    else
+        hipLaunchKernelGGL((causal_conv_kernel<T, W, false>), grid, dim3(256), 0, st, a, steps, tiles, threads);
     return MI_OK;
 }
 
