@@ -50,11 +50,11 @@ struct W4Args {
     int64_t ldx;
     const uint32_t *packed;
     const S *scales;
-    const uint8_t *zeros;
+    const uint8_t *zeros;   // without zero points any readable bytes, `zeroed` false
     const float *bias;
     T *y;
     int64_t ldy;
-    int m, n, k, group, ng;
+    int m, n, k, group, ng, zeroed;
 };
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -96,7 +96,15 @@ struct W4Type<f16_t> {
     static __device__ __forceinline__ Vec weights(uint32_t w, float zero) {
         const v4u r = {((w << 6) & 0x03c003c0u) | 0x4c004c00u, ((w << 2) & 0x03c003c0u) | 0x4c004c00u,
                        ((w >> 2) & 0x03c003c0u) | 0x4c004c00u, ((w >> 6) & 0x03c003c0u) | 0x4c004c00u};
-        return __builtin_bit_cast(Vec, r) - (f16_t)(16.0f + zero);
+        typedef f16_t v2h __attribute__((ext_vector_type(2)));
+        const v2h off = (f16_t)(-16.0f - zero);
+        v4u o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t pair = r[i];   // (bit_cast of a vector's element itself takes element 0)
+            o[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, pair) + off);
+        }
+        return __builtin_bit_cast(Vec, o);
     }
     static __device__ __forceinline__ void split(const Packed<f16_t, 8> &x, Vec (&o)[1]) {
         o[0] = __builtin_bit_cast(Vec, x);
@@ -143,7 +151,7 @@ struct W4Type<float> {
 // come from a product with ones.
 // The loads of a whole column block stand in no branch (one in a branch is waited for
 // where it ends); the columns past the whole blocks are a last step of their own.
-template <class T, class S, int MT, int NT, int KS>
+template <class T, class S, int MT, int NT, int KS, int PER>
 __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
     using W = W4Type<T>;
     using Vec = typename W::Vec;
@@ -153,8 +161,7 @@ __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
     const int wave = wave_id(), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int nb_all = (a.n + kW4Rows - 1) / kW4Rows, kb_all = (a.k + kW4Cols - 1) / kW4Cols, kb_whole = a.k / kW4Cols;
     const int m0 = blockIdx.y * 16 * MT;
-    const int per = a.group < kW4Cols ? kW4Cols / a.group : 1;             // groups of a column block
-    const int each = a.group < kW4Cols ? 1 : a.group / kW4Cols;            // column blocks of a group
+    const int each = PER > 1 ? 1 : a.group / kW4Cols;                      // column blocks of a group
     const v4u *words[NT];
     const S *scales[NT];
     const uint8_t *zeros[NT];
@@ -163,9 +170,9 @@ __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
         const int64_t nb = min((int)blockIdx.x * NT + nt, nb_all - 1);     // past the last: not stored
         words[nt] = reinterpret_cast<const v4u *>(a.packed) + nb * kb_all * 64 + lane;
         // a lane loads one of the column block's (group, row) values, and gets those it needs from other lanes
-        const int64_t at = nb * a.ng * kW4Rows + (lane & (16 * per - 1));
+        const int64_t at = nb * a.ng * kW4Rows + (lane & (16 * PER - 1));
         scales[nt] = a.scales + at;
-        zeros[nt] = a.zeros ? a.zeros + at : reinterpret_cast<const uint8_t *>(scales[nt]);
+        zeros[nt] = a.zeros + at;
     }
     const T *x[MT];
 #pragma unroll
@@ -176,12 +183,12 @@ __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
         float sj[NT], zj[NT];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (j == 0 || per == 4 || (per == 2 && j == 2)) {
-                const int from = (per == 4 ? 16 * j : per == 2 ? 16 * (j / 2) : 0) + r;
+            if (j % (4 / PER) == 0) {
+                const int from = 16 * (j * PER / 4) + r;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    sj[nt] = per == 1 ? s[nt] : __shfl(s[nt], from);
-                    zj[nt] = per == 1 ? z[nt] : __shfl(z[nt], from);
+                    sj[nt] = PER == 1 ? s[nt] : __shfl(s[nt], from);
+                    zj[nt] = PER == 1 ? z[nt] : __shfl(z[nt], from);
                 }
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
@@ -204,7 +211,7 @@ __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
                     for (int nt = 0; nt < NT; ++nt) d[mt][nt] = mfma(parts[p], wj[nt], d[mt][nt]);
                 }
             }
-            if (j == 3 || per == 4 || (per == 2 && j == 1)) {
+            if ((j + 1) % (4 / PER) == 0) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -213,7 +220,7 @@ __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
             }
         }
     };
-    auto zero_of = [&](uint8_t z) { return a.zeros ? (float)z : 8.0f; };
+    auto zero_of = [&](uint8_t z) { return a.zeroed ? (float)z : 8.0f; };
     for (int kb = wave; kb < kb_whole; kb += KS) {
         v4u w[NT];
         S s[NT];
@@ -222,8 +229,8 @@ __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             w[nt] = words[nt][(int64_t)kb * 64];
-            s[nt] = scales[nt][(int64_t)(kb / each) * (16 * per)];
-            z[nt] = zeros[nt][(int64_t)(kb / each) * (16 * per)];
+            s[nt] = scales[nt][(int64_t)(kb / each) * (16 * PER)];
+            z[nt] = zeros[nt][(int64_t)(kb / each) * (16 * PER)];
         }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -244,8 +251,8 @@ __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             w[nt] = words[nt][(int64_t)kb_whole * 64];
-            s[nt] = (float)scales[nt][(int64_t)(kb_whole / each) * (16 * per)];
-            z[nt] = zero_of(zeros[nt][(int64_t)(kb_whole / each) * (16 * per)]);
+            s[nt] = (float)scales[nt][(int64_t)(kb_whole / each) * (16 * PER)];
+            z[nt] = zero_of(zeros[nt][(int64_t)(kb_whole / each) * (16 * PER)]);
         }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -276,10 +283,16 @@ __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
     }
 }
 
+// PER: groups of a column block (1 for a group of 128 columns and more).
 template <class T, class S, int MT, int NT, int KS>
 void launch_w4(const W4Args<T, S> &a, hipStream_t st) {
     const dim3 grid((unsigned)((a.n + 16 * NT - 1) / (16 * NT)), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
-    hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, KS>), grid, dim3(64 * KS), 0, st, a);
+    if (a.group == 32)
+        hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, KS, 4>), grid, dim3(64 * KS), 0, st, a);
+    else if (a.group == 64)
+        hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, KS, 2>), grid, dim3(64 * KS), 0, st, a);
+    else
+        hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, KS, 1>), grid, dim3(64 * KS), 0, st, a);
 }
 
 // More weight rows a block read x fewer times; fewer leave more blocks.  Measured (us;
@@ -368,8 +381,9 @@ extern "C" mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const ui
         auto go = [&](auto s) {
             using S = decltype(s);
             const W4Args<T, S> a{static_cast<const T *>(x), ldx, reinterpret_cast<const uint32_t *>(packed),
-                                 static_cast<const S *>(scales), zeros, bias, static_cast<T *>(y), ldy, m, n, k, group,
-                                 w4_groups(k, group)};
+                                 static_cast<const S *>(scales),
+                                 zeros ? zeros : static_cast<const uint8_t *>(scales), bias, static_cast<T *>(y), ldy, m, n,
+                                 k, group, w4_groups(k, group), zeros != nullptr};
             launch_w4_shape<T, S>(a, st);
         };
         if (scale_type == MI_F32)
