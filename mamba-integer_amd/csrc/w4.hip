@@ -295,23 +295,28 @@ void launch_w4(const W4Args<T, S> &a, hipStream_t st) {
         hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, KS, 1>), grid, dim3(64 * KS), 0, st, a);
 }
 
-// More weight rows a block read x fewer times; fewer leave more blocks.  Measured (us;
-// 16-bit rows, weights of three sets in turn): 1 x 2048 -> 32000 NT 4, 2, 1: 9.4, 9.4,
-// 10.1 (8 rows 10.4, 11.7, 14.7; 32-bit rows 13.4 with four waves, 14.7, 19.8); 64 x
-// 2048 -> 8192 10.6, 11.8, 19.3; 64 x 2048 -> 2048 8.6, 7.1, 7.2.  64 rows as one tile of
-// x 64 x 2048 -> 8192 12.3, as two of 32 rows, which read the weights twice, 10.6.
+// More weight rows a block read x fewer times; fewer leave more blocks.  Measured (us
+// of a call among others, 6.8 of them the host's; weights of three sets in turn): NT 4, 2
+// and 1, 16-bit rows, 8 x 2048 -> 32000 9.1 to 10.1, 10.5 to 11.4, 14.0; 1 x 2048 -> 8192
+// 8.2 to 9.1, 7.5 to 7.8, 7.1; MT 2 and NT 4, 2: 64 x 2048 -> 8192 9.0 to 9.6 and 12.2; 64
+// x 2048 -> 2048 7.7 and 7.0 to 7.4.  64 rows as one tile of x, 64 x 2048 -> 8192: 11.9 to
+// 12.6, as two of 32 rows, which read the weights twice, 9.0 to 9.6.  Four waves instead of
+// eight where column blocks are fewer than those: 64 x 768 -> 32000 14.7 to
+// 15.3 and 17.8.
 template <class T, class S>
 void launch_w4_shape(const W4Args<T, S> &a, hipStream_t st) {
-    const int nb = (a.n + kW4Rows - 1) / kW4Rows, cus = device_cus();
+    const int nb = (a.n + kW4Rows - 1) / kW4Rows, kb = (a.k + kW4Cols - 1) / kW4Cols, cus = device_cus();
     if (a.m <= 16) {
         if (nb >= 4 * cus)
-            launch_w4<T, S, 1, 4, std::is_same<T, float>::value ? 4 : 8>(a, st);
+            launch_w4<T, S, 1, 4, 8>(a, st);
         else if (nb >= 2 * cus)
             launch_w4<T, S, 1, 2, 8>(a, st);
         else
             launch_w4<T, S, 1, 1, 8>(a, st);
     } else if (a.m <= 32 || nb < 2 * cus) {
         launch_w4<T, S, 2, 2, 8>(a, st);
+    } else if (kb < 8) {
+        launch_w4<T, S, 2, 4, 4>(a, st);
     } else {
         launch_w4<T, S, 2, 4, 8>(a, st);
     }
