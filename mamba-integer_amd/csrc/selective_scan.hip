@@ -282,14 +282,29 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
         // ---- the recurrence: the states n0 .. + S - 1
         const int n0 = wave * S;
         float am[S / 4][4], h[S / 4][4];
+        // a channel's values from n0 on of rows of N states: four at once where N % 4 == 0
+        auto states = [&](const float *p, float (&o)[S / 4][4]) {
+            p += n0;
+#pragma unroll
+            for (int q = 0; q < S / 4; ++q) {
+                if (N % 4 == 0) {
+                    const Packed<float, 4> v = load_packed<4>(p + min(4 * q, N - 4 - n0));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[q][i] = n0 + 4 * q < N ? v.v[i] : 0.0f;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[q][i] = n0 + 4 * q + i < N ? p[4 * q + i] : 0.0f;
+                }
+            }
+        };
+        states(a.a + (int64_t)c * N, am);
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const int n = n0 + i;
-            float v = n < N ? a.a[(int64_t)c * N + n] : 0.0f;
-            am[i / 4][i % 4] = v < -kMaxFloat ? -kMaxFloat : v;  // (a step of 0 then keeps the state whatever a is)
+            float &v = am[i / 4][i % 4];
+            v = v < -kMaxFloat ? -kMaxFloat : v;  // (a step of 0 then keeps the state whatever a is)
             h[i / 4][i % 4] = 0.0f;
-            if (PASS != kParts && k == 0 && a.h_in && n < N) h[i / 4][i % 4] = a.h_in[(b * a.dim + c) * N + n];
         }
+        if (PASS != kParts && k == 0 && a.h_in) states(a.h_in + (b * a.dim + c) * N, h);
         if (PASS == kEnds && k == 0) {
             // the second pass reads the first state here: h_out, which it writes, may be h_in
             float *e = sp.ends + (b * sp.chunks + sp.chunks - 1) * (N + 1) * a.dim + c;
@@ -366,9 +381,17 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
                 if (n0 + i < N) e[(int64_t)(n0 + i) * a.dim] = h[i / 4][i % 4];
             if (wave == 0) e[(int64_t)N * a.dim] = sum;
         } else if (a.h_out && (PASS == kWhole || k == sp.chunks - 1)) {
+            float *o = a.h_out + (b * a.dim + c) * N + n0;
 #pragma unroll
-            for (int i = 0; i < S; ++i)
-                if (n0 + i < N) a.h_out[(b * a.dim + c) * N + n0 + i] = h[i / 4][i % 4];
+            for (int q = 0; q < S / 4; ++q) {
+                if (N % 4 == 0) {
+                    if (n0 + 4 * q < N) store_packed<4>(o + 4 * q, Packed<float, 4>{{h[q][0], h[q][1], h[q][2], h[q][3]}});
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (n0 + 4 * q + i < N) o[4 * q + i] = h[q][i];
+                }
+            }
         }
         return;
     }
