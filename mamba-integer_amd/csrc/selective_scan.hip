@@ -283,6 +283,8 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
         const int n0 = wave * S;
         float am[S / 4][4], h[S / 4][4];
         // a channel's values from n0 on of rows of N states: four at once where N % 4 == 0
+        // (3 x 701 x 1000 x 64 53.3 us instead of 59.5; 8 x 2048 x 1536 x 16 151.0 instead of
+        // 149.1).  N is at least 4 there, so the last four, N - 4 on, are in the row
         auto states = [&](const float *p, float (&o)[S / 4][4]) {
             p += n0;
 #pragma unroll
