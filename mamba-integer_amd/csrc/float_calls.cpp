@@ -296,8 +296,8 @@ PyObject *w4_matvec(PyObject *const *a, Py_ssize_t n_args) {
     t_device = x.device().index();
     if (x.dim() != 2) raise(PyExc_ValueError, "x must be [rows, k], got %s", text(x.sizes()).c_str());
     const int64_t M = x.size(0), k = x.size(1), n = int_of(a[4]), group = int_of(a[5]);
-    if (group != 32 && group != 64 && (group <= 0 || group % 128))
-        raise(PyExc_ValueError, "group=%lld must be 32, 64 or a multiple of 128", (long long)group);
+    if (group != 32 && group != 64 && (group <= 0 || group > INT32_MAX || group % 128))
+        raise(PyExc_ValueError, "group=%lld must be 32, 64 or a multiple of 128 below 2^31", (long long)group);
     if (n < 0) raise(PyExc_ValueError, "n=%lld must not be negative", (long long)n);
     const Tensor &scales = tensor(a[3], "scales");
     const at::ScalarType stype = scales.scalar_type();

@@ -542,14 +542,17 @@ def pack_w4(codes, scales, group: int, zeros=None):
     ceil(K/group)] (float16 kept, other float types as float32), zeros uint8 of the same shape
     (None: 8), weight = (code - zero) * scale.  Returns (packed uint8 [nb, kb, 1024], scales
     [nb, ng, 16], zeros uint8 [nb, ng, 16] or None); include/mamba_int.h has the order."""
+    # (ctypes cuts what does not fit an int to its low 32 bits)
+    if not (group in (32, 64) or 0 < group < 2 ** 31 and group % 128 == 0):
+        raise ValueError(f"group={group} must be 32, 64 or a multiple of 128 below 2^31")
     _req(codes, torch.uint8, "codes")
     if codes.dim() != 2:
         raise ValueError(f"codes must be [n, k], got {tuple(codes.shape)}")
-    if not (group in (32, 64) or group > 0 and group % 128 == 0):
-        raise ValueError(f"group={group} must be 32, 64 or a multiple of 128")
     if not isinstance(scales, torch.Tensor) or scales.dtype not in _FLOAT:
         raise TypeError("scales must be a float32, bfloat16 or float16 tensor")
     n, k = codes.shape
+    if n >= 2 ** 31 or k >= 2 ** 31:
+        raise ValueError(f"codes {tuple(codes.shape)} are out of range")
     nb, kb, have = -(-n // 16), -(-k // 128), -(-k // group)
     ng = kb * 128 // group if group < 128 else have
     if scales.dtype != torch.float16:
