@@ -322,10 +322,12 @@ void launch_w4_shape(const W4Args<T, S> &a, hipStream_t st) {
     }
 }
 
+// Scales of a row (a group may be any number of columns above k: no sum with it).
+inline int w4_scales(int k, int group) { return k / group + (k % group != 0); }
 // Groups of one packed row block: whole column blocks of them.
 inline int w4_groups(int k, int group) {
     const int kp = (k + kW4Cols - 1) / kW4Cols * kW4Cols;
-    return group < kW4Cols ? kp / group : (k + group - 1) / group;
+    return group < kW4Cols ? kp / group : w4_scales(k, group);
 }
 inline bool w4_group_ok(int group) { return group == 32 || group == 64 || (group > 0 && group % kW4Cols == 0); }
 
@@ -347,7 +349,7 @@ extern "C" mi_status mi_pack_w4(const uint8_t *codes, const void *scales, int sc
     MI_REQUIRE(!zeros == !zeros_out, MI_ERR_NULL_POINTER, "mi_pack_w4: zeros and zeros_out go together");
     MI_REQUIRE(aligned(packed, 16), MI_ERR_BAD_ALIGNMENT, "mi_pack_w4: packed must be 16-byte aligned");
     const int64_t nb = (n + kW4Rows - 1) / kW4Rows, kb = (k + kW4Cols - 1) / kW4Cols;
-    const int ng = (k + group - 1) / group, ng_pad = w4_groups(k, group);
+    const int ng = w4_scales(k, group), ng_pad = w4_groups(k, group);
     const int64_t words = nb * kb * 256, vals = nb * ng_pad * kW4Rows;
     MI_REQUIRE(words < ((int64_t)1 << 32), MI_ERR_BAD_DIM, "mi_pack_w4: n * k is too large");
     const int64_t ids = words > vals ? words : vals;

@@ -20,3 +20,21 @@ def test_codes_past_32_bits_are_refused(cuda):
     codes = torch.empty((1, 2 ** 32 + 128), dtype=torch.uint8, device=cuda)
     with pytest.raises(ValueError, match="codes"):
         ops.pack_w4(codes, torch.zeros((1, 5), device=cuda), 2 ** 30)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [2 ** 31 - 128, 2 ** 30])
+def test_groups_far_above_k(cuda, group):
+    """One scale and zero point a row, as with a group that just holds it."""
+    from mamba_int import ops
+    g = torch.Generator().manual_seed(7)
+    n, k = 70, 2048
+    codes = torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8).to(cuda)
+    scales = (0.5 + torch.rand(n, 1, generator=g)).to(cuda)
+    zeros = torch.randint(0, 16, (n, 1), generator=g, dtype=torch.uint8).to(cuda)
+    x = torch.randn(3, k, generator=g).to(cuda)
+    got, want = ([*ops.pack_w4(codes, scales, by, zeros=zeros)] for by in (group, k))
+    for i in range(3):
+        assert torch.equal(got[i], want[i])
+    a, b = (ops.w4_matvec(x, *p[:2], n, by, zeros=p[2]) for p, by in ((got, group), (want, k)))
+    assert torch.equal(a, b)
