@@ -140,9 +140,11 @@ class SelectiveRunner:
     @torch.no_grad()
     def forward(self, ids: torch.Tensor, state: SelectiveState, lens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Logits float32 [B, vocab] of each sequence's last token; ids int64 [B, L], state is
-        updated in place.  lens int32 [B]: tokens of each sequence (at least one; the rest of
-        its row is padding)."""
+        updated in place.  lens int32 [B]: tokens of each sequence, taken as within [0, L] (the
+        rest of its row is padding); one of no tokens has logits of zero."""
         B, L = ids.shape
+        if L < 1:
+            raise ValueError("ids must hold at least one token a sequence")
         dims, D, N, R = self.dims, self.dims.d_inner, self.dims.d_state, self.dims.dt_rank
         r = self.params.emb[ids.reshape(-1)]
         x = None
@@ -160,9 +162,12 @@ class SelectiveRunner:
             y = ops.selective_scan(u, dt, ly.a, xp[..., R:R + N], xp[..., R + N:], d_skip=ly.d, z=uz[..., D:],
                                    dt_bias=ly.dt_bias, h_in=state.h[i], h_out=state.h[i], lens=lens)
             x = ops.bitlinear_f32(y.view(B * L, D), ly.w_out.packed, ly.w_out.scale)
-        last = (lens.long() if lens is not None else torch.full((B,), L, device=self.device)) - 1
+        # a row of its own sequence, whatever lens holds
+        last = (lens.clamp(1, L).long() if lens is not None else torch.full((B,), L, device=self.device)) - 1
         rows = last + L * torch.arange(B, device=self.device)
         y, _ = ops.add_rms_norm(x[rows], self.params.norm_f, residual=r[rows])
+        if lens is not None:
+            y.masked_fill_((lens < 1).unsqueeze(1), 0.0)
         packed, scales, zeros = self.params.head
         return ops.w4_matvec(y, packed, scales, dims.vocab_size, HEAD_GROUP, zeros=zeros)
 
