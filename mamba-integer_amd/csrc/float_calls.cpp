@@ -5,7 +5,7 @@
 // kernel takes on a decode step's rows.
 //
 // The entry points come as addresses (the library is loaded once, by _lib), the
-// stream as its handle.
+// stream as its handle and device.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -29,7 +29,7 @@ decltype(&mi_w4_matvec) g_w4;
 decltype(&mi_last_error_string) g_last_error;
 PyObject *g_mi_error;   // _lib.MIError
 
-thread_local c10::DeviceIndex t_device;   // of the call's first tensor
+thread_local long t_device;   // the current device: the stream's, and the one that all tensors have to be on
 
 struct Raised {};       // a Python error is set
 
@@ -87,7 +87,9 @@ const Tensor &like(PyObject *o, at::IntArrayRef shape, at::ScalarType type, cons
     if (t.scalar_type() != type) raise(PyExc_TypeError, "%s must be %s, got %s", name, type_name(type), type_name(t.scalar_type()));
     if (t.sizes() != shape) raise(PyExc_ValueError, "%s must be %s, got %s", name, text(shape).c_str(), text(t.sizes()).c_str());
     if (!t.is_cuda()) raise(PyExc_ValueError, "%s must be a device tensor (libmamba_int has no host path)", name);
-    if (t.device().index() != t_device) raise(PyExc_ValueError, "%s must be on the device of the other tensors", name);
+    if (t.device().index() != t_device)
+        raise(PyExc_ValueError, "%s is on cuda:%d, but the call runs on the stream of the current device, cuda:%ld", name,
+              (int)t.device().index(), t_device);
     if (t.requires_grad() && c10::GradMode::is_enabled())
         raise(PyExc_ValueError, "%s requires a gradient; the float operators are forward only", name);
     return t;
@@ -154,7 +156,7 @@ struct Ref {
 void count(Py_ssize_t n, Py_ssize_t want, const char *fn) {
     if (n != want) raise(PyExc_TypeError, "%s takes %zd arguments, got %zd", fn, want, n);
 }
-void *stream_of(PyObject *o) {
+void *address(PyObject *o) {
     void *p = PyLong_AsVoidPtr(o);
     if (PyErr_Occurred()) throw Raised{};
     return p;
@@ -163,6 +165,12 @@ int64_t int_of(PyObject *o) {
     const int64_t v = PyLong_AsLongLong(o);
     if (v == -1 && PyErr_Occurred()) throw Raised{};
     return v;
+}
+// (handle of the current stream, its device)
+void *stream_of(PyObject *o) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2) raise(PyExc_TypeError, "the stream must be a tuple of its handle and device");
+    t_device = (long)int_of(PyTuple_GET_ITEM(o, 1));
+    return address(PyTuple_GET_ITEM(o, 0));
 }
 int size_of(int64_t v, const char *name) {
     if (v < 0 || v > INT32_MAX) raise(PyExc_ValueError, "%s=%lld is out of range", name, (long long)v);
@@ -173,9 +181,9 @@ int size_of(int64_t v, const char *name) {
 // residual_out), else (q, scale, residual_out) with q's rows rounded up to unit.
 PyObject *add_rms_norm(PyObject *const *a, Py_ssize_t n) {
     count(n, 8, "add_rms_norm");
+    void *stream = stream_of(a[0]);
     const Tensor &x = tensor(a[1], "x");
     const int code = float_type(x, "x");
-    t_device = x.device().index();
     if (x.dim() != 2) raise(PyExc_ValueError, "x must be [tokens, dim], got %s", text(x.sizes()).c_str());
     const int64_t T = x.size(0), d = x.size(1), unit = int_of(a[7]);
     const auto shape = x.sizes();
@@ -199,7 +207,7 @@ PyObject *add_rms_norm(PyObject *const *a, Py_ssize_t n) {
         Ref y(output(a[6], shape, x));
         yr = rows(y.p, shape, x.scalar_type(), "out", true);
         check("mi_add_rms_norm", g_norm(xr.p, code, xr.ld, rr.p, rcode, rr.ld, w, (float)eps, yr.p, yr.ld, nullptr, 0,
-                                        nullptr, ro.p, ro.ld, size_of(T, "tokens"), size_of(d, "dim"), stream_of(a[0])));
+                                        nullptr, ro.p, ro.ld, size_of(T, "tokens"), size_of(d, "dim"), stream));
         return Py_BuildValue("(NN)", y.release(), res.release());
     }
     if (unit < 1) raise(PyExc_ValueError, "unit=%lld must be at least 1", (long long)unit);
@@ -209,16 +217,16 @@ PyObject *add_rms_norm(PyObject *const *a, Py_ssize_t n) {
           g_norm(xr.p, code, xr.ld, rr.p, rcode, rr.ld, w, (float)eps, nullptr, 0,
                  static_cast<int8_t *>(THPVariable_Unpack(q.p).data_ptr()), dp,
                  static_cast<float *>(THPVariable_Unpack(scale.p).data_ptr()), ro.p, ro.ld, size_of(T, "tokens"),
-                 size_of(d, "dim"), stream_of(a[0])));
+                 size_of(d, "dim"), stream));
     return Py_BuildValue("(NNN)", q.release(), scale.release(), res.release());
 }
 
 // (stream, x, weight, bias, silu, state_in, state_out, lens, out)
 PyObject *causal_conv(PyObject *const *a, Py_ssize_t n) {
     count(n, 9, "causal_conv");
+    void *stream = stream_of(a[0]);
     const Tensor &x = tensor(a[1], "x");
     const int code = float_type(x, "x");
-    t_device = x.device().index();
     if (x.dim() != 3) raise(PyExc_ValueError, "x must be [batch, len, dim], got %s", text(x.sizes()).c_str());
     const at::ScalarType type = x.scalar_type();
     const auto shape = x.sizes();
@@ -235,8 +243,7 @@ PyObject *causal_conv(PyObject *const *a, Py_ssize_t n) {
     Ref y(output(a[8], shape, x));
     const Rows yr = rows(y.p, shape, type, "out", true);
     check("mi_causal_conv", g_conv(xr.p, xr.ld, xr.bs, code, w, bias, size_of(W, "width"), (int)int_of(a[4]), si, so, lens,
-                                   yr.p, yr.ld, yr.bs, size_of(B, "batch"), size_of(L, "len"), size_of(D, "dim"),
-                                   stream_of(a[0])));
+                                   yr.p, yr.ld, yr.bs, size_of(B, "batch"), size_of(L, "len"), size_of(D, "dim"), stream));
     return y.release();
 }
 
@@ -253,9 +260,9 @@ Rows group_rows(PyObject *o, int64_t B, int64_t L, int64_t G, int64_t N, at::Sca
 // (stream, u, dt, a, b, c, d_skip, z, dt_bias, dt_softplus, h_in, h_out, lens, out)
 PyObject *selective_scan(PyObject *const *a, Py_ssize_t n) {
     count(n, 14, "selective_scan");
+    void *stream = stream_of(a[0]);
     const Tensor &u = tensor(a[1], "u");
     const int code = float_type(u, "u");
-    t_device = u.device().index();
     if (u.dim() != 3) raise(PyExc_ValueError, "u must be [batch, len, dim], got %s", text(u.sizes()).c_str());
     const at::ScalarType type = u.scalar_type();
     const auto shape = u.sizes();
@@ -284,16 +291,16 @@ PyObject *selective_scan(PyObject *const *a, Py_ssize_t n) {
     check("mi_selective_scan",
           g_scan(ur.p, ur.ld, ur.bs, tr.p, tr.ld, tr.bs, am, br.p, br.ld, br.bs, cr.p, cr.ld, cr.bs, skip, zr.p, zr.ld,
                  zr.bs, bias, PyObject_IsTrue(a[9]) == 1, h_in, h_out, lens, yr.p, yr.ld, yr.bs, code, bi, li, di, ni, gi,
-                 bytes ? ws.data_ptr() : nullptr, bytes, stream_of(a[0])));
+                 bytes ? ws.data_ptr() : nullptr, bytes, stream));
     return y.release();
 }
 
 // (stream, x, packed, scales, n, group, zeros, bias, out)
 PyObject *w4_matvec(PyObject *const *a, Py_ssize_t n_args) {
     count(n_args, 9, "w4_matvec");
+    void *stream = stream_of(a[0]);
     const Tensor &x = tensor(a[1], "x");
     const int code = float_type(x, "x");
-    t_device = x.device().index();
     if (x.dim() != 2) raise(PyExc_ValueError, "x must be [rows, k], got %s", text(x.sizes()).c_str());
     const int64_t M = x.size(0), k = x.size(1), n = int_of(a[4]), group = int_of(a[5]);
     if (group != 32 && group != 64 && (group <= 0 || group > INT32_MAX || group % 128))
@@ -313,8 +320,7 @@ PyObject *w4_matvec(PyObject *const *a, Py_ssize_t n_args) {
     Ref y(output(a[8], shape, x));
     const Rows yr = rows(y.p, shape, x.scalar_type(), "out", true);
     check("mi_w4_matvec", g_w4(xr.p, xr.ld, code, packed, s, stype == at::kHalf ? MI_F16 : MI_F32, zeros, bias, yr.p, yr.ld,
-                               size_of(M, "rows"), size_of(n, "n"), size_of(k, "k"), size_of(group, "group"),
-                               stream_of(a[0])));
+                               size_of(M, "rows"), size_of(n, "n"), size_of(k, "k"), size_of(group, "group"), stream));
     return y.release();
 }
 
@@ -322,7 +328,7 @@ PyObject *w4_matvec(PyObject *const *a, Py_ssize_t n_args) {
 PyObject *init(PyObject *const *a, Py_ssize_t n) {
     count(n, 7, "init");
     void *p[6];
-    for (int i = 0; i < 6; ++i) p[i] = stream_of(a[i + 1]);
+    for (int i = 0; i < 6; ++i) p[i] = address(a[i + 1]);
     g_norm = reinterpret_cast<decltype(g_norm)>(p[0]);
     g_conv = reinterpret_cast<decltype(g_conv)>(p[1]);
     g_scan_size = reinterpret_cast<decltype(g_scan_size)>(p[2]);

@@ -491,10 +491,14 @@ def _calls():
     return _float_calls
 
 
-def _raw_stream() -> int:
-    """The current stream's handle, without a stream object around it (2.8 us less);
-    0 where there is no device (every call then refuses its tensors)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) if torch.cuda.is_initialized() else 0
+def _here() -> Tuple[int, int]:
+    """The current stream's handle, without a stream object around it (2.8 us less), and its
+    device, which the calls' tensors have to be on; (0, -1) where there is no device (every
+    call then refuses its tensors)."""
+    if not torch.cuda.is_initialized():
+        return 0, -1
+    device = torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(device), device
 
 
 def add_rms_norm(x, weight, residual=None, eps: float = 1e-5, residual_out=None, out=None):
@@ -502,7 +506,7 @@ def add_rms_norm(x, weight, residual=None, eps: float = 1e-5, residual_out=None,
     (normed rows in x's type, s in the residual's type).  weight float32 [d]; the residual
     has x's type or float32 (None: s = x, returned only if ``residual_out`` is passed, else
     None).  ``residual_out`` may be the residual itself, ``out`` may be x.  Forward only."""
-    return _calls().add_rms_norm(_raw_stream(), x, weight, residual, eps, residual_out, out, 0)
+    return _calls().add_rms_norm(_here(), x, weight, residual, eps, residual_out, out, 0)
 
 
 def add_rms_norm_quant(x, weight, residual=None, eps: float = 1e-5, residual_out=None, unit: int = 64):
@@ -511,7 +515,7 @@ def add_rms_norm_quant(x, weight, residual=None, eps: float = 1e-5, residual_out
     reads with ``x_scale=scale``, bit-identical to ``act_quant`` of the float32 norm."""
     if unit < 1:
         raise ValueError(f"unit={unit} must be at least 1")
-    return _calls().add_rms_norm(_raw_stream(), x, weight, residual, eps, residual_out, None, unit)
+    return _calls().add_rms_norm(_here(), x, weight, residual, eps, residual_out, None, unit)
 
 
 def causal_conv(x, weight, bias=None, activation: Optional[str] = "silu", state_in=None, state_out=None, lens=None,
@@ -523,7 +527,7 @@ def causal_conv(x, weight, bias=None, activation: Optional[str] = "silu", state_
     sequence, the rows of the output past them are zero.  Forward only."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be 'silu' or None, got {activation!r}")
-    return _calls().causal_conv(_raw_stream(), x, weight, bias, _ACTIVATIONS[activation], state_in, state_out, lens, out)
+    return _calls().causal_conv(_here(), x, weight, bias, _ACTIVATIONS[activation], state_in, state_out, lens, out)
 
 
 def selective_scan(u, dt, a, b, c, d_skip=None, z=None, dt_bias=None, dt_softplus: bool = True, h_in=None, h_out=None,
@@ -534,7 +538,7 @@ def selective_scan(u, dt, a, b, c, d_skip=None, z=None, dt_bias=None, dt_softplu
     a float32 [D, N], d_skip, dt_bias float32 [D]; h_in / h_out float32 [B, D, N] (None: zeros;
     may be the same tensor); L = 1 is a decode step.  lens int32 [B]: tokens of each sequence
     (h_out: the state after them; rows of the output past them are zero).  Forward only."""
-    return _calls().selective_scan(_raw_stream(), u, dt, a, b, c, d_skip, z, dt_bias, dt_softplus, h_in, h_out, lens, out)
+    return _calls().selective_scan(_here(), u, dt, a, b, c, d_skip, z, dt_bias, dt_softplus, h_in, h_out, lens, out)
 
 
 def pack_w4(codes, scales, group: int, zeros=None):
@@ -553,6 +557,9 @@ def pack_w4(codes, scales, group: int, zeros=None):
     n, k = codes.shape
     if n >= 2 ** 31 or k >= 2 ** 31:
         raise ValueError(f"codes {tuple(codes.shape)} are out of range")
+    for name, t in (("codes", codes), ("scales", scales), ("zeros", zeros)):
+        if t is not None and t.is_cuda and t.device.index != _here()[1]:
+            raise ValueError(f"{name} must be on the current device, whose stream the call runs on")
     nb, kb, have = -(-n // 16), -(-k // 128), -(-k // group)
     ng = kb * 128 // group if group < 128 else have
     if scales.dtype != torch.float16:
@@ -572,4 +579,4 @@ def pack_w4(codes, scales, group: int, zeros=None):
 def w4_matvec(x, packed, scales, n: int, group: int, zeros=None, bias=None, out=None):
     """y [M, n] = x [M, K] @ W^T (+ bias float32 [n]) for the 4-bit weights of ``pack_w4``:
     made for the rows of a decode step (1..64; more are computed too).  Forward only."""
-    return _calls().w4_matvec(_raw_stream(), x, packed, scales, n, group, zeros, bias, out)
+    return _calls().w4_matvec(_here(), x, packed, scales, n, group, zeros, bias, out)

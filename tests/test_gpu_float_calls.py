@@ -1,0 +1,31 @@
+"""What the float operators' calls refuse beside shapes and types, on the device."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def every_call(cuda):
+    """name -> a small call, its first tensor's name."""
+    from mamba_int import ops
+    x, w = torch.randn(3, 16, device=cuda), torch.ones(16, device=cuda)
+    a, bc = -torch.ones(16, 4, device=cuda), torch.randn(1, 3, 4, device=cuda)
+    codes, scales = torch.zeros(4, 16, dtype=torch.uint8, device=cuda), torch.ones(4, 1, device=cuda)
+    packed, s, _ = ops.pack_w4(codes, scales, 32)
+    return {"norm": lambda: ops.add_rms_norm(x, w), "quant": lambda: ops.add_rms_norm_quant(x, w),
+            "conv": lambda: ops.causal_conv(x[None], torch.ones(16, 4, device=cuda)),
+            "scan": lambda: ops.selective_scan(x[None], x[None], a, bc, bc),
+            "w4": lambda: ops.w4_matvec(x, packed, s, 4, 32), "pack": lambda: ops.pack_w4(codes, scales, 32)}
+
+
+@pytest.mark.parametrize("name", ["norm", "quant", "conv", "scan", "w4", "pack"])
+def test_tensors_of_another_device_than_the_streams(cuda, name, monkeypatch):
+    """The call would run on the current device's stream, not behind what made its tensors."""
+    from mamba_int import ops
+    call = every_call(cuda)[name]
+    call()
+    stream, device = ops._here()
+    assert device == cuda.index and stream == torch.cuda.current_stream().cuda_stream
+    monkeypatch.setattr(ops, "_here", lambda: (stream, device + 1))
+    with pytest.raises(ValueError, match="current device"):
+        call()
