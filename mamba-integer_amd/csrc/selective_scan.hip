@@ -246,6 +246,15 @@ __device__ __forceinline__ void static_for(F &&f) {
 // state); kParts starts each part from the states in front of it, joined from those.
 enum ScanPass { kWhole, kEnds, kParts };
 
+// The state that a place of a block's holds.  The N states do not always fill the places
+// (at most 2 N, or 4): one past N holds a second copy of a state, and a state's copies
+// share its C in equal parts, halves or quarters, which are exact.  (Zeros there would
+// make 0 * inf of an infinite input or step, a NaN in the channel's sum.)
+__device__ __forceinline__ int place_state(int place, int N) { return place < N ? place : N > 1 ? place - N : 0; }
+__device__ __forceinline__ float place_share(int place, int N, int places) {
+    return N == 1 ? 1.0f / places : place_state(place, N) + N < places ? 0.5f : 1.0f;
+}
+
 struct ScanSplit {
     float *ends;
     int chunks, chunk, blocks;   // blocks: of 64 channels, a group
@@ -284,18 +293,17 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
         float am[S / 4][4], h[S / 4][4];
         // a channel's values from n0 on of rows of N states: four at once where N % 4 == 0
         // (3 x 701 x 1000 x 64 53.3 us instead of 59.5; 8 x 2048 x 1536 x 16 151.0 instead of
-        // 149.1).  N is at least 4 there, so the last four, N - 4 on, are in the row
+        // 149.1)
         auto states = [&](const float *p, float (&o)[S / 4][4]) {
-            p += n0;
 #pragma unroll
             for (int q = 0; q < S / 4; ++q) {
                 if (N % 4 == 0) {
-                    const Packed<float, 4> v = load_packed<4>(p + min(4 * q, N - 4 - n0));
+                    const Packed<float, 4> v = load_packed<4>(p + place_state(n0 + 4 * q, N));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[q][i] = n0 + 4 * q < N ? v.v[i] : 0.0f;
+                    for (int i = 0; i < 4; ++i) o[q][i] = v.v[i];
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[q][i] = n0 + 4 * q + i < N ? p[4 * q + i] : 0.0f;
+                    for (int i = 0; i < 4; ++i) o[q][i] = p[place_state(n0 + 4 * q + i, N)];
                 }
             }
         };
@@ -320,12 +328,12 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
             const float *e = sp.ends + b * sp.chunks * (N + 1) * a.dim + c;
             const float *first = e + (int64_t)(sp.chunks - 1) * (N + 1) * a.dim;
 #pragma unroll
-            for (int i = 0; i < S; ++i) h[i / 4][i % 4] = n0 + i < N ? first[(int64_t)(n0 + i) * a.dim] : 0.0f;
+            for (int i = 0; i < S; ++i) h[i / 4][i % 4] = first[(int64_t)place_state(n0 + i, N) * a.dim];
             for (int j = 0; j < k; ++j, e += (int64_t)(N + 1) * a.dim) {
                 const float sum = e[(int64_t)N * a.dim];
 #pragma unroll
                 for (int i = 0; i < S; ++i) {
-                    const float last = n0 + i < N ? e[(int64_t)(n0 + i) * a.dim] : 0.0f;
+                    const float last = e[(int64_t)place_state(n0 + i, N) * a.dim];
                     float &hi = h[i / 4][i % 4];
                     hi = hi != 0.0f ? __builtin_fmaf(__builtin_amdgcn_exp2f(am[i / 4][i % 4] * sum), hi, last) : last;
                 }
@@ -404,6 +412,8 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
     const int hw = wave - NW, r0 = hw * kRows, tid = hw * 64 + lane;
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.0f, skip = a.d_skip ? a.d_skip[c] : 0.0f;
     const bool gate = kY && a.z.p != nullptr;
+    static_assert(64 * kHelpers % kStates == 0, "a thread stages one place's C");
+    const float share = place_share(min(tid, TT * kStates - 1) % kStates, N, kStates);
     // Rows are read from the tile's first row, whose address every lane shares, by
     // 32-bit offsets that stay the same from tile to tile.
     uint32_t dt_off[kRows], u_off[kRows], z_off[kRows], y_off[kRows], b_off[kLoadBC], c_off[kLoadBC];
@@ -419,7 +429,7 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
 #pragma unroll
         for (int i = 0; i < kLoadBC; ++i) {
             const int e = min(tid + i * 64 * kHelpers, TT * kStates - 1);
-            const uint32_t row = min(e / kStates, last), col = g * N + min(e % kStates, N - 1);
+            const uint32_t row = min(e / kStates, last), col = g * N + place_state(e % kStates, N);
             b_off[i] = (row * (uint32_t)a.b.ld + col) * sizeof(T);
             c_off[i] = (row * (uint32_t)a.c.ld + col) * sizeof(T);
         }
@@ -479,9 +489,8 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
 #pragma unroll
         for (int i = 0; i < kLoadBC; ++i) {
             const int e = min(tid + i * 64 * kHelpers, TT * kStates - 1);
-            const bool real = e % kStates < N;
-            bs[buf][e] = real && e / kStates < rows ? (float)b_next[i] : 0.0f;
-            if (kY) cs[buf][e] = real ? (float)c_next[i] : 0.0f;
+            bs[buf][e] = e / kStates < rows ? (float)b_next[i] : 0.0f;
+            if (kY) cs[buf][e] = share * (float)c_next[i];
         }
     };
     auto finish = [&](int t, int buf, const float (&uf)[kRows], const float (&zf)[kRows]) {

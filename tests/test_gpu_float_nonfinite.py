@@ -1,0 +1,63 @@
+"""Infinite inputs, steps and states of the selective scan, as the recurrence in 64 bits has them."""
+import pytest
+import torch
+
+import float_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+def same(got, want, err, dtype):
+    """NaN and infinities where want has them, the rest within err."""
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    odd = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), odd) and torch.equal(got[odd], want[odd])
+    on = torch.isfinite(want)
+    R.close(got[on].to(dtype), want[on], err[on], dtype)
+
+
+def positive(B, L, D, N, dtype, seed):
+    """Decays that leave a state above 2^-40 over 20 steps; B, C, u and D positive."""
+    g = torch.Generator().manual_seed(seed)
+
+    def rand(*shape):
+        return (0.1 + 0.9 * torch.rand(*shape, generator=g)).to(dtype)
+    return {"u": rand(B, L, D), "dt": rand(B, L, D) - 1.0, "b": rand(B, L, 1, N), "c": rand(B, L, 1, N),
+            "a": -(0.1 + 0.9 * torch.rand(D, N, generator=g)), "d_skip": torch.rand(D, generator=g)}
+
+
+def run(s, cuda, **more):
+    from mamba_int import ops
+    h = torch.zeros(s["u"].shape[0], *s["a"].shape, device=cuda)
+    y = ops.selective_scan(**{k: v.to(cuda) for k, v in s.items()}, h_out=h, **more)
+    return y, h
+
+
+# L: steps one after another, tiles of a whole sequence (many blocks), tiles of its parts
+@pytest.mark.parametrize("B,L,D", [(2, 1, 9), (2, 5, 9), (2, 30, 9), (300, 20, 5), (1, 200, 9)])
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 5, 7, 8, 12, 13, 16, 20, 40, 100, 129, 200])
+@pytest.mark.parametrize("what", ["u", "dt"])
+def test_infinite_input_or_step(cuda, B, L, D, N, what):
+    """Infinite from that step on, whatever N: no place of a block beside the states makes a NaN."""
+    s = positive(B, L, D, N, torch.float32, 3 * N + L)
+    t = L // 3
+    s[what][B // 2, t, 4] = float("inf")
+    got, h = run(s, cuda)
+    y, ey, hw, eh = R.scan(s["u"], s["dt"], s["a"], s["b"], s["c"], s["d_skip"])
+    assert torch.isinf(y[B // 2, t:, 4]).all() and torch.isinf(y).sum() == L - t
+    same(got, y, ey, torch.float32)
+    same(h, hw, eh, torch.float32)
+
+
+@pytest.mark.parametrize("N", [3, 12, 16, 20])
+def test_infinite_input_of_16_bits_with_a_gate(cuda, N):
+    for dtype in (torch.bfloat16, torch.float16):
+        s = positive(3, 40, 70, N, dtype, N)
+        s["z"] = s["u"].clone()
+        s["u"][1, 17, 66] = -float("inf")
+        got, h = run(s, cuda)
+        y, ey, hw, eh = R.scan(s["u"], s["dt"], s["a"], s["b"], s["c"], s["d_skip"], s["z"])
+        assert (y[1, 17:, 66] == -float("inf")).all()
+        same(got, y, ey, dtype)
+        same(h, hw, eh, torch.float32)
