@@ -329,13 +329,18 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
             const float *first = e + (int64_t)(sp.chunks - 1) * (N + 1) * a.dim;
 #pragma unroll
             for (int i = 0; i < S; ++i) h[i / 4][i % 4] = first[(int64_t)place_state(n0 + i, N) * a.dim];
+            // A part's decay in two equal factors, each held at 2^-126 where it would be
+            // flushed to zero: one exponential of the whole loses a state of up to 2^128 that
+            // has not decayed yet, and makes a NaN of an infinite one.  (An infinite step's is 0.)
             for (int j = 0; j < k; ++j, e += (int64_t)(N + 1) * a.dim) {
-                const float sum = e[(int64_t)N * a.dim];
+                const float sum = 0.5f * e[(int64_t)N * a.dim];
+                const float least = fabsf(sum) <= kMaxFloat ? -126.0f : -__builtin_inff();
 #pragma unroll
                 for (int i = 0; i < S; ++i) {
                     const float last = e[(int64_t)place_state(n0 + i, N) * a.dim];
                     float &hi = h[i / 4][i % 4];
-                    hi = hi != 0.0f ? __builtin_fmaf(__builtin_amdgcn_exp2f(am[i / 4][i % 4] * sum), hi, last) : last;
+                    const float decay = __builtin_amdgcn_exp2f(fmaxf(am[i / 4][i % 4] * sum, least));
+                    hi = hi != 0.0f ? __builtin_fmaf(decay, decay * hi, last) : last;
                 }
             }
         }

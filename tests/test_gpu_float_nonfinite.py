@@ -61,3 +61,24 @@ def test_infinite_input_of_16_bits_with_a_gate(cuda, N):
         assert (y[1, 17:, 66] == -float("inf")).all()
         same(got, y, ey, dtype)
         same(h, hw, eh, torch.float32)
+
+
+@pytest.mark.parametrize("N", [1, 8, 16, 20])
+@pytest.mark.parametrize("L", [300, 2000])
+def test_large_and_infinite_states_in_a_split_sequence(cuda, L, N):
+    """States that decay by 2^-2.9 a step: a part's decay is below the smallest float, that of
+    each step is not.  Without inputs the state alone is left."""
+    s = positive(1, L, 5, N, torch.float32, L + N)
+    s["u"].zero_()
+    s["dt"].fill_(2.0)
+    s["a"].fill_(-1.0)
+    s["h_in"] = torch.full((1, 5, N), 1e38)
+    s["h_in"][0, 1] = float("inf")
+    s["h_in"][0, 2] = -float("inf")
+    s["h_in"][0, 3] = float("nan")
+    s["h_in"][0, 4] = -1e30
+    got, h = run(s, cuda, dt_softplus=False)
+    y, ey, hw, eh = R.scan(s["u"], s["dt"], s["a"], s["b"], s["c"], s["d_skip"], sp=False, h_in=s["h_in"])
+    # what is left near the end of the type's range may be flushed to zero
+    same(got, y, ey + 2.0 ** -110, torch.float32)
+    same(h, hw, eh + 2.0 ** -110, torch.float32)
