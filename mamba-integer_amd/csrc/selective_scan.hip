@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs<T> a) {
         }
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) y += __shfl_xor(y, o);
-        y = __builtin_fmaf(skip, u, y);
+        if (a.d_skip) y = __builtin_fmaf(skip, u, y);          // (0 * inf without it)
         if (a.z.p) y *= silu((float)a.z.row(b, t)[c]);
         if (on && lane == 0) a.y.row(b, t)[c] = (T)y;
     }
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256) void scan_token_kernel(ScanArgs<T> a) {
         if (!on || (int)b0 + s >= a.batch) continue;
         if (a.h_out && mine) store_packed<4>(a.h_out + at[s], next);
         if (lane == 0) {
-            y = __builtin_fmaf(skip, uf, y);
+            if (a.d_skip) y = __builtin_fmaf(skip, uf, y);
             if (a.z.p) y *= silu((float)z[s]);
             a.y.row(b[s], 0)[c] = (T)(run ? y : 0.0f);
         }
@@ -499,14 +499,20 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
         }
     };
     auto finish = [&](int t, int buf, const float (&uf)[kRows], const float (&zf)[kRows]) {
+        float v[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) v[i] = parts[buf][0][r0 + i][lane];
+        if (a.d_skip) {                                        // (0 * inf without it)
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) v[i] = __builtin_fmaf(skip, uf[i], v[i]);
+        }
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            float v = skip * uf[i];
 #pragma unroll
-            for (int w = 0; w < NW; ++w) v += parts[buf][w][r0 + i][lane];
-            const float gated = v * silu(zf[i]);
+            for (int w = 1; w < NW; ++w) v[i] += parts[buf][w][r0 + i][lane];
+            const float gated = v[i] * silu(zf[i]);
             if (on && t + r0 + i < end)
-                *reinterpret_cast<T *>(reinterpret_cast<char *>(y_p) + y_off[i]) = (T)(gate ? gated : v);
+                *reinterpret_cast<T *>(reinterpret_cast<char *>(y_p) + y_off[i]) = (T)(gate ? gated : v[i]);
         }
         y_p += TT * a.y.ld;
     };

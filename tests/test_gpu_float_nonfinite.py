@@ -82,3 +82,16 @@ def test_large_and_infinite_states_in_a_split_sequence(cuda, L, N):
     # what is left near the end of the type's range may be flushed to zero
     same(got, y, ey + 2.0 ** -110, torch.float32)
     same(h, hw, eh + 2.0 ** -110, torch.float32)
+
+
+@pytest.mark.parametrize("B,L,D,N", [(2, 1, 9, 16), (3, 1, 9, 5), (2, 5, 9, 16), (2, 30, 9, 16), (1, 200, 9, 16)])
+def test_infinite_input_without_a_skip(cuda, B, L, D, N):
+    s = positive(B, L, D, N, torch.float32, L)
+    del s["d_skip"]
+    t = L // 3
+    s["u"][B // 2, t, 4] = float("inf")
+    got, h = run(s, cuda)
+    y, ey, hw, eh = R.scan(s["u"], s["dt"], s["a"], s["b"], s["c"])
+    y[B // 2, t:, 4], ey[B // 2, t, 4] = float("inf"), 0.0     # (the oracle's own skip of 0 times inf)
+    same(got, y, ey, torch.float32)
+    same(h, hw, eh, torch.float32)
