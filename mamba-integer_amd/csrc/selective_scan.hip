@@ -260,6 +260,9 @@ struct ScanSplit {
     int chunks, chunk, blocks;   // blocks: of 64 channels, a group
 };
 
+// 16 bytes at any float's address
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+
 // kHelpers waves of a block turn rows into a tile's d, d u, B and C in LDS and the
 // recurring waves' parts of y into output rows, one tile ahead and one behind.
 constexpr int kHelpers = 4;
@@ -298,9 +301,10 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
 #pragma unroll
             for (int q = 0; q < S / 4; ++q) {
                 if (N % 4 == 0) {
-                    const Packed<float, 4> v = load_packed<4>(p + place_state(n0 + 4 * q, N));
+                    // (a vector: four floats of a struct are merged with the loads below)
+                    const v4f_any v = *reinterpret_cast<const v4f_any *>(p + place_state(n0 + 4 * q, N));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[q][i] = v.v[i];
+                    for (int i = 0; i < 4; ++i) o[q][i] = v[i];
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[q][i] = p[place_state(n0 + 4 * q + i, N)];
