@@ -74,8 +74,6 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs<T> a) {
     float h[4] = {}, am[4] = {};
     four(a.a + (int64_t)c * N + n0, am);
     if (a.h_in) four(a.h_in + (int64_t)ch * N + n0, h);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) am[i] *= 1.44269504f;
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.0f, skip = a.d_skip ? a.d_skip[c] : 0.0f;
     for (int t = 0; t < len; ++t) {
         float bn[4] = {}, cn[4] = {};
@@ -84,11 +82,11 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs<T> a) {
         const float u = (float)a.u.row(b, t)[c];
         float dt = (float)a.dt.row(b, t)[c] + bias;
         if (a.softplus) dt = softplus(dt);
-        const float du = dt * u;
+        const float du = dt * u, dl = kLog2e * dt;             // (kLog2e * am may be infinite, and the step 0)
         float y = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * am[i]), h[i], du * bn[i]);
+            h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dl * am[i]), h[i], du * bn[i]);
             if (n0 + i < N) y = __builtin_fmaf(cn[i], h[i], y);
         }
 #pragma unroll

@@ -95,3 +95,19 @@ def test_infinite_input_without_a_skip(cuda, B, L, D, N):
     y[B // 2, t:, 4], ey[B // 2, t, 4] = float("inf"), 0.0     # (the oracle's own skip of 0 times inf)
     same(got, y, ey, torch.float32)
     same(h, hw, eh, torch.float32)
+
+
+@pytest.mark.parametrize("B,L,D,N", [(2, 1, 9, 16), (2, 1, 9, 5), (2, 5, 9, 16), (2, 30, 9, 16), (1, 200, 9, 16)])
+def test_the_fastest_decays(cuda, B, L, D, N):
+    """a near the lowest float: a step of 0 keeps the state, any other clears it."""
+    s = positive(B, L, D, N, torch.float32, L)
+    s["a"].fill_(-3.4e38)
+    s["dt"].zero_()
+    s["dt"][:, L - 1, 3] = 0.25
+    s["h_in"] = torch.ones(B, D, N)
+    got, h = run(s, cuda, dt_softplus=False)
+    y, ey, hw, eh = R.scan(s["u"], s["dt"], s["a"], s["b"], s["c"], s["d_skip"], sp=False, h_in=s["h_in"])
+    assert (hw[:, :3] == 1).all() and (hw[:, 3] < 1).all()
+    # (the bound of a decay of 0 is not finite: its exponent's error times 0 is meant)
+    same(got, y, torch.where(torch.isfinite(ey), ey, 8 * R.U * y.abs()), torch.float32)
+    same(h, hw, torch.where(torch.isfinite(eh), eh, 8 * R.U * hw.abs()), torch.float32)
