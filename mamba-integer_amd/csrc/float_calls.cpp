@@ -261,6 +261,8 @@ Rows group_rows(PyObject *o, int64_t B, int64_t L, int64_t G, int64_t N, at::Sca
 PyObject *selective_scan(PyObject *const *a, Py_ssize_t n) {
     count(n, 14, "selective_scan");
     void *stream = stream_of(a[0]);
+    const int softplus = PyObject_IsTrue(a[9]);
+    if (softplus < 0) throw Raised{};
     const Tensor &u = tensor(a[1], "u");
     const int code = float_type(u, "u");
     if (u.dim() != 3) raise(PyExc_ValueError, "u must be [batch, len, dim], got %s", text(u.sizes()).c_str());
@@ -290,7 +292,7 @@ PyObject *selective_scan(PyObject *const *a, Py_ssize_t n) {
     if (bytes) ws = at::empty({(int64_t)bytes}, u.options().dtype(at::kByte));
     check("mi_selective_scan",
           g_scan(ur.p, ur.ld, ur.bs, tr.p, tr.ld, tr.bs, am, br.p, br.ld, br.bs, cr.p, cr.ld, cr.bs, skip, zr.p, zr.ld,
-                 zr.bs, bias, PyObject_IsTrue(a[9]) == 1, h_in, h_out, lens, yr.p, yr.ld, yr.bs, code, bi, li, di, ni, gi,
+                 zr.bs, bias, softplus, h_in, h_out, lens, yr.p, yr.ld, yr.bs, code, bi, li, di, ni, gi,
                  bytes ? ws.data_ptr() : nullptr, bytes, stream));
     return y.release();
 }
