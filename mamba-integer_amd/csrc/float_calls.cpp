@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -92,6 +93,9 @@ const Tensor &like(PyObject *o, at::IntArrayRef shape, at::ScalarType type, cons
               (int)t.device().index(), t_device);
     if (t.requires_grad() && c10::GradMode::is_enabled())
         raise(PyExc_ValueError, "%s requires a gradient; the float operators are forward only", name);
+    if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        raise(PyExc_ValueError, "%s carries a tangent; the float operators are forward only", name);
+    if (t.is_neg()) raise(PyExc_ValueError, "%s is a negated view of other values; resolve_neg() makes them", name);
     return t;
 }
 

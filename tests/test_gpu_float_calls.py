@@ -29,3 +29,28 @@ def test_tensors_of_another_device_than_the_streams(cuda, name, monkeypatch):
     monkeypatch.setattr(ops, "_here", lambda: (stream, device + 1))
     with pytest.raises(ValueError, match="current device"):
         call()
+
+
+def test_tangents_are_refused(cuda):
+    """A dual tensor's result would have none, without an error."""
+    from mamba_int import ops
+    x, w = torch.randn(3, 16, device=cuda), torch.ones(16, device=cuda)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.add_rms_norm(dual, w), lambda: ops.add_rms_norm(x, w, residual=dual),
+                     lambda: ops.causal_conv(dual[None], torch.ones(16, 4, device=cuda))):
+            with pytest.raises(ValueError, match="forward only"):
+                call()
+        with torch.autograd.forward_ad._set_fwd_grad_enabled(False):
+            ops.add_rms_norm(dual, w)
+    ops.add_rms_norm(x, w)
+
+
+def test_negated_views_are_refused(cuda):
+    """Their memory holds the values before the negation."""
+    from mamba_int import ops
+    x, w = torch.randn(3, 16, device=cuda), torch.ones(16, device=cuda)
+    neg = torch._neg_view(x)
+    with pytest.raises(ValueError, match="resolve_neg"):
+        ops.add_rms_norm(neg, w)
+    assert torch.equal(ops.add_rms_norm(neg.resolve_neg(), w)[0], ops.add_rms_norm(-x, w)[0])
