@@ -133,6 +133,14 @@ T *vec(PyObject *o, at::IntArrayRef shape, at::ScalarType type, const char *name
     return static_cast<T *>(t.data_ptr());
 }
 
+// The call has written a tensor that was passed in (or None): a backward pass that saved
+// it has to notice.
+void written(PyObject *o) {
+    if (o == Py_None) return;
+    const Tensor &t = THPVariable_Unpack(o);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 PyObject *empty(at::IntArrayRef shape, const Tensor &x, at::ScalarType type) {
     return THPVariable_Wrap(at::empty(shape, x.options().dtype(type)));
 }
@@ -212,6 +220,8 @@ PyObject *add_rms_norm(PyObject *const *a, Py_ssize_t n) {
         yr = rows(y.p, shape, x.scalar_type(), "out", true);
         check("mi_add_rms_norm", g_norm(xr.p, code, xr.ld, rr.p, rcode, rr.ld, w, (float)eps, yr.p, yr.ld, nullptr, 0,
                                         nullptr, ro.p, ro.ld, size_of(T, "tokens"), size_of(d, "dim"), stream));
+        written(a[5]);
+        written(a[6]);
         return Py_BuildValue("(NN)", y.release(), res.release());
     }
     if (unit < 1) raise(PyExc_ValueError, "unit=%lld must be at least 1", (long long)unit);
@@ -222,6 +232,7 @@ PyObject *add_rms_norm(PyObject *const *a, Py_ssize_t n) {
                  static_cast<int8_t *>(THPVariable_Unpack(q.p).data_ptr()), dp,
                  static_cast<float *>(THPVariable_Unpack(scale.p).data_ptr()), ro.p, ro.ld, size_of(T, "tokens"),
                  size_of(d, "dim"), stream));
+    written(a[5]);
     return Py_BuildValue("(NNN)", q.release(), scale.release(), res.release());
 }
 
@@ -247,7 +258,10 @@ PyObject *causal_conv(PyObject *const *a, Py_ssize_t n) {
     Ref y(output(a[8], shape, x));
     const Rows yr = rows(y.p, shape, type, "out", true);
     check("mi_causal_conv", g_conv(xr.p, xr.ld, xr.bs, code, w, bias, size_of(W, "width"), (int)int_of(a[4]), si, so, lens,
-                                   yr.p, yr.ld, yr.bs, size_of(B, "batch"), size_of(L, "len"), size_of(D, "dim"), stream));
+                                   yr.p, yr.ld, yr.bs, size_of(B, "batch"), size_of(L, "len"), size_of(D, "dim"),
+                                   stream));
+    written(a[6]);
+    written(a[8]);
     return y.release();
 }
 
@@ -298,6 +312,8 @@ PyObject *selective_scan(PyObject *const *a, Py_ssize_t n) {
           g_scan(ur.p, ur.ld, ur.bs, tr.p, tr.ld, tr.bs, am, br.p, br.ld, br.bs, cr.p, cr.ld, cr.bs, skip, zr.p, zr.ld,
                  zr.bs, bias, softplus, h_in, h_out, lens, yr.p, yr.ld, yr.bs, code, bi, li, di, ni, gi,
                  bytes ? ws.data_ptr() : nullptr, bytes, stream));
+    written(a[11]);
+    written(a[13]);
     return y.release();
 }
 
@@ -327,6 +343,7 @@ PyObject *w4_matvec(PyObject *const *a, Py_ssize_t n_args) {
     const Rows yr = rows(y.p, shape, x.scalar_type(), "out", true);
     check("mi_w4_matvec", g_w4(xr.p, xr.ld, code, packed, s, stype == at::kHalf ? MI_F16 : MI_F32, zeros, bias, yr.p, yr.ld,
                                size_of(M, "rows"), size_of(n, "n"), size_of(k, "k"), size_of(group, "group"), stream));
+    written(a[8]);
     return y.release();
 }
 

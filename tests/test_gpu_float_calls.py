@@ -54,3 +54,30 @@ def test_negated_views_are_refused(cuda):
     with pytest.raises(ValueError, match="resolve_neg"):
         ops.add_rms_norm(neg, w)
     assert torch.equal(ops.add_rms_norm(neg.resolve_neg(), w)[0], ops.add_rms_norm(-x, w)[0])
+
+
+def test_written_tensors_count_a_version(cuda):
+    """A backward pass that saved a buffer which a call has overwritten since is an error."""
+    from mamba_int import ops
+    x, w = torch.randn(3, 16, device=cuda), torch.ones(16, device=cuda)
+    a, bc = -torch.ones(16, 4, device=cuda), torch.randn(1, 3, 4, device=cuda)
+    packed, s, _ = ops.pack_w4(torch.zeros(4, 16, dtype=torch.uint8, device=cuda), torch.ones(4, 1, device=cuda), 32)
+    out, res, state, h = (torch.empty(*v, device=cuda) for v in ((3, 16), (3, 16), (1, 3, 16), (1, 16, 4)))
+    y = torch.empty(3, 4, device=cuda)
+    calls = [((out, res), lambda: ops.add_rms_norm(x, w, residual=x, residual_out=res, out=out)),
+             ((res,), lambda: ops.add_rms_norm_quant(x, w, residual=x, residual_out=res)),
+             ((out, state), lambda: ops.causal_conv(x[None], torch.ones(16, 4, device=cuda), state_out=state, out=out[None])),
+             ((out, h), lambda: ops.selective_scan(x[None], x[None], a, bc, bc, h_out=h, out=out[None])),
+             ((y,), lambda: ops.w4_matvec(x, packed, s, 4, 32, out=y))]
+    for buffers, call in calls:
+        before, inputs = [b._version for b in buffers], (x._version, w._version)
+        call()
+        assert all(b._version > v for b, v in zip(buffers, before)) and inputs == (x._version, w._version)
+    with torch.inference_mode():
+        buf = torch.empty(3, 16, device=cuda)
+        ops.add_rms_norm(x, w, out=buf)
+    p = torch.ones(1, 16, 4, device=cuda, requires_grad=True)
+    loss = (p * h).sum()
+    ops.selective_scan(x[None], x[None], a, bc, bc, h_in=h, h_out=h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
