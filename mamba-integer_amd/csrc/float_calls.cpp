@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -181,6 +182,8 @@ int64_t int_of(PyObject *o) {
 // (handle of the current stream, its device)
 void *stream_of(PyObject *o) {
     if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2) raise(PyExc_TypeError, "the stream must be a tuple of its handle and device");
+    if (at::tracer::impl::is_dispatch_enabled())
+        raise(PyExc_RuntimeError, "the float operators cannot be traced: the trace would hold their results as constants");
     t_device = (long)int_of(PyTuple_GET_ITEM(o, 1));
     return address(PyTuple_GET_ITEM(o, 0));
 }
