@@ -1,5 +1,6 @@
 """Builds libmamba_int.so (hipcc, gfx950) in-tree, next to this package, and the module
-of the float operators' calls (host C++ against torch) in it."""
+of the float operators' calls (host C++ against torch) in it.  The library needs hipcc
+alone; without torch, a C++ compiler or Python's headers the module is left out."""
 from __future__ import annotations
 
 import concurrent.futures
@@ -40,9 +41,20 @@ def _run(cmd: list, verbose: bool) -> None:
     errs = "\n".join(l for l in (res.stdout + res.stderr).splitlines()
                      if "packed-fp32-ops" not in l)
     if res.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({res.returncode}): {' '.join(cmd)}\n{errs}")
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({res.returncode}): {' '.join(cmd)}\n{errs}")
     if verbose and errs.strip():
         print(errs, file=sys.stderr)
+
+
+def calls_missing() -> list:
+    """What the calls' module would need here and does not find."""
+    import importlib.util
+    missing = [] if importlib.util.find_spec("torch") else ["torch"]
+    if shutil.which(CXX) is None:
+        missing.append(CXX)
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        missing.append("Python.h")
+    return missing
 
 
 def calls_command(out: str) -> list:
@@ -60,20 +72,29 @@ def calls_command(out: str) -> list:
 def build(verbose: bool = False) -> str:
     """Compiles every source to an object in parallel (each file's kernels are
     self-contained: no relocatable device code), then links the library; beside
-    them, the calls' module."""
+    them, the calls' module.  An error of the module's leaves the library built."""
     srcs = sources()
+    missing = calls_missing()
     with tempfile.TemporaryDirectory(prefix="mamba_int_build_") as tmp:
         objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in srcs]
         jobs = [[HIPCC, *FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", s, "-o", o] for s, o in zip(srcs, objs)]
-        jobs.append(calls_command(os.path.join(tmp, "calls.so")))
-        workers = max(1, min(len(jobs), os.cpu_count() or 1, 8))
+        calls = os.path.join(tmp, "calls.so")
+        workers = max(1, min(len(jobs) + 1, os.cpu_count() or 1, 8))
         with concurrent.futures.ThreadPoolExecutor(max_workers=workers) as pool:
-            for f in [pool.submit(_run, j, verbose) for j in jobs]:
+            futures = [pool.submit(_run, j, verbose) for j in jobs]
+            module = None if missing else pool.submit(lambda: _run(calls_command(calls), verbose))
+            for f in futures:
                 f.result()
         _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", LIB_PATH + ".tmp"], verbose)
-        shutil.copyfile(os.path.join(tmp, "calls.so"), CALLS_PATH + ".tmp")
-    os.replace(CALLS_PATH + ".tmp", CALLS_PATH)
-    os.replace(LIB_PATH + ".tmp", LIB_PATH)
+        os.replace(LIB_PATH + ".tmp", LIB_PATH)
+        if os.path.exists(CALLS_PATH):
+            os.remove(CALLS_PATH)          # never one of another build's
+        if module is None:
+            print(f"the module of the float operators' calls is left out: no {', '.join(missing)}", file=sys.stderr)
+        else:
+            module.result()
+            shutil.copyfile(calls, CALLS_PATH + ".tmp")
+            os.replace(CALLS_PATH + ".tmp", CALLS_PATH)
     return LIB_PATH
 
 

@@ -484,7 +484,11 @@ _ACTIVATIONS = {None: 0, "none": 0, "silu": 1}
 @functools.lru_cache(maxsize=None)
 def _calls():
     lib = _lib.load()
-    from . import _float_calls     # built with the library: its absence is an error
+    try:
+        from . import _float_calls
+    except ImportError as e:
+        raise ImportError("the module of the float operators' calls is not built; build the library where torch, a C++ "
+                          "compiler and Python's headers are") from e
     entries = ("mi_add_rms_norm", "mi_causal_conv", "mi_selective_scan_workspace_size", "mi_selective_scan",
                "mi_w4_matvec", "mi_last_error_string")
     _float_calls.init(_lib.MIError, *(ctypes.cast(getattr(lib, e), ctypes.c_void_p).value for e in entries))
