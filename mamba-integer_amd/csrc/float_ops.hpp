@@ -10,7 +10,6 @@ typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
 inline bool known_type(int t) { return t == MI_F32 || t == MI_BF16 || t == MI_F16; }
-inline int type_size(int t) { return t == MI_F32 ? 4 : 2; }
 
 // Calls f with a value of the element type's C++ type.
 template <class F>

@@ -10,7 +10,7 @@
 
 namespace mi {
 
-constexpr int kNormMaxDim = 16384;
+constexpr int kNormMaxDim = 16384;   // 8 vectors of 16 bits a thread, 16 of 32 bits
 
 struct NormArgs {
     const void *x, *res;
@@ -172,7 +172,7 @@ void launch_rows(const NormArgs &a, hipStream_t st) {
     hipLaunchKernelGGL((add_rms_norm_kernel<T, R, TPR, E>), dim3((unsigned)blocks), dim3(256), 0, st, a);
 }
 
-// A wave a row while a lane holds at most 32 elements, then a block a row.
+// A wave a row while a lane holds at most 32 elements, then a block a row (up to 64 a thread).
 template <class T, class R>
 void launch_add_rms_norm(const NormArgs &a, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);
@@ -187,15 +187,13 @@ void launch_add_rms_norm(const NormArgs &a, hipStream_t st) {
         launch_rows<T, R, 64, 3>(a, st);
     else if (e <= 4)
         launch_rows<T, R, 64, 4>(a, st);
-    else if (V == 4 && e <= 8)
-        launch_rows<T, R, 64, 8>(a, st);
     else if (e <= 8)
-        launch_rows<T, R, 256, 2>(a, st);
+        launch_rows<T, R, V == 4 ? 64 : 256, V == 4 ? 8 : 2>(a, st);
     else if (e <= 16)
         launch_rows<T, R, 256, 4>(a, st);
-    else if (e <= 32)
+    else if (V == 8 || e <= 32)
         launch_rows<T, R, 256, 8>(a, st);
-    else
+    else if constexpr (V == 4)
         launch_rows<T, R, 256, 16>(a, st);
 }
 
