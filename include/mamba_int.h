@@ -531,6 +531,7 @@ typedef enum { MI_F32 = 0, MI_BF16 = 1, MI_F16 = 2 } mi_dtype;
  *            [tokens]: scale = max(max |y|, 1e-8) / 127 and q = clamp(
  *            round_half_even(y * (127 / max(max |y|, 1e-8))), +-127), the rule
  *            of mi_act_quant_f32.  A row with a NaN in y has a NaN scale.
+ * Squares are summed in 32 bits: a row whose sum passes 3.4e38 has y of zeros.
  * dim in [1, 16384]; dim <= ldq <= 32768; tokens < 2^22. */
 mi_status mi_add_rms_norm(const void *x, int x_type, int64_t ldx, const void *residual, int res_type,
                           int64_t ldr, const float *weight, float eps, void *y, int64_t ldy, int8_t *q,
@@ -591,8 +592,12 @@ mi_status mi_pack_w4(const uint8_t *codes, const void *scales, int scale_type, c
 /* y[m,n] = bias[n] + sum_k x[m,k] * (code[n,k] - zero[n,k/group]) *
  * scale[n,k/group] (n <= 2^28, k <= 2^30): x and y rows of `type`, weights as mi_pack_w4 lays them
  * out (zeros NULL: 8), bias fp32 [n] nullable.  Made for the few rows of a
- * decode step (m up to 64 read the weights once); any m is computed.  A float32
- * or bf16 row with an infinite x gives NaN where the product is infinite. */
+ * decode step; any m is computed (up to 32 rows read the weights once, more rows
+ * once for every 32).  A float32 or bf16 row with an infinite x gives NaN where
+ * the product is infinite.  float32 and f16 weights have their zero points taken
+ * off exactly; bf16 products are made with 16 + code and (16 + zero) * sum(x)
+ * taken off, so their 32-bit sums carry about ten times the rounding where x has
+ * one sign. */
 mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const uint8_t *packed, const void *scales,
                        int scale_type, const uint8_t *zeros, const float *bias, void *y, int64_t ldy, int m,
                        int n, int k, int group, void *stream);

@@ -150,7 +150,9 @@ struct W4Type<float> {
 // so a lane's results belong to one weight row and its scale.  Row sums of x (bf16)
 // come from a product with ones.
 // The loads of a whole column block stand in no branch (one in a branch is waited for
-// where it ends); the columns past the whole blocks are a last step of their own.
+// where it ends), though where its products are many the compiler issues some of x's
+// among them (three of the eight with 16-bit rows, MT 2, NT 4 and groups of 32); the
+// columns past the whole blocks are a last step of their own.
 template <class T, class S, int MT, int NT, int KS, int PER>
 __global__ __launch_bounds__(64 * KS) void w4_kernel(W4Args<T, S> a) {
     using W = W4Type<T>;
@@ -295,14 +297,17 @@ void launch_w4(const W4Args<T, S> &a, hipStream_t st) {
         hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, KS, 1>), grid, dim3(64 * KS), 0, st, a);
 }
 
-// More weight rows a block read x fewer times; fewer leave more blocks.  Measured (us
-// of a call among others, 6.8 of them the host's; weights of three sets in turn): NT 4, 2
-// and 1, 16-bit rows, 8 x 2048 -> 32000 9.1 to 10.1, 10.5 to 11.4, 14.0; 1 x 2048 -> 8192
-// 8.2 to 9.1, 7.5 to 7.8, 7.1; MT 2 and NT 4, 2: 64 x 2048 -> 8192 9.0 to 9.6 and 12.2; 64
-// x 2048 -> 2048 7.7 and 7.0 to 7.4.  64 rows as one tile of x, 64 x 2048 -> 8192: 11.9 to
-// 12.6, as two of 32 rows, which read the weights twice, 9.0 to 9.6.  Four waves instead of
-// eight where column blocks are fewer than those: 64 x 768 -> 32000 14.7 to
-// 15.3 and 17.8.
+// More weight rows a block read x fewer times; fewer leave more blocks.  Kernel times in
+// us (traced, weights of three sets in turn), bf16 rows and groups of 128 unless named.
+// One tile of 16 rows of x, NT 4, 2 and 1: 1 x 2048 -> 32000 8.1, 9.6, 8.9; 8 x 2048 ->
+// 32000 10.1, 10.9, 13.7; 1 x 2048 -> 8192 5.2, 3.9, 4.1; 1 x 2048 -> 2048 4.7, 3.4, 3.1.
+// Two tiles, NT 4 and 2: 64 x 2048 -> 8192 8.3 and 11.1, f16 with groups of 32 9.3 and 12.0;
+// 64 x 2048 -> 2048 7.5 and 7.2.  64 rows as one block of four tiles, 64 x 2048 -> 8192: 13.2,
+// as two of two tiles, which read the weights twice, 8.3.  Four waves and eight where column
+// blocks are fewer than those: 64 x 768 -> 32000 14.8 and 17.7 (float32 rows, groups of 64:
+// 35.1 and 30.6).  One tile a block is faster than the two taken for 17 to 32 rows (32 x 2048
+// -> 8192, NT 4: 6.2, two tiles and NT 2 8.0) and for few row blocks (64 x 2048 -> 2048, NT 2:
+// 5.0 and 7.2).
 template <class T, class S>
 void launch_w4_shape(const W4Args<T, S> &a, hipStream_t st) {
     const int nb = (a.n + kW4Rows - 1) / kW4Rows, kb = (a.k + kW4Cols - 1) / kW4Cols, cus = device_cus();

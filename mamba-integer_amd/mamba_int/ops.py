@@ -474,9 +474,11 @@ def embed_argmax(keys, ids_out, emb, r, row_stats) -> None:
 
 # -------------------------------------------- float operators (forward only)
 # Rows may be strided views (a half of in_proj's rows, slices of x_proj's): only
-# the elements of a row must be adjacent.  Inputs that require gradients are
-# refused while autograd records: these operators have no backward.  The tensors'
-# checks, the outputs and the call are csrc/float_calls.cpp's.
+# the elements of a row must be adjacent.  Tensors have to be on the current device,
+# and outputs must not overlap inputs except where stated.  Inputs that require
+# gradients are refused while autograd records, and so are dual tensors and calls
+# inside a trace: these operators have no backward.  The tensors' checks, the outputs
+# and the call are csrc/float_calls.cpp's.
 _FLOAT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _ACTIVATIONS = {None: 0, "none": 0, "silu": 1}
 
