@@ -13,9 +13,10 @@
 namespace mi {
 
 constexpr int kScanMaxStates = 256;
-// Up to these steps a lane walks them with their loads (us, that and the tiles below: 1
-// x 1536 channels 8 steps 8.2 and 8.6, 16 steps 13.3 and 9.3; 64 x 4096 8 steps 26 and 31,
-// 12 steps 41 and 31).
+// Up to these steps a lane walks them with their loads, a memory latency each.  Kernel
+// times in us, that and the tiles below, of 2, 4 and 8 steps: 1 x 1536 channels 4.1, 5.0, 8.2
+// and 4.4, 4.5, 4.6; 64 x 4096 13.9, 20.4, 32.4 and 25.8, 25.6, 26.2.  (The tiles are ahead
+// from 4 and 6 steps on; the host covers the difference where channels are few.)
 constexpr int kScanStepLen = 8;
 constexpr int64_t kScanMaxLd = (int64_t)1 << 25;   // 16 rows' offsets in 32 bits
 
@@ -293,8 +294,7 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
         const int n0 = wave * S;
         float am[S / 4][4], h[S / 4][4];
         // a channel's values from n0 on of rows of N states: four at once where N % 4 == 0
-        // (3 x 701 x 1000 x 64 53.3 us instead of 59.5; 8 x 2048 x 1536 x 16 151.0 instead of
-        // 149.1)
+        // (3 x 701 x 1000 x 64 49.1 us instead of 54.6; 8 x 2048 x 1536 x 16 the same)
         auto states = [&](const float *p, float (&o)[S / 4][4]) {
 #pragma unroll
             for (int q = 0; q < S / 4; ++q) {
