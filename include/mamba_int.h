@@ -561,8 +561,9 @@ mi_status mi_causal_conv(const void *x, int64_t ldx, int64_t bsx, int type, cons
  * nstate values of `type`; d_skip, dt_bias fp32 [dim], z: nullable; h_in /
  * h_out fp32 [batch,dim,nstate] nullable (NULL h_in: zeros), may be the same.
  * lens as for mi_causal_conv (h_out: the state after lens[b] tokens).
- * Infinite values give what the formulas give, except that an infinite state
- * may become a NaN at a step whose decay exp(d * a) is below 2^-126.
+ * Infinite values give what the formulas give, except that a of -inf is taken
+ * as the lowest float (d = 0 keeps the state), and that an infinite state may
+ * become a NaN at a step whose decay exp(d * a) is below 2^-126.
  * workspace: 16-byte aligned, mi_selective_scan_workspace_size bytes (0: may
  * be NULL).  nstate in [1, 256]; batch * dim, groups * nstate and, for more
  * than 8 steps, row strides <= 2^25; len <= 2^30. */

@@ -46,6 +46,10 @@ __device__ __forceinline__ float softplus(float v) {
     return v > 0.0f ? v + s : (v <= 0.0f ? s : v);
 }
 
+// A decay of -inf is the lowest float's: a step of 0 then keeps the state whatever a is.
+// (The maximum that keeps a NaN, one instruction.)
+__device__ __forceinline__ float finite_decay(float a) { return __builtin_elementwise_maximum(a, -kMaxFloat); }
+
 // LANES lanes of a wave hold a channel, four states each (adjacent: 16-byte loads
 // of the state, of A and of B and C's rows where N % 4 == 0); step after step.
 template <class T, int LANES, bool QUADS>
@@ -74,6 +78,8 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs<T> a) {
     };
     float h[4] = {}, am[4] = {};
     four(a.a + (int64_t)c * N + n0, am);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) am[i] = finite_decay(am[i]);
     if (a.h_in) four(a.h_in + (int64_t)ch * N + n0, h);
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.0f, skip = a.d_skip ? a.d_skip[c] : 0.0f;
     for (int t = 0; t < len; ++t) {
@@ -139,7 +145,9 @@ __global__ __launch_bounds__(256) void scan_token_kernel(ScanArgs<T> a) {
         cn[s] = load_packed<4>(a.c.row(b[s], 0) + g0);
         if (a.z.p) z[s] = a.z.row(b[s], 0)[c];
     }
-    const Packed<float, 4> am = load_packed<4>(a.a + (int64_t)c * N + n0);
+    Packed<float, 4> am = load_packed<4>(a.a + (int64_t)c * N + n0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) am.v[i] = finite_decay(am.v[i]);
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.0f, skip = a.d_skip ? a.d_skip[c] : 0.0f;
 #pragma unroll
     for (int s = 0; s < kSeqs; ++s) {
@@ -147,13 +155,13 @@ __global__ __launch_bounds__(256) void scan_token_kernel(ScanArgs<T> a) {
         const float uf = (float)u[s];
         float d = (float)dt[s] + bias;
         if (a.softplus) d = softplus(d);
-        const float du = d * uf;
+        const float du = d * uf, dl = kLog2e * d;
         float y = 0.0f;
         Packed<float, 4> next;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float was = a.h_in ? h[s].v[i] : 0.0f;
-            const float now = __builtin_fmaf(__builtin_amdgcn_exp2f(kLog2e * (d * am.v[i])), was, du * (float)bn[s].v[i]);
+            const float now = __builtin_fmaf(__builtin_amdgcn_exp2f(dl * am.v[i]), was, du * (float)bn[s].v[i]);
             y = __builtin_fmaf((float)cn[s].v[i], now, y);
             next.v[i] = run ? now : was;
         }
@@ -313,7 +321,7 @@ scan_tile_kernel(ScanArgs<T> a, ScanSplit sp) {
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             float &v = am[i / 4][i % 4];
-            v = v < -kMaxFloat ? -kMaxFloat : v;  // (a step of 0 then keeps the state whatever a is)
+            v = finite_decay(v);
             h[i / 4][i % 4] = 0.0f;
         }
         if (PASS != kParts && k == 0 && a.h_in) states(a.h_in + (b * a.dim + c) * N, h);

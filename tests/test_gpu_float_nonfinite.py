@@ -111,3 +111,30 @@ def test_the_fastest_decays(cuda, B, L, D, N):
     # (the bound of a decay of 0 is not finite: its exponent's error times 0 is meant)
     same(got, y, torch.where(torch.isfinite(ey), ey, 8 * R.U * y.abs()), torch.float32)
     same(h, hw, torch.where(torch.isfinite(eh), eh, 8 * R.U * hw.abs()), torch.float32)
+
+
+@pytest.mark.parametrize("B,L,D,N", [(2, 1, 9, 16), (2, 1, 9, 5), (2, 5, 9, 16), (2, 5, 9, 5), (2, 30, 9, 16), (1, 200, 9, 16)])
+def test_decays_of_minus_infinity(cuda, B, L, D, N):
+    """... are the lowest float's, in a prompt as token by token: a step of 0 keeps the state."""
+    s = positive(B, L, D, N, torch.float32, L)
+    s["a"].fill_(-float("inf"))
+    s["dt"].zero_()
+    s["dt"][:, L // 2, 3] = 0.25
+    s["h_in"] = torch.ones(B, D, N)
+    got, h = run(s, cuda, dt_softplus=False)
+    s["a"].fill_(-3.4e38)
+    y, ey, hw, eh = R.scan(s["u"], s["dt"], s["a"], s["b"], s["c"], s["d_skip"], sp=False, h_in=s["h_in"])
+    same(got, y, torch.where(torch.isfinite(ey), ey, 8 * R.U * y.abs()), torch.float32)
+    same(h, hw, torch.where(torch.isfinite(eh), eh, 8 * R.U * hw.abs()), torch.float32)
+
+
+@pytest.mark.parametrize("B,L,D,N", [(2, 1, 9, 16), (2, 5, 9, 5), (2, 30, 9, 12), (1, 200, 9, 16)])
+def test_a_decay_that_is_no_number(cuda, B, L, D, N):
+    s = positive(B, L, D, N, torch.float32, L)
+    s["a"][4, N - 1] = float("nan")
+    s["h_in"] = torch.ones(B, D, N)
+    got, h = run(s, cuda)
+    bad = torch.zeros(D, dtype=torch.bool, device=cuda)
+    bad[4] = True
+    assert torch.equal(torch.isnan(got), bad.expand(B, L, D))
+    assert torch.isnan(h[:, 4, N - 1]).all() and int(torch.isnan(h).sum()) == B
