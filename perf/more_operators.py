@@ -87,9 +87,9 @@ def draw(rng):
         n = rng.choice([768, 2048, 8192, _log(rng, 200, 8192)])
         rank = rng.choice([4, 8, 16, 32, 64, _log(rng, 1, 64)])
         length = 1 if rng.random() < 0.5 else _log(rng, 2, 2048)
-        most = max(1, 8 * 2048 * 6144 // (length * (k + n)) * 32 // max(rank, 32))
-        batch = _log(rng, 1, min(64, most))
         typ = rng.choice(["f32", "bf16", "f16", "i8"])
+        most = 8 * 2048 * 6144 * 32 // (length * (k + n) * max(rank, 32) * (1 if typ in ("bf16", "f16") else 2))
+        batch = _log(rng, 1, max(1, min(64, most)))
         return {"kind": kind, "batch": batch, "len": length, "k": k, "n": n, "rank": rank, "bank": _log(rng, 1, 128),
                 "type": typ, "weights": rng.choice(["f32", "bf16", "f16"]), "out": "f32" if typ == "i8" else typ,
                 "lens": length > 1 and rng.random() < 0.3, "none": rng.choice([0.0, 0.3])}
