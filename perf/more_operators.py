@@ -323,7 +323,7 @@ def _exact_sample(s):
     import numpy as np
     logits, u = s["logits"].double().cpu().numpy(), s["u"].double().cpu().numpy()
     B, V = logits.shape
-    par = {n: np.broadcast_to(v.double().cpu().numpy() if isinstance(v, torch.Tensor) else np.float64(v), (B,))
+    par = {n: np.broadcast_to(v.double().cpu().numpy() if isinstance(v, torch.Tensor) else np.float64(np.float32(v)), (B,))
            for n, v in ((n, s[n]) for n in ("temperature", "top_k", "top_p", "min_p"))}
     ids, logprob = np.zeros(B, np.int64), np.zeros(B)
     for b in range(B):
