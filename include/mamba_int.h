@@ -518,7 +518,12 @@ mi_status mi_decode_step_static(const mi_model_params *params, int m, const int6
  * strides (bs*) count elements; a stride of an input may be 0 (one row for
  * all).  The elements of a row are adjacent.  Outputs must not overlap inputs
  * except where stated. */
-typedef enum { MI_F32 = 0, MI_BF16 = 1, MI_F16 = 2 } mi_dtype;
+typedef enum {
+    MI_F32 = 0,
+    MI_BF16 = 1,
+    MI_F16 = 2,
+    MI_I32 = 3, /* logits of mi_sample_tokens only */
+} mi_dtype;
 
 /* Residual addition and root-mean-square norm of `tokens` rows of dim values:
  *   s = residual + x,  y = s / sqrt(mean(s^2) + eps) * weight
@@ -602,6 +607,35 @@ mi_status mi_pack_w4(const uint8_t *codes, const void *scales, int scale_type, c
 mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const uint8_t *packed, const void *scales,
                        int scale_type, const uint8_t *zeros, const float *bias, void *y, int64_t ldy, int m,
                        int n, int k, int group, void *stream);
+
+/* The next token of each of `rows` rows of `vocab` logits, drawn with a given
+ * random number.  With l = logit * scale, e_i = exp((l_i - max l) /
+ * temperature) and the order "larger l first, of equal ones the lower token":
+ *   keep the first top_k tokens of the order (top_k <= 0 or >= vocab: all);
+ *   of those the shortest beginning of the order whose sum of e is at least
+ *   top_p times theirs (top_p >= 1 or a NaN: all; at least one token);
+ *   of those the tokens with e >= min_p (min_p <= 0 or a NaN: all), and the
+ *   first of the order in any case.
+ * ids: the first kept token, by number, at which the sum of the kept e up to
+ * and with it exceeds u times the sum of them all (u <= 0 or a NaN: the first
+ * kept one with a mass; u >= 1: the last).  logprob, nullable: log of the
+ * token's e over that sum.  temperature <= 0 or a NaN: the first of the order,
+ * logprob 0.  A NaN or -inf is never drawn; a row of nothing else has id -1 and
+ * logprob -inf.  Where the largest logit is +inf, the tokens with +inf have e =
+ * 1 and the others 0.  Sums are exact: a token's mass is e as a 64-bit
+ * integer in units of 2^-(62 - ceil(log2 vocab)), at least 2^-52 (an e below
+ * half a unit is 0), so a row's token depends on nothing but the row.
+ *   logits  rows of type MI_F32, MI_BF16, MI_F16 or MI_I32, ld elements from
+ *           one to the next; scale in (0, 1e30];
+ *   u       fp32 [rows];
+ *   temperature, top_k, top_p, min_p   [rows], or NULL for the one value
+ *           *_all of every row (which must be a number);
+ *   ids int64, logprob fp32 [rows].
+ * vocab in [1, 2^24], rows < 2^22. */
+mi_status mi_sample_tokens(const void *logits, int type, int64_t ld, double scale, const float *u,
+                           const float *temperature, float temperature_all, const int32_t *top_k, int top_k_all,
+                           const float *top_p, float top_p_all, const float *min_p, float min_p_all,
+                           int64_t *ids, float *logprob, int rows, int vocab, void *stream);
 
 /* ------------------------------------------------ integer checkpoints */
 /* The integer parameters above in a versioned file (format 2, spec

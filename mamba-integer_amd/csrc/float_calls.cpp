@@ -1,5 +1,5 @@
 // The host side of the float operators' calls (mamba_int.ops: add_rms_norm,
-// add_rms_norm_quant, causal_conv, selective_scan, w4_matvec): checks of the
+// add_rms_norm_quant, causal_conv, selective_scan, w4_matvec, sample_tokens): checks of the
 // tensors, outputs, and the call of the C ABI, as a Python module.  Through ctypes
 // and checks in Python a call took 9 to 18 us of host time, several times what its
 // kernel takes on a decode step's rows.
@@ -28,6 +28,7 @@ decltype(&mi_causal_conv) g_conv;
 decltype(&mi_selective_scan) g_scan;
 decltype(&mi_selective_scan_workspace_size) g_scan_size;
 decltype(&mi_w4_matvec) g_w4;
+decltype(&mi_sample_tokens) g_sample;
 decltype(&mi_last_error_string) g_last_error;
 PyObject *g_mi_error;   // _lib.MIError
 
@@ -65,6 +66,7 @@ const char *type_name(at::ScalarType t) {
         case at::kBFloat16: return "bfloat16";
         case at::kHalf: return "float16";
         case at::kInt: return "int32";
+        case at::kLong: return "int64";
         case at::kByte: return "uint8";
         default: return c10::toString(t);
     }
@@ -350,17 +352,60 @@ PyObject *w4_matvec(PyObject *const *a, Py_ssize_t n_args) {
     return y.release();
 }
 
-// (MIError, addresses of the six entry points)
+// A parameter of every row: a tensor [rows] of this type, or one number for all of them.
+template <class T>
+const T *each(PyObject *o, int64_t rows, at::ScalarType type, const char *name, T &all) {
+    if (THPVariable_Check(o)) return vec<T>(o, {rows}, type, name);
+    if constexpr (std::is_same<T, float>::value) {
+        all = (float)PyFloat_AsDouble(o);
+        if (PyErr_Occurred()) throw Raised{};
+    } else {
+        all = (T)std::min<int64_t>(std::max<int64_t>(int_of(o), INT32_MIN), INT32_MAX);
+    }
+    return nullptr;
+}
+
+// (stream, logits, u, temperature, top_k, top_p, min_p, scale, logprob, out)
+PyObject *sample_tokens(PyObject *const *a, Py_ssize_t n) {
+    count(n, 10, "sample_tokens");
+    void *stream = stream_of(a[0]);
+    const Tensor &x = tensor(a[1], "logits");
+    const int code = x.scalar_type() == at::kInt ? (int)MI_I32 : float_type(x, "logits");
+    if (x.dim() != 2) raise(PyExc_ValueError, "logits must be [rows, vocab], got %s", text(x.sizes()).c_str());
+    const int64_t B = x.size(0), V = x.size(1);
+    const double scale = PyFloat_AsDouble(a[7]);
+    if (PyErr_Occurred()) throw Raised{};
+    const int with_logprob = PyObject_IsTrue(a[8]);
+    if (with_logprob < 0) throw Raised{};
+    const Rows xr = rows(a[1], x.sizes(), x.scalar_type(), "logits");
+    const float *u = vec<float>(a[2], {B}, at::kFloat, "u");
+    float t_all = 1.0f, p_all = 1.0f, min_all = 0.0f;
+    int32_t k_all = 0;
+    const float *t = each<float>(a[3], B, at::kFloat, "temperature", t_all);
+    const int32_t *k = each<int32_t>(a[4], B, at::kInt, "top_k", k_all);
+    const float *p = each<float>(a[5], B, at::kFloat, "top_p", p_all), *least = each<float>(a[6], B, at::kFloat, "min_p", min_all);
+    Ref ids(a[9] != Py_None ? (Py_INCREF(a[9]), a[9]) : empty({B}, x, at::kLong));
+    int64_t *ip = vec<int64_t>(ids.p, {B}, at::kLong, "out");
+    Ref lp(with_logprob ? empty({B}, x, at::kFloat) : (Py_INCREF(Py_None), Py_None));
+    float *lpp = with_logprob ? static_cast<float *>(THPVariable_Unpack(lp.p).data_ptr()) : nullptr;
+    check("mi_sample_tokens", g_sample(xr.p, code, xr.ld, scale, u, t, t_all, k, k_all, p, p_all, least, min_all, ip, lpp,
+                                       size_of(B, "rows"), size_of(V, "vocab"), stream));
+    written(a[9]);
+    return with_logprob ? Py_BuildValue("(NN)", ids.release(), lp.release()) : ids.release();
+}
+
+// (MIError, addresses of the entry points)
 PyObject *init(PyObject *const *a, Py_ssize_t n) {
-    count(n, 7, "init");
-    void *p[6];
-    for (int i = 0; i < 6; ++i) p[i] = address(a[i + 1]);
+    count(n, 8, "init");
+    void *p[7];
+    for (int i = 0; i < 7; ++i) p[i] = address(a[i + 1]);
     g_norm = reinterpret_cast<decltype(g_norm)>(p[0]);
     g_conv = reinterpret_cast<decltype(g_conv)>(p[1]);
     g_scan_size = reinterpret_cast<decltype(g_scan_size)>(p[2]);
     g_scan = reinterpret_cast<decltype(g_scan)>(p[3]);
     g_w4 = reinterpret_cast<decltype(g_w4)>(p[4]);
-    g_last_error = reinterpret_cast<decltype(g_last_error)>(p[5]);
+    g_sample = reinterpret_cast<decltype(g_sample)>(p[5]);
+    g_last_error = reinterpret_cast<decltype(g_last_error)>(p[6]);
     Py_INCREF(a[0]);
     Py_XDECREF(g_mi_error);
     g_mi_error = a[0];
@@ -383,7 +428,7 @@ PyObject *guarded(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 #define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<f>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(init),           METHOD(add_rms_norm), METHOD(causal_conv),
-                         METHOD(selective_scan), METHOD(w4_matvec),    {nullptr, nullptr, 0, nullptr}};
+                         METHOD(selective_scan), METHOD(w4_matvec),    METHOD(sample_tokens), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_float_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -492,7 +492,7 @@ def _calls():
         raise ImportError("the module of the float operators' calls is not built; build the library where torch, a C++ "
                           "compiler and Python's headers are") from e
     entries = ("mi_add_rms_norm", "mi_causal_conv", "mi_selective_scan_workspace_size", "mi_selective_scan",
-               "mi_w4_matvec", "mi_last_error_string")
+               "mi_w4_matvec", "mi_sample_tokens", "mi_last_error_string")
     _float_calls.init(_lib.MIError, *(ctypes.cast(getattr(lib, e), ctypes.c_void_p).value for e in entries))
     return _float_calls
 
@@ -586,3 +586,19 @@ def w4_matvec(x, packed, scales, n: int, group: int, zeros=None, bias=None, out=
     """y [M, n] = x [M, K] @ W^T (+ bias float32 [n]) for the 4-bit weights of ``pack_w4``:
     made for the rows of a decode step (1..64; more are computed too).  Forward only."""
     return _calls().w4_matvec(_here(), x, packed, scales, n, group, zeros, bias, out)
+
+
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, scale: float = 1.0, logprob: bool = False,
+                  out=None):
+    """The next token of each row of logits [B, V] (any float type, or int32 that count in
+    ``scale``), drawn with the random numbers u float32 [B] in [0, 1): ids int64 [B], or with
+    ``logprob`` (ids, the log of the probability each was drawn with float32 [B]).
+
+    With l = logits * scale, e = exp((l - max l) / temperature) and tokens in the order of
+    their l (equal ones by number): the first top_k are kept (0: all), of those the fewest
+    first ones with at least top_p of their sum of e (1: all), of those the ones with e >=
+    min_p; the first of the order in any case.  The token is the first kept one, by number,
+    at which their sum of e exceeds u of the whole.  temperature 0 takes the first of the
+    order.  The four parameters are numbers or tensors [B] (float32; top_k int32).  NaN and
+    -inf are never drawn; a row with nothing else has id -1.  Forward only."""
+    return _calls().sample_tokens(_here(), logits, u, temperature, top_k, top_p, min_p, scale, logprob, out)
