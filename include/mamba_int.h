@@ -523,6 +523,7 @@ typedef enum {
     MI_BF16 = 1,
     MI_F16 = 2,
     MI_I32 = 3, /* logits of mi_sample_tokens only */
+    MI_I8 = 4   /* rows of mi_adapter_add only */
 } mi_dtype;
 
 /* Residual addition and root-mean-square norm of `tokens` rows of dim values:
@@ -636,6 +637,55 @@ mi_status mi_sample_tokens(const void *logits, int type, int64_t ld, double scal
                            const float *temperature, float temperature_all, const int32_t *top_k, int top_k_all,
                            const float *top_p, float top_p_all, const float *min_p, float min_p_all,
                            int64_t *ids, float *logprob, int rows, int vocab, void *stream);
+
+/* Low-rank adapters beside a shared projection, each sequence with its own of
+ * a bank:
+ *   out[b,t,:] = y[b,t,:] + scales[id] * x_scale[b,t] * (x[b,t,:] A[id]^T) B[id]^T
+ * with id = ids[b]; out = y where id is not in [0, bank), and for the tokens of
+ * sequence b from lens[b] on.  x rows of k values of `type`, or MI_I8 rows with
+ * a scale each (x_scale fp32 [batch,len], NULL otherwise: 1); y and out rows of
+ * n values of `type`, out may be y itself (with its strides): rows without an
+ * adapter are not touched then.  A [bank,rank,k] and B [bank,n,rank] of
+ * weight_type; scales fp32 [bank], nullable (1); lens int32 [batch], nullable.
+ * The products and the sum with y are in 32 bits, rounded once.  A row with an
+ * infinite x or adapter value may give a NaN where the formula gives an
+ * infinity.  rank in [0, 128]; k and n <= 2^23; batch * len < 2^22.
+ * workspace: 16-byte aligned, mi_adapter_workspace_size bytes. */
+mi_status mi_adapter_workspace_size(int batch, int len, int rank, size_t *bytes);
+mi_status mi_adapter_add(const void *x, int x_type, int64_t ldx, int64_t bsx, const float *x_scale, const void *a,
+                         const void *b, int weight_type, const float *scales, const int32_t *ids,
+                         const int32_t *lens, const void *y, int64_t ldy, int64_t bsy, void *out, int64_t ldo,
+                         int64_t bso, int type, int batch, int len, int k, int n, int rank, int bank,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
+/* Gated linear recurrence over [batch,len,dim] rows of `type`, with h in 32 bits:
+ *   s = sigmoid(r[b,t,c]),  a = exp(-rate * softplus(decay[c]) * s)
+ *   h[c] = a * h[c] + sqrt(1 - a^2) * sigmoid(i[b,t,c]) * x[b,t,c]
+ *   y[b,t,c] = h[c], or h[c] * z / (1 + exp(-z)) with z[b,t,c] (z nullable)
+ * decay fp32 [dim]; rate in [0, 1e30]; h_in / h_out fp32 [batch,dim] nullable
+ * (NULL h_in: zeros), may be the same; lens as for mi_causal_conv (h_out: the
+ * state after lens[b] tokens).  workspace (forward_bytes) and saved
+ * (saved_bytes; nullable: what mi_gated_scan_backward reads of a forward pass
+ * with the same inputs) as mi_gated_scan_sizes says, 16-byte aligned, of any
+ * content.  batch <= 65535, dim <= 2^24, len <= 2^30. */
+mi_status mi_gated_scan_sizes(int batch, int len, int dim, size_t *forward_bytes, size_t *backward_bytes,
+                              size_t *saved_bytes);
+mi_status mi_gated_scan(const void *x, int64_t ldx, int64_t bsx, const void *r, int64_t ldr, int64_t bsr,
+                        const void *i, int64_t ldi, int64_t bsi, const float *decay, float rate, const void *z,
+                        int64_t ldz, int64_t bsz, const float *h_in, float *h_out, const int32_t *lens, void *y,
+                        int64_t ldy, int64_t bsy, float *saved, int type, int batch, int len, int dim,
+                        void *workspace, size_t workspace_bytes, void *stream);
+/* Its gradients from dy, the gradient of y: dx, dr, di, dz contiguous
+ * [batch,len,dim] of `type` (zero for tokens past lens), ddecay fp32 [dim],
+ * dh_in fp32 [batch,dim], each nullable; the other arguments as in the forward
+ * pass, whose `saved` it reads.  workspace: backward_bytes.  No sum depends on
+ * the order in which blocks run. */
+mi_status mi_gated_scan_backward(const void *dy, int64_t ldy, int64_t bsy, const void *x, int64_t ldx, int64_t bsx,
+                                 const void *r, int64_t ldr, int64_t bsr, const void *i, int64_t ldi, int64_t bsi,
+                                 const float *decay, float rate, const void *z, int64_t ldz, int64_t bsz,
+                                 const int32_t *lens, const float *saved, void *dx, void *dr, void *di, void *dz,
+                                 float *ddecay, float *dh_in, int type, int batch, int len, int dim, void *workspace,
+                                 size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------ integer checkpoints */
 /* The integer parameters above in a versioned file (format 2, spec

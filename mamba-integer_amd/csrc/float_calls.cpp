@@ -1,6 +1,6 @@
 // The host side of the float operators' calls (mamba_int.ops: add_rms_norm,
-// add_rms_norm_quant, causal_conv, selective_scan, w4_matvec, sample_tokens): checks of the
-// tensors, outputs, and the call of the C ABI, as a Python module.  Through ctypes
+// add_rms_norm_quant, causal_conv, selective_scan, w4_matvec, sample_tokens, adapter_add,
+// gated_scan): checks of the tensors, outputs, and the call of the C ABI, as a Python module.  Through ctypes
 // and checks in Python a call took 9 to 18 us of host time, several times what its
 // kernel takes on a decode step's rows.
 //
@@ -13,7 +13,10 @@
 #include <ATen/TracerMode.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <stdarg.h>
 
@@ -29,6 +32,11 @@ decltype(&mi_selective_scan) g_scan;
 decltype(&mi_selective_scan_workspace_size) g_scan_size;
 decltype(&mi_w4_matvec) g_w4;
 decltype(&mi_sample_tokens) g_sample;
+decltype(&mi_adapter_workspace_size) g_adapter_size;
+decltype(&mi_adapter_add) g_adapter;
+decltype(&mi_gated_scan_sizes) g_gated_sizes;
+decltype(&mi_gated_scan) g_gated;
+decltype(&mi_gated_scan_backward) g_gated_backward;
 decltype(&mi_last_error_string) g_last_error;
 PyObject *g_mi_error;   // _lib.MIError
 
@@ -394,18 +402,168 @@ PyObject *sample_tokens(PyObject *const *a, Py_ssize_t n) {
     return with_logprob ? Py_BuildValue("(NN)", ids.release(), lp.release()) : ids.release();
 }
 
+// Rows [batch, len, dim], or [batch, dim] as sequences of one token.
+Rows sequences(PyObject *o, bool flat, int64_t B, int64_t L, int64_t D, at::ScalarType type, const char *name, bool out = false) {
+    if (!flat) return rows(o, {B, L, D}, type, name, out);
+    Rows r = rows(o, {B, D}, type, name, out);
+    return {r.p, D, r.ld};
+}
+
+// (stream, y, x, a, b, ids, scales, x_scale, lens, out)
+PyObject *adapter_add(PyObject *const *a, Py_ssize_t n_args) {
+    count(n_args, 10, "adapter_add");
+    void *stream = stream_of(a[0]);
+    const Tensor &y = tensor(a[1], "y"), &x = tensor(a[2], "x"), &am = tensor(a[3], "a"), &bm = tensor(a[4], "b");
+    const int code = float_type(y, "y"), wcode = float_type(am, "a");
+    const bool flat = y.dim() == 2, bytes_in = x.scalar_type() == at::kChar;
+    if (y.dim() != 2 && y.dim() != 3) raise(PyExc_ValueError, "y must be [batch, dim] or [batch, len, dim], got %s", text(y.sizes()).c_str());
+    if (x.dim() != y.dim()) raise(PyExc_ValueError, "x must have y's dimensions, got %s beside %s", text(x.sizes()).c_str(), text(y.sizes()).c_str());
+    if (am.dim() != 3) raise(PyExc_ValueError, "a must be [bank, rank, k], got %s", text(am.sizes()).c_str());
+    const int64_t B = y.size(0), L = flat ? 1 : y.size(1), N = y.size(-1), bank = am.size(0), R = am.size(1), K = am.size(2);
+    const Rows xr = sequences(a[2], flat, B, L, K, bytes_in ? at::kChar : y.scalar_type(), "x");
+    const void *ap = vec<void>(a[3], {bank, R, K}, am.scalar_type(), "a"), *bp = vec<void>(a[4], {bank, N, R}, am.scalar_type(), "b");
+    const int32_t *ids = vec<int32_t>(a[5], {B}, at::kInt, "ids");
+    if (!ids && B > 0) raise(PyExc_TypeError, "ids must be a torch.Tensor");
+    const float *scales = vec<float>(a[6], {bank}, at::kFloat, "scales");
+    if (bytes_in != (a[7] != Py_None)) raise(PyExc_ValueError, "x_scale goes with int8 rows");
+    const float *x_scale = flat ? vec<float>(a[7], {B}, at::kFloat, "x_scale") : vec<float>(a[7], {B, L}, at::kFloat, "x_scale");
+    const int32_t *lens = vec<int32_t>(a[8], {B}, at::kInt, "lens");
+    Ref out(output(a[9], y.sizes(), y));
+    const Rows outr = sequences(out.p, flat, B, L, N, y.scalar_type(), "out", true);
+    Rows yr = sequences(a[1], flat, B, L, N, y.scalar_type(), "y");
+    if (yr.p && yr.p == outr.p) {
+        // (strides of dimensions of one element are free)
+        if ((L > 1 && yr.ld != outr.ld) || (B > 1 && yr.bs != outr.bs))
+            raise(PyExc_ValueError, "out overlaps y: in place, it must have y's strides");
+        yr = outr;
+    }
+    const int bi = size_of(B, "batch"), li = size_of(L, "len"), ri = size_of(R, "rank");
+    size_t bytes = 0;
+    check("mi_adapter_workspace_size", g_adapter_size(bi, li, ri, &bytes));
+    Tensor ws;
+    if (bytes) ws = at::empty({(int64_t)bytes}, y.options().dtype(at::kByte));
+    check("mi_adapter_add",
+          g_adapter(xr.p, bytes_in ? (int)MI_I8 : code, xr.ld, xr.bs, x_scale, ap, bp, wcode, scales, ids, lens, yr.p, yr.ld, yr.bs,
+                    outr.p, outr.ld, outr.bs, code, bi, li, size_of(K, "k"), size_of(N, "n"), ri, size_of(bank, "bank"),
+                    bytes ? ws.data_ptr() : nullptr, bytes, stream));
+    written(a[9]);
+    return out.release();
+}
+
+// What a gated recurrence and its backward pass read.
+struct Gated {
+    int64_t B, L, D;
+    at::ScalarType type;
+    int code, bi, li, di;
+    Rows x, r, i, z;
+    const float *decay;
+    float rate;
+    const int32_t *lens;
+    size_t forward_bytes = 0, backward_bytes = 0, saved_bytes = 0;
+
+    Gated(PyObject *xo, PyObject *ro, PyObject *io, PyObject *decay_o, PyObject *zo, PyObject *rate_o, PyObject *lens_o) {
+        const Tensor &t = tensor(xo, "x");
+        code = float_type(t, "x");
+        if (t.dim() != 3) raise(PyExc_ValueError, "x must be [batch, len, dim], got %s", text(t.sizes()).c_str());
+        B = t.size(0), L = t.size(1), D = t.size(2), type = t.scalar_type();
+        bi = size_of(B, "batch"), li = size_of(L, "len"), di = size_of(D, "dim");
+        x = rows(xo, {B, L, D}, type, "x"), r = rows(ro, {B, L, D}, type, "r"), i = rows(io, {B, L, D}, type, "i");
+        z = zo != Py_None ? rows(zo, {B, L, D}, type, "z") : Rows{};
+        decay = static_cast<const float *>(like(decay_o, {D}, at::kFloat, "decay").data_ptr());
+        if (!THPVariable_Unpack(decay_o).is_contiguous()) raise(PyExc_ValueError, "decay must be contiguous");
+        rate = (float)PyFloat_AsDouble(rate_o);
+        if (PyErr_Occurred()) throw Raised{};
+        lens = vec<int32_t>(lens_o, {B}, at::kInt, "lens");
+        check("mi_gated_scan_sizes", g_gated_sizes(bi, li, di, &forward_bytes, &backward_bytes, &saved_bytes));
+    }
+};
+
+// (stream, x, r, i, decay, z, rate, h_in, h_out, lens, out, save): y, or (y, what the backward pass reads)
+PyObject *gated_scan(PyObject *const *a, Py_ssize_t n) {
+    count(n, 12, "gated_scan");
+    void *stream = stream_of(a[0]);
+    const Gated g(a[1], a[2], a[3], a[4], a[5], a[6], a[9]);
+    const Tensor &x = THPVariable_Unpack(a[1]);
+    const float *h_in = vec<float>(a[7], {g.B, g.D}, at::kFloat, "h_in");
+    float *h_out = vec<float>(a[8], {g.B, g.D}, at::kFloat, "h_out");
+    const bool save = a[11] == Py_True;
+    Ref y(output(a[10], x.sizes(), x));
+    const Rows yr = rows(y.p, x.sizes(), g.type, "out", true);
+    Ref saved(save ? empty({(int64_t)(g.saved_bytes / sizeof(float))}, x, at::kFloat) : (Py_INCREF(Py_None), Py_None));
+    Tensor ws;
+    if (g.forward_bytes) ws = at::empty({(int64_t)g.forward_bytes}, x.options().dtype(at::kByte));
+    check("mi_gated_scan",
+          g_gated(g.x.p, g.x.ld, g.x.bs, g.r.p, g.r.ld, g.r.bs, g.i.p, g.i.ld, g.i.bs, g.decay, g.rate, g.z.p, g.z.ld, g.z.bs, h_in,
+                  h_out, g.lens, yr.p, yr.ld, yr.bs, save ? static_cast<float *>(THPVariable_Unpack(saved.p).data_ptr()) : nullptr,
+                  g.code, g.bi, g.li, g.di, g.forward_bytes ? ws.data_ptr() : nullptr, g.forward_bytes, stream));
+    written(a[8]);
+    written(a[10]);
+    return save ? Py_BuildValue("(NN)", y.release(), saved.release()) : y.release();
+}
+
+// (stream, dy, x, r, i, decay, z, rate, lens, saved, needs): the gradients of x, r, i, decay, z and
+// h_in, None where `needs`, a tuple of six truth values, has a false one.
+PyObject *gated_scan_backward(PyObject *const *a, Py_ssize_t n) {
+    count(n, 11, "gated_scan_backward");
+    void *stream = stream_of(a[0]);
+    const Gated g(a[2], a[3], a[4], a[5], a[6], a[7], a[8]);
+    const Tensor &x = THPVariable_Unpack(a[2]);
+    const Rows dy = rows(a[1], x.sizes(), g.type, "dy");
+    const float *saved = vec<float>(a[9], {(int64_t)(g.saved_bytes / sizeof(float))}, at::kFloat, "saved");
+    if (!PyTuple_Check(a[10]) || PyTuple_GET_SIZE(a[10]) != 6) raise(PyExc_TypeError, "needs must be a tuple of six");
+    const int64_t row[1] = {g.D}, state[2] = {g.B, g.D};
+    const auto grad = [&](int k, at::IntArrayRef shape, at::ScalarType type) {
+        return PyTuple_GET_ITEM(a[10], k) == Py_True ? empty(shape, x, type) : (Py_INCREF(Py_None), Py_None);
+    };
+    Ref dx(grad(0, x.sizes(), g.type)), dr(grad(1, x.sizes(), g.type)), di(grad(2, x.sizes(), g.type)), dd(grad(3, row, at::kFloat)),
+        dz(grad(4, x.sizes(), g.type)), dh(grad(5, state, at::kFloat));
+    const auto at_ = [](const Ref &t) { return t.p == Py_None ? nullptr : THPVariable_Unpack(t.p).data_ptr(); };
+    Tensor ws;
+    if (g.backward_bytes) ws = at::empty({(int64_t)g.backward_bytes}, x.options().dtype(at::kByte));
+    check("mi_gated_scan_backward",
+          g_gated_backward(dy.p, dy.ld, dy.bs, g.x.p, g.x.ld, g.x.bs, g.r.p, g.r.ld, g.r.bs, g.i.p, g.i.ld, g.i.bs, g.decay, g.rate,
+                           g.z.p, g.z.ld, g.z.bs, g.lens, saved, at_(dx), at_(dr), at_(di), at_(dz), static_cast<float *>(at_(dd)),
+                           static_cast<float *>(at_(dh)), g.code, g.bi, g.li, g.di, g.backward_bytes ? ws.data_ptr() : nullptr,
+                           g.backward_bytes, stream));
+    return Py_BuildValue("(NNNNNN)", dx.release(), dr.release(), di.release(), dd.release(), dz.release(), dh.release());
+}
+
+// (stream, name, tensor): raises where the tensor is a leaf whose gradient another live graph
+// adds up on another stream than this one.
+PyObject *check_accumulator(PyObject *const *a, Py_ssize_t n) {
+    count(n, 3, "check_accumulator");
+    void *stream = stream_of(a[0]);
+    const Tensor &t = tensor(a[2], "the input");
+    const char *name = PyUnicode_AsUTF8(a[1]);
+    if (!name) throw Raised{};
+    if (t.requires_grad() && t.is_leaf()) {
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+        const auto on = node ? node->stream() : std::nullopt;
+        // (a stream object of the current stream is the same as what the node keeps)
+        if (on && c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device()) != *on)
+            raise(PyExc_RuntimeError,
+                  "%s is a leaf of another graph that lives, recorded on another stream: a backward pass captured here would make "
+                  "that stream wait for the capture; drop that graph's outputs first", name);
+    }
+    Py_RETURN_NONE;
+}
+
 // (MIError, addresses of the entry points)
 PyObject *init(PyObject *const *a, Py_ssize_t n) {
-    count(n, 8, "init");
-    void *p[7];
-    for (int i = 0; i < 7; ++i) p[i] = address(a[i + 1]);
-    g_norm = reinterpret_cast<decltype(g_norm)>(p[0]);
-    g_conv = reinterpret_cast<decltype(g_conv)>(p[1]);
-    g_scan_size = reinterpret_cast<decltype(g_scan_size)>(p[2]);
-    g_scan = reinterpret_cast<decltype(g_scan)>(p[3]);
-    g_w4 = reinterpret_cast<decltype(g_w4)>(p[4]);
-    g_sample = reinterpret_cast<decltype(g_sample)>(p[5]);
-    g_last_error = reinterpret_cast<decltype(g_last_error)>(p[6]);
+    const auto entry = [&](int i, auto &f) { f = reinterpret_cast<std::decay_t<decltype(f)>>(address(a[i])); };
+    count(n, 13, "init");
+    entry(1, g_norm);
+    entry(2, g_conv);
+    entry(3, g_scan_size);
+    entry(4, g_scan);
+    entry(5, g_w4);
+    entry(6, g_sample);
+    entry(7, g_adapter_size);
+    entry(8, g_adapter);
+    entry(9, g_gated_sizes);
+    entry(10, g_gated);
+    entry(11, g_gated_backward);
+    entry(12, g_last_error);
     Py_INCREF(a[0]);
     Py_XDECREF(g_mi_error);
     g_mi_error = a[0];
@@ -428,7 +586,7 @@ PyObject *guarded(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 #define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<f>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(init),           METHOD(add_rms_norm), METHOD(causal_conv),
-                         METHOD(selective_scan), METHOD(w4_matvec),    METHOD(sample_tokens), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(selective_scan), METHOD(w4_matvec),    METHOD(sample_tokens), METHOD(adapter_add), METHOD(gated_scan), METHOD(gated_scan_backward), METHOD(check_accumulator), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_float_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

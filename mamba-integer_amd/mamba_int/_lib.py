@@ -16,7 +16,7 @@ LIB_PATH = os.environ.get("MAMBA_INT_LIB", os.path.join(PKG_ROOT, "libmamba_int.
 
 MI_OK, MI_ERR_NULL_POINTER, MI_ERR_BAD_DIM, MI_ERR_BAD_ALIGNMENT, MI_ERR_BAD_ARG, MI_ERR_HIP = range(6)
 OUT_INT32, OUT_INT8, OUT_DECAY_MOD, OUT_RESIDUAL, OUT_FLOAT = range(5)
-F32, BF16, F16, I32 = range(4)   # mi_dtype
+F32, BF16, F16, I32, I8 = range(5)   # mi_dtype
 
 P = ctypes.c_void_p
 I = ctypes.c_int
@@ -72,6 +72,12 @@ SIGNATURES = {
     "mi_pack_w4": [P, P, I, P, P, P, P, I, I, I, P],
     "mi_w4_matvec": [P, I64, I, P, P, I, P, P, P, I64, I, I, I, I, P],
     "mi_sample_tokens": [P, I, I64, D, P, P, F, P, I, P, F, P, F, P, P, I, I, P],
+    "mi_adapter_workspace_size": [I, I, I, P],
+    "mi_adapter_add": [P, I, I64, I64, P, P, P, I, P, P, P, P, I64, I64, P, I64, I64, I, I, I, I, I, I, I, P, SZ, P],
+    "mi_gated_scan_sizes": [I, I, I, P, P, P],
+    "mi_gated_scan": [P, I64, I64, P, I64, I64, P, I64, I64, P, F, P, I64, I64, P, P, P, P, I64, I64, P, I, I, I, I, P, SZ, P],
+    "mi_gated_scan_backward": [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, P, F, P, I64, I64, P, P, P, P, P, P, P, P,
+                               I, I, I, I, P, SZ, P],
     "mi_checkpoint_open": [ctypes.c_char_p, P],
     "mi_checkpoint_get_info": [P, P],
     "mi_checkpoint_upload": [P, P, ctypes.c_size_t, P, P, I, P],

@@ -472,13 +472,13 @@ def embed_argmax(keys, ids_out, emb, r, row_stats) -> None:
               row_stats.shape[0], _stream())
 
 
-# -------------------------------------------- float operators (forward only)
+# ------------------------------------------------------------ float operators
 # Rows may be strided views (a half of in_proj's rows, slices of x_proj's): only
 # the elements of a row must be adjacent.  Tensors have to be on the current device,
 # and outputs must not overlap inputs except where stated.  Inputs that require
 # gradients are refused while autograd records, and so are dual tensors and calls
-# inside a trace: these operators have no backward.  The tensors' checks, the outputs
-# and the call are csrc/float_calls.cpp's.
+# inside a trace: these operators have no backward, but for gated_scan.  The tensors'
+# checks, the outputs and the call are csrc/float_calls.cpp's.
 _FLOAT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _ACTIVATIONS = {None: 0, "none": 0, "silu": 1}
 
@@ -492,7 +492,8 @@ def _calls():
         raise ImportError("the module of the float operators' calls is not built; build the library where torch, a C++ "
                           "compiler and Python's headers are") from e
     entries = ("mi_add_rms_norm", "mi_causal_conv", "mi_selective_scan_workspace_size", "mi_selective_scan",
-               "mi_w4_matvec", "mi_sample_tokens", "mi_last_error_string")
+               "mi_w4_matvec", "mi_sample_tokens", "mi_adapter_workspace_size", "mi_adapter_add", "mi_gated_scan_sizes", "mi_gated_scan",
+               "mi_gated_scan_backward", "mi_last_error_string")
     _float_calls.init(_lib.MIError, *(ctypes.cast(getattr(lib, e), ctypes.c_void_p).value for e in entries))
     return _float_calls
 
@@ -602,3 +603,70 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, sca
     order.  The four parameters are numbers or tensors [B] (float32; top_k int32).  NaN and
     -inf are never drawn; a row with nothing else has id -1.  Forward only."""
     return _calls().sample_tokens(_here(), logits, u, temperature, top_k, top_p, min_p, scale, logprob, out)
+
+
+def adapter_add(y, x, a, b, ids, scales=None, x_scale=None, lens=None, out=None):
+    """Low-rank adapters beside a shared projection, each sequence with its own of a bank:
+    y + scales[id] * (x @ a[id]^T) @ b[id]^T with id = ids[sequence].  y [B, L, N] and x [B,
+    L, K] (or [B, N] and [B, K]: sequences of one token) of one float type, or x int8 rows
+    with x_scale float32 [B, L] (what ``add_rms_norm_quant`` returns); a [bank, rank, K], b
+    [bank, N, rank] of one float type, rank up to 128; ids int32 [B] (outside [0, bank): no
+    adapter), scales float32 [bank] (None: 1), lens int32 [B]: tokens of each sequence, the
+    rows past them are y's.  ``out`` may be y: rows without an adapter are not touched then.
+    Forward only."""
+    return _calls().adapter_add(_here(), y, x, a, b, ids, scales, x_scale, lens, out)
+
+
+class _GatedScanGrad(torch.autograd.Function):
+    """gated_scan's gradients, as a node whose own gradient is an error: a second derivative
+    that leaves this part out would be wrong without one."""
+
+    @staticmethod
+    def forward(ctx, dy, x, r, i, decay, z, rate, lens, saved, needs):
+        return _calls().gated_scan_backward(_here(), dy, x, r, i, decay, z, rate, lens, saved, needs)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("gated_scan is differentiable once")
+
+
+class _GatedScan(torch.autograd.Function):
+    """gated_scan while autograd records."""
+
+    @staticmethod
+    def forward(ctx, x, r, i, decay, z, h_in, rate, lens):
+        y, saved = _calls().gated_scan(_here(), x, r, i, decay, z, rate, h_in, None, lens, None, True)
+        ctx.save_for_backward(x, r, i, decay, z, lens, saved)
+        ctx.rate = rate
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, r, i, decay, z, lens, saved = ctx.saved_tensors
+        if dy.stride(-1) != 1 or dy.is_neg():
+            dy = dy.clone(memory_format=torch.contiguous_format)    # (contiguous() keeps an empty tensor's strides)
+        grads = _GatedScanGrad.apply(dy, x, r, i, decay, z, ctx.rate, lens, saved, ctx.needs_input_grad[:6])
+        return (*grads, None, None)
+
+
+def gated_scan(x, r, i, decay, z=None, rate: float = 8.0, h_in=None, h_out=None, lens=None, out=None):
+    """Gated linear recurrence: with s = sigmoid(r), a = exp(-rate * softplus(decay) * s),
+    h = a * h + sqrt(1 - a^2) * sigmoid(i) * x,  y = h (* silu(z)).
+    x, r, i, z [B, L, D] of one float type; decay float32 [D]; h_in / h_out float32 [B, D]
+    (None: zeros; may be the same tensor); L = 1 is a decode step.  lens int32 [B]: tokens of
+    each sequence (h_out: the state after them; rows of the output past them are zero).
+
+    Differentiable, once, in x, r, i, decay, z and h_in; while autograd records one of them,
+    out and h_out cannot be given.  In a graph's capture no other live graph may hold such a
+    leaf from another stream."""
+    if torch.is_grad_enabled():
+        leaves = [(n, t) for n, t in (("x", x), ("r", r), ("i", i), ("decay", decay), ("z", z), ("h_in", h_in))
+                  if isinstance(t, torch.Tensor) and t.requires_grad]
+        if leaves:
+            if out is not None or h_out is not None:
+                raise ValueError("out and h_out cannot be given while autograd records the inputs")
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                for n, t in leaves:
+                    _calls().check_accumulator(_here(), n, t)
+            return _GatedScan.apply(x, r, i, decay, z, h_in, rate, lens)
+    return _calls().gated_scan(_here(), x, r, i, decay, z, rate, h_in, h_out, lens, out, False)
