@@ -11,55 +11,72 @@
 //   dx = g m q,  di = g m q x (1 - q),  dz = dy h silu'(z),  dh[-1] = a[0] g[0]
 //   p = n dn = g (q x a^2 n / m - n a h[t-1]),  dr = p (1 - s)
 //   ddecay = sigmoid(decay) / softplus(decay) * sum over b, t of p
+#include <algorithm>
+#include <type_traits>
+
 #include "float_ops.hpp"
 
 namespace mi {
 
-constexpr int kWaves = 8;                     // of a block with a whole chunk
-constexpr int kSteps = 16;                    // of a wave
-constexpr int kGatedChunk = kWaves * kSteps;  // steps of a block, and between the saved states
-constexpr int kJoin = 8;                      // chunks between the states that are passed on as such
+// Steps of a wave and waves of a block with a whole chunk.  Forwards 16 x 16: 8 x 2048 x 1536 in
+// bf16 68.6 us, 1 x 16384 x 1536 in float32 86.6; 8 waves 69.7 and 88.3, 4 waves 93 and 111, waves
+// of 8 steps with two channels a lane 78 and 101.  Backwards 4 waves of 16, since a wave there
+// takes 150 registers and a block of 8 leaves no room for a second one: 133 us against 166.
+constexpr int kSteps = 16, kWaves = 16;
+constexpr int kStepsBack = 16, kWavesBack = 4;
+constexpr int kChunk = kSteps * kWaves, kChunkBack = kStepsBack * kWavesBack;
+static_assert(kChunkBack % kSteps == 0, "a wave of the forward pass saves the state in front of it");
 
 struct GatedRows {
     void *p;
     int64_t ld, bs;
     template <class T>
-    __device__ __forceinline__ T *row(int64_t b, int64_t t) const { return static_cast<T *>(p) + b * bs + t * ld; }
+    __device__ __forceinline__ T *row(int64_t b, int64_t t) const {
+        return static_cast<T *>(p) + (b * bs + t * ld);
+    }
 };
 
 struct GatedArgs {
     GatedRows x, r, i, z, y;             // y: dy in a backward pass
     GatedRows dx, dr, di, dz;
     const float *decay, *h_in;
-    float *h_out, *saved;                // saved [batch, chunks, dim]: the state in front of each chunk
+    float *h_out, *saved;                // saved [batch, kept, dim]: the state in front of each chunk of the backward pass
     float *dh_in, *sums;                 // sums [batch, chunks, dim]: of p over a chunk's steps
     const int32_t *lens;
     uint32_t *ticket;                    // what the blocks pass on, 0 at first (GatedWords)
     uint64_t *words;
     float rate;
-    int batch, len, dim, chunks, groups;
+    int batch, len, dim, chunks, kept, groups;
 };
 
 __device__ __forceinline__ int gated_len(const GatedArgs &a, int b) {
     return a.lens ? min(max(a.lens[b], 0), a.len) : a.len;
 }
-// log(1 + exp(v)), with the relative precision of exp(v) for low v
-__device__ __forceinline__ float gated_softplus(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
+// log(1 + exp(v)) = max(v, 0) + log(w) + (e - (w - 1)) / w, e = exp(-|v|), w = 1 + e rounded: the
+// last term is what the rounding of w lost (w = 1 wherever it matters).  The exponent's
+// product with log2 e is kept in two parts, so a low v, whose value is e, has e's precision.
+__device__ __forceinline__ float gated_softplus(float v) {
+    const float u = -fabsf(v), p = u * 1.44269504f;
+    const float e = __builtin_amdgcn_exp2f(p);
+    const float lost = __builtin_fmaf(u, 1.44269504f, -p) + u * 1.925963033e-8f;      // log2 e's next bits
+    const float f = __builtin_fmaf(e, lost * 0.693147181f, e), w = 1.0f + f;
+    return fmaxf(v, 0.0f) + __builtin_fmaf(__builtin_amdgcn_logf(w), 0.693147181f, f - (w - 1.0f));
+}
 __device__ __forceinline__ float sigmoid(float v) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * v));
 }
-// 1 - exp(-2 n) for n >= 0 and a = exp(-n): by its series where the difference would cancel
+// 1 - exp(-2 n) for n >= 0 and a = exp(-n).  Where the difference would cancel, v times a
+// polynomial of (1 - exp(-v)) / v, v = 2 n: of the six coefficients that leave the least
+// relative error on [0, 0.5], 0.12 * 2^-24.
 __device__ __forceinline__ float one_minus_square(float n, float a) {
     const float v = 2.0f * n;
-    // v - v^2/2 + v^3/6 - ...: the term after the last is below 2^-24 of the sum at v = 0.5
-    float s = __builtin_fmaf(v, -1.0f / 40320.0f, 1.0f / 5040.0f);
-    s = __builtin_fmaf(v, -s, 1.0f / 720.0f);
-    s = __builtin_fmaf(v, -s, 1.0f / 120.0f);
-    s = __builtin_fmaf(v, -s, 1.0f / 24.0f);
-    s = __builtin_fmaf(v, -s, 1.0f / 6.0f);
-    s = __builtin_fmaf(v, -s, 0.5f);
-    s = __builtin_fmaf(v, -s, 1.0f);
-    return v < 0.5f ? v * s : __builtin_fmaf(-a, a, 1.0f);
+    float s = __builtin_fmaf(v, -0.0011216348502784967f, 0.008187386207282543f);
+    s = __builtin_fmaf(v, s, -0.041629090905189514f);
+    s = __builtin_fmaf(v, s, 0.16666224598884583f);
+    s = __builtin_fmaf(v, s, -0.4999998211860657f);
+    s = __builtin_fmaf(v, s, 1.0f) * v;
+    asm("" : "+v"(s));      // (selected, not branched over)
+    return v < 0.5f ? s : __builtin_fmaf(-a, a, 1.0f);
 }
 
 // One step's decay and input.
@@ -76,12 +93,12 @@ struct GatedStep {
 };
 
 // ---------------------------------------------------------------- chunks
-// A block has a chunk of a sequence's steps (16 a wave) and 64 C channels, C in a lane
-// (4 bytes of a row).  A wave keeps its rows in registers, sums its steps up as one step
+// A block has a chunk of a sequence's steps (16 a wave) and 64 C channels, C in a lane.  A
+// wave keeps its rows in registers, sums its steps up as one step
 // h -> A h + H, and starts from the state in front of it, which comes from the waves
 // before it through LDS, and from the chunks before through memory: every block passes
 // its chunk's (A, H) on as soon as it has them, and every kJoin-th chunk the state behind
-// it.  A block reads at most the last such state and kJoin - 1 sums, so the rows are read
+// it.  A block reads at most the last such state and JOIN - 1 sums, so the rows are read
 // once, and only every kJoin-th chunk waits for a state; which values are joined in which
 // order depends on the chunk alone, not on who was first.
 //
@@ -96,13 +113,14 @@ struct GatedWords {
 
     __device__ __forceinline__ explicit GatedWords(const GatedArgs &a)
         : p(a.words), seq((int64_t)a.dim * 2), dim(a.dim), batch(a.batch) {}
-    // the sums of chunk k of the order, and the state behind it for every last one of kJoin
+    // the sums of chunk k of the order, and the state behind it for every last one of JOIN
     __device__ __forceinline__ uint64_t *sums(int b, int k) const { return p + ((int64_t)k * batch + b) * seq; }
+    template <int JOIN>
     __device__ __forceinline__ uint64_t *state(int b, int k, int chunks) const {
-        return p + (int64_t)chunks * batch * seq + ((int64_t)(k / kJoin) * batch + b) * dim;
+        return p + (int64_t)chunks * batch * seq + ((int64_t)(k / JOIN) * batch + b) * dim;
     }
-    static size_t count(int64_t batch, int64_t dim, int64_t chunks) {
-        return (size_t)(batch * dim * (2 * chunks + chunks / kJoin));
+    static size_t count(int64_t batch, int64_t dim, int64_t chunks, int join) {
+        return (size_t)(batch * dim * (2 * chunks + chunks / join));
     }
 };
 __device__ __forceinline__ void pass_on(uint64_t *p, float v) {
@@ -122,60 +140,82 @@ __global__ __launch_bounds__(256) void gated_clear_kernel(uint64_t *p, int64_t n
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
 
-// What a block works on.
-struct GatedBlock {
-    int chunk, b, group;
-};
-template <bool MANY>
-__device__ __forceinline__ GatedBlock gated_block(const GatedArgs &a, uint32_t *lds) {
-    uint32_t at = blockIdx.x;
-    if constexpr (MANY) {
-        if (threadIdx.x == 0) *lds = atomicAdd(a.ticket, 1u);
-        __syncthreads();
-        at = (uint32_t)__builtin_amdgcn_readfirstlane((int)*lds);
-    }
-    const uint32_t per = (uint32_t)a.groups * (uint32_t)a.batch, rest = at % per;
-    return {(int)(at / per), (int)(rest / (uint32_t)a.groups), (int)(rest % (uint32_t)a.groups)};
-}
+// What a block works on: a chunk of a sequence and a group of channels.
+struct GatedTile {
+    int b, chunk, group, len, start;
+    bool full;      // every lane has its channels, and the sequence fills the chunk
 
-// C channels of a row from the lane's first one on.  FULL: every lane of the wave has them.
-template <int C, bool FULL, class T>
-__device__ __forceinline__ Packed<T, C> load_channels(const T *row, int c, int dim) {
-    if constexpr (FULL) return load_packed<C>(row + c);
-    Packed<T, C> v;
-#pragma unroll
-    for (int j = 0; j < C; ++j) v.v[j] = c + j < dim ? row[c + j] : T(0);
-    return v;
-}
-template <int C, bool FULL, class T>
-__device__ __forceinline__ void store_channels(T *row, int c, int dim, const Packed<T, C> &v) {
-    if constexpr (FULL)
-        store_packed<C>(row + c, v);
-    else {
-#pragma unroll
-        for (int j = 0; j < C; ++j)
-            if (c + j < dim) row[c + j] = v.v[j];
+    // BACKWARDS: the last chunk first
+    template <int C, int CHUNK, bool BACKWARDS, bool MANY, class Lds>
+    static __device__ __forceinline__ GatedTile take(const GatedArgs &a, Lds &s) {
+        uint32_t at = blockIdx.x;
+        if constexpr (MANY) {
+            if (threadIdx.x == 0) s.ticket = atomicAdd(a.ticket, 1u);
+            __syncthreads();
+            at = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.ticket);
+        }
+        const uint32_t per = (uint32_t)a.groups * (uint32_t)a.batch, rest = at % per;
+        GatedTile t;
+        t.chunk = BACKWARDS ? a.chunks - 1 - (int)(at / per) : (int)(at / per);
+        t.b = (int)(rest / (uint32_t)a.groups);
+        t.group = (int)(rest % (uint32_t)a.groups);
+        t.len = gated_len(a, t.b);
+        t.start = t.chunk * CHUNK;
+        t.full = (t.group + 1) * 64 * C <= a.dim && t.start + CHUNK <= t.len;
+        return t;
     }
-}
+};
+
+// Rows of a tensor from row (b, t) on, and C channels of each from the lane's first one on.
+// The row's address is the wave's, the channel's offset the lane's, which keeps a row's
+// access to one instruction.  FULL: every lane of the wave has its channels.
+template <class T>
+struct Cursor {
+    T *p;
+    int64_t step;
+    __device__ __forceinline__ Cursor(const GatedRows &r, int b, int t) : p(r.row<T>(b, t)), step(r.ld) {}
+    __device__ __forceinline__ void next(bool more = true) { p += more ? step : 0; }
+    __device__ __forceinline__ void back() { p -= step; }
+
+    template <int C, bool FULL>
+    __device__ __forceinline__ Packed<std::remove_const_t<T>, C> load(uint32_t c, int dim) const {
+        if constexpr (FULL) return load_packed<C>(p + c);
+        Packed<std::remove_const_t<T>, C> v;
+#pragma unroll
+        for (int j = 0; j < C; ++j) v.v[j] = (int)c + j < dim ? p[c + j] : T(0);
+        return v;
+    }
+    template <int C, bool FULL>
+    __device__ __forceinline__ void store(uint32_t c, int dim, const Packed<T, C> &v) const {
+        if constexpr (FULL)
+            store_packed<C>(p + c, v);
+        else {
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+                if ((int)c + j < dim) p[c + j] = v.v[j];
+        }
+    }
+};
 
 // The sums of the block's waves, and of the chunks in front of it.
 template <int C, int WAVES, bool MANY>
 struct GatedLds {
-    static constexpr int kBefore = MANY ? kJoin : 1;
+    static constexpr int kBefore = MANY ? WAVES : 1;
     float a[WAVES][64 * C], h[WAVES][64 * C], first[64 * C];
     float before_a[kBefore][64 * C], before_h[kBefore][64 * C];
+    uint32_t ticket;
 };
 template <int C>
 struct GatedLds<C, 1, false> {};
 
 // The state in front of chunk `at` > 0 of the order, from what the chunks before passed on;
 // this block's (A, H) are passed on first.  Chunk 0 passes the state behind it on, from
-// `first`, which is its own.  Every wave; LDS holds the waves' sums.  `behind`: whether
+// `first`, which is its s.  Every wave; LDS holds the waves' sums.  `behind`: whether
 // chunks follow.  BACKWARDS: the waves' order.
 template <int C, int WAVES, bool BACKWARDS>
 __device__ __forceinline__ void join_chunks(const GatedArgs &a, GatedLds<C, WAVES, true> &s, int b, int at, bool behind, int c,
                                             const float *first, float *carry) {
-    static_assert(WAVES >= kJoin, "a wave for each chunk that is read");
+    constexpr int JOIN = WAVES;      // a wave for each chunk that is read, and one for the state
     const int lane = threadIdx.x & 63, wave = wave_id();
     const GatedWords words(a);
     float A[C], H[C];
@@ -204,85 +244,127 @@ __device__ __forceinline__ void join_chunks(const GatedArgs &a, GatedLds<C, WAVE
             }
     }
     if (at == 0) return;
-    const int base = at / kJoin * kJoin;
-    // wave w < kJoin - 1 reads the sums of chunk base + w, wave kJoin - 1 the state in front of base
-    if (wave < kJoin - 1 ? base + wave < at : wave == kJoin - 1 && base > 0) {
-        const uint64_t *p = wave < kJoin - 1 ? words.sums(b, base + wave) : words.state(b, base - 1, a.chunks);
+    const int base = at / JOIN * JOIN;
+    // wave w < JOIN - 1 reads the sums of chunk base + w, wave JOIN - 1 the state in front of base
+    if (wave < JOIN - 1 ? base + wave < at : wave == JOIN - 1 && base > 0) {
+        const uint64_t *p = wave < JOIN - 1 ? words.sums(b, base + wave) : words.template state<JOIN>(b, base - 1, a.chunks);
 #pragma unroll
         for (int j = 0; j < C; ++j)
             if (c + j < a.dim) {
                 s.before_h[wave][lane * C + j] = wait_for(p + c + j);
-                if (wave < kJoin - 1 && base + wave > 0) s.before_a[wave][lane * C + j] = wait_for(p + a.dim + c + j);
+                if (wave < JOIN - 1 && base + wave > 0) s.before_a[wave][lane * C + j] = wait_for(p + a.dim + c + j);
             }
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-        float h = base > 0 ? s.before_h[kJoin - 1][lane * C + j] : s.before_h[0][lane * C + j];
+        float h = base > 0 ? s.before_h[JOIN - 1][lane * C + j] : s.before_h[0][lane * C + j];
         for (int w = base > 0 ? 0 : 1; base + w < at; ++w)
             h = __builtin_fmaf(s.before_a[w][lane * C + j], h, s.before_h[w][lane * C + j]);
         carry[j] = h;
     }
-    if (wave == 0 && at % kJoin == kJoin - 1 && behind) {
-        uint64_t *p = words.state(b, at, a.chunks);
+    if (wave == 0 && at % JOIN == JOIN - 1 && behind) {
+        uint64_t *p = words.template state<JOIN>(b, at, a.chunks);
 #pragma unroll
         for (int j = 0; j < C; ++j)
             if (c + j < a.dim) pass_on(p + c + j, __builtin_fmaf(A[j], carry[j], H[j]));
     }
 }
 
-template <class T, int C, int STEPS, int WAVES, bool MANY, bool FULL>
-__device__ __forceinline__ void gated_forward(const GatedArgs &a, GatedLds<C, WAVES, MANY> &s, const GatedBlock &at) {
-    const int lane = threadIdx.x & 63, wave = wave_id(), b = at.b;
-    const int c = (at.group * 64 + lane) * C, len = gated_len(a, b);
-    const int start = at.chunk * STEPS * WAVES, t0 = start + wave * STEPS;
-    Packed<T, C> zero;
-#pragma unroll
-    for (int j = 0; j < C; ++j) zero.v[j] = T(0);
-    if (start >= len && at.chunk > 0) {      // past the sequence: zeros
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t)
-            if (t0 + t < a.len) store_channels<C, FULL>(a.y.row<T>(b, t0 + t), c, a.dim, zero);
-        return;
-    }
-    float av[STEPS][C], bv[STEPS][C], A[C], H[C];
-    Packed<T, C> z[STEPS];
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-        A[j] = 1.0f;
-        H[j] = 0.0f;
-    }
-    if (t0 < len) {
-        Packed<T, C> x[STEPS], r[STEPS], i[STEPS];
+// A wave's rows in registers.  FULL: the tile is.  (Past the sequence the last row again.)
+template <class T, int C, int STEPS>
+struct GatedInputs {
+    Packed<T, C> x[STEPS], r[STEPS], i[STEPS];
+
+    template <bool FULL>
+    __device__ __forceinline__ void load(const GatedArgs &a, const GatedTile &at, int t0, uint32_t c) {
+        if (!FULL && t0 >= at.len) return;
+        Cursor<const T> xp(a.x, at.b, t0), rp(a.r, at.b, t0), ip(a.i, at.b, t0);
 #pragma unroll
         for (int t = 0; t < STEPS; ++t) {
-            const int row = min(t0 + t, len - 1);
-            r[t] = load_channels<C, FULL>(a.r.row<const T>(b, row), c, a.dim);
-            i[t] = load_channels<C, FULL>(a.i.row<const T>(b, row), c, a.dim);
-            x[t] = load_channels<C, FULL>(a.x.row<const T>(b, row), c, a.dim);
-            if (a.z.p) z[t] = load_channels<C, FULL>(a.z.row<const T>(b, row), c, a.dim);
+            r[t] = rp.template load<C, FULL>(c, a.dim);
+            i[t] = ip.template load<C, FULL>(c, a.dim);
+            x[t] = xp.template load<C, FULL>(c, a.dim);
+            const bool more = FULL || t0 + t + 1 < at.len;
+            rp.next(more), ip.next(more), xp.next(more);
         }
-        float k[C];
+    }
+    template <bool FULL>
+    static __device__ __forceinline__ void load_one(Packed<T, C> *to, const GatedArgs &a, const GatedRows &rows, const GatedTile &at,
+                                                    int t0, uint32_t c) {
+        if (!FULL && t0 >= at.len) return;
+        Cursor<const T> p(rows, at.b, t0);
 #pragma unroll
-        for (int j = 0; j < C; ++j) k[j] = FULL || c + j < a.dim ? a.rate * gated_softplus(a.decay[c + j]) : 0.0f;
+        for (int t = 0; t < STEPS; ++t, p.next(FULL || t0 + t < at.len)) to[t] = p.template load<C, FULL>(c, a.dim);
+    }
+    // Each step's decay and input, and the wave's steps as one: h -> A h + H.
+    template <bool FULL>
+    __device__ __forceinline__ void steps(const GatedArgs &a, const GatedTile &at, int t0, const float *k, float (*av)[C], float (*bv)[C],
+                                          float *A, float *H, float (*m2)[C] = nullptr) const {
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            A[j] = 1.0f;
+            H[j] = 0.0f;
+        }
+        if (!FULL && t0 >= at.len) return;
 #pragma unroll
         for (int t = 0; t < STEPS; ++t) {
+            const bool on = FULL || t0 + t < at.len;
 #pragma unroll
             for (int j = 0; j < C; ++j) {
                 const GatedStep g(k[j], (float)x[t].v[j], (float)r[t].v[j], (float)i[t].v[j]);
-                av[t][j] = t0 + t < len ? g.a : 1.0f;
-                bv[t][j] = t0 + t < len ? g.b : 0.0f;
+                av[t][j] = on ? g.a : 1.0f;
+                bv[t][j] = on ? g.b : 0.0f;
+                if (m2) m2[t][j] = g.m2;
                 H[j] = __builtin_fmaf(av[t][j], H[j], bv[t][j]);
                 A[j] *= av[t][j];
             }
         }
     }
+};
+
+template <int C>
+__device__ __forceinline__ uint32_t first_channel(const GatedTile &at) {
+    return (uint32_t)(at.group * 64 + (int)(threadIdx.x & 63)) * C;
+}
+template <int C, bool FULL>
+__device__ __forceinline__ void decays(const GatedArgs &a, uint32_t c, float *k) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) k[j] = FULL || (int)c + j < a.dim ? a.rate * gated_softplus(a.decay[c + j]) : 0.0f;
+}
+
+template <class T, int C, int STEPS, int WAVES, bool MANY>
+__global__ __launch_bounds__(WAVES * 64) void gated_scan_kernel(GatedArgs a) {
+    using Inputs = GatedInputs<T, C, STEPS>;
+    constexpr int CHUNK = STEPS * WAVES;
+    __shared__ GatedLds<C, WAVES, MANY> s;
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const GatedTile at = GatedTile::take<C, CHUNK, false, MANY>(a, s);
+    Inputs in;
+    const int b = at.b, t0 = at.start + wave * STEPS;
+    const uint32_t c = first_channel<C>(at);
+    const auto has = [&](int j) { return (int)c + j < a.dim; };
+    // (chunks past the sequence pass nothing on, and nothing reads them)
+    const bool work = at.start < at.len || at.chunk == 0;
+    float av[STEPS][C], bv[STEPS][C], A[C], H[C], h[C], k[C];
+    Packed<T, C> z[STEPS];
+    if (at.full) {
+        in.template load<true>(a, at, t0, c);
+        decays<C, true>(a, c, k);
+        in.template steps<true>(a, at, t0, k, av, bv, A, H);
+        // (they arrive while the block waits for the state in front of it)
+        if (a.z.p) Inputs::template load_one<true>(z, a, a.z, at, t0, c);
+    } else {
+        in.template load<false>(a, at, t0, c);
+        decays<C, false>(a, c, k);
+        in.template steps<false>(a, at, t0, k, av, bv, A, H);
+        if (a.z.p) Inputs::template load_one<false>(z, a, a.z, at, t0, c);
+    }
     const int64_t state = (int64_t)b * a.dim + c;
-    float h[C];
     // (one wave reads h_in, so that it has been read before a later chunk, or wave, writes
     // h_out in its place)
 #pragma unroll
-    for (int j = 0; j < C; ++j) h[j] = a.h_in && wave == 0 && at.chunk == 0 && (FULL || c + j < a.dim) ? a.h_in[state + j] : 0.0f;
+    for (int j = 0; j < C; ++j) h[j] = a.h_in && wave == 0 && at.chunk == 0 && has(j) ? a.h_in[state + j] : 0.0f;
     if constexpr (WAVES > 1) {
 #pragma unroll
         for (int j = 0; j < C; ++j) {
@@ -294,124 +376,95 @@ __device__ __forceinline__ void gated_forward(const GatedArgs &a, GatedLds<C, WA
         float first[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) h[j] = first[j] = s.first[lane * C + j];
-        if constexpr (MANY) join_chunks<C, WAVES, false>(a, s, b, at.chunk, len - start > STEPS * WAVES, c, first, h);
-    }
-    if (a.saved && wave == 0) {
-        float *p = a.saved + ((int64_t)b * a.chunks + at.chunk) * a.dim;
-#pragma unroll
-        for (int j = 0; j < C; ++j)
-            if (FULL || c + j < a.dim) p[c + j] = h[j];
+        if constexpr (MANY)
+            if (work) join_chunks<C, WAVES, false>(a, s, b, at.chunk, at.len - at.start > CHUNK, (int)c, first, h);
     }
     if constexpr (WAVES > 1)
         for (int w = 0; w < wave; ++w) {
 #pragma unroll
             for (int j = 0; j < C; ++j) h[j] = __builtin_fmaf(s.a[w][lane * C + j], h[j], s.h[w][lane * C + j]);
         }
-#pragma unroll
-    for (int t = 0; t < STEPS; ++t) {
-        if (t0 + t >= a.len) break;
-        Packed<T, C> y = zero;
-        if (t0 + t < len) {
-#pragma unroll
-            for (int j = 0; j < C; ++j) {
-                h[j] = __builtin_fmaf(av[t][j], h[j], bv[t][j]);
-                y.v[j] = (T)(a.z.p ? h[j] * silu((float)z[t].v[j]) : h[j]);
-            }
-        }
-        store_channels<C, FULL>(a.y.row<T>(b, t0 + t), c, a.dim, y);
-    }
-    if (a.h_out && wave == WAVES - 1 && start + STEPS * WAVES >= len) {
+    if (a.saved && t0 % kChunkBack == 0 && t0 < a.len) {
+        float *p = a.saved + ((int64_t)b * a.kept + t0 / kChunkBack) * a.dim;
 #pragma unroll
         for (int j = 0; j < C; ++j)
-            if (FULL || c + j < a.dim) a.h_out[state + j] = h[j];
+            if (has(j)) p[c + j] = h[j];
+    }
+    Cursor<T> to(a.y, b, t0);
+    const auto step = [&](int t) {
+        Packed<T, C> y;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            h[j] = __builtin_fmaf(av[t][j], h[j], bv[t][j]);
+            y.v[j] = (T)(a.z.p ? h[j] * silu((float)z[t].v[j]) : h[j]);
+        }
+        return y;
+    };
+    if (at.full) {
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t, to.next()) to.template store<C, true>(c, a.dim, step(t));
+    } else {
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t, to.next()) {
+            if (t0 + t >= a.len) break;
+            Packed<T, C> y;
+#pragma unroll
+            for (int j = 0; j < C; ++j) y.v[j] = T(0);
+            if (t0 + t < at.len) y = step(t);
+            to.template store<C, false>(c, a.dim, y);
+        }
+    }
+    if (a.h_out && wave == WAVES - 1 && work && at.start + CHUNK >= at.len) {
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+            if (has(j)) a.h_out[state + j] = h[j];
     }
 }
 
 template <class T, int C, int STEPS, int WAVES, bool MANY>
-__global__ __launch_bounds__(WAVES * 64) void gated_scan_kernel(GatedArgs a) {
+__global__ __launch_bounds__(WAVES * 64) void gated_scan_backward_kernel(GatedArgs a) {
+    using Inputs = GatedInputs<T, C, STEPS>;
+    constexpr int CHUNK = STEPS * WAVES;
     __shared__ GatedLds<C, WAVES, MANY> s;
-    __shared__ uint32_t ticket;
-    const GatedBlock at = gated_block<MANY>(a, &ticket);
-    if ((at.group + 1) * 64 * C <= a.dim)
-        gated_forward<T, C, STEPS, WAVES, MANY, true>(a, s, at);
-    else
-        gated_forward<T, C, STEPS, WAVES, MANY, false>(a, s, at);
-}
-
-template <class T, int C, int STEPS, int WAVES, bool MANY, bool FULL>
-__device__ __forceinline__ void gated_backward(const GatedArgs &a, GatedLds<C, WAVES, MANY> &s, GatedBlock at) {
-    const int lane = threadIdx.x & 63, wave = wave_id(), b = at.b;
-    at.chunk = a.chunks - 1 - at.chunk;      // from the last one
-    const int c = (at.group * 64 + lane) * C, len = gated_len(a, b);
-    const int start = at.chunk * STEPS * WAVES, t0 = start + wave * STEPS;
-    const int64_t kept = ((int64_t)b * a.chunks + at.chunk) * a.dim;
-    Packed<T, C> zero;
-#pragma unroll
-    for (int j = 0; j < C; ++j) zero.v[j] = T(0);
-    const auto store = [&](const GatedRows &to, int t, const Packed<T, C> &v) {
-        if (to.p) store_channels<C, FULL>(to.row<T>(b, t), c, a.dim, v);
-    };
-    if (start >= len) {      // past the sequence: zeros
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t)
-            if (t0 + t < a.len) {
-                store(a.dx, t0 + t, zero);
-                store(a.dr, t0 + t, zero);
-                store(a.di, t0 + t, zero);
-                store(a.dz, t0 + t, zero);
-            }
-#pragma unroll
-        for (int j = 0; j < C; ++j)
-            if (wave == 0 && (FULL || c + j < a.dim)) {
-                a.sums[kept + c + j] = 0.0f;
-                if (a.dh_in && at.chunk == 0) a.dh_in[(int64_t)b * a.dim + c + j] = 0.0f;
-            }
-        return;
-    }
-    const int last = (len - 1) / (STEPS * WAVES);
-    Packed<T, C> x[STEPS], r[STEPS], i[STEPS], z[STEPS], dy[STEPS];
-    float av[STEPS][C], hv[STEPS][C], A[C], H[C], G[C], k[C];
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const GatedTile at = GatedTile::take<C, CHUNK, true, MANY>(a, s);
+    const int b = at.b, t0 = at.start + wave * STEPS;
+    const uint32_t c = first_channel<C>(at);
+    const auto has = [&](int j) { return (int)c + j < a.dim; };
+    const bool work = at.start < at.len;
+    float av[STEPS][C], hv[STEPS][C], m2[STEPS][C], A[C], H[C], G[C], k[C], h[C], carry[C], sum[C];
+    Inputs in;
+    Packed<T, C> z[STEPS], dy[STEPS];
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-        A[j] = 1.0f;
-        H[j] = 0.0f;
         G[j] = 0.0f;
-        k[j] = FULL || c + j < a.dim ? a.rate * gated_softplus(a.decay[c + j]) : 0.0f;
+        carry[j] = 0.0f;
+        sum[j] = 0.0f;
+        h[j] = work && has(j) ? a.saved[((int64_t)b * a.chunks + at.chunk) * a.dim + c + j] : 0.0f;
     }
-    if (t0 < len) {
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t) {
-            const int row = min(t0 + t, len - 1);
-            r[t] = load_channels<C, FULL>(a.r.row<const T>(b, row), c, a.dim);
-            i[t] = load_channels<C, FULL>(a.i.row<const T>(b, row), c, a.dim);
-            x[t] = load_channels<C, FULL>(a.x.row<const T>(b, row), c, a.dim);
-            dy[t] = load_channels<C, FULL>(a.y.row<const T>(b, row), c, a.dim);
-            if (a.z.p) z[t] = load_channels<C, FULL>(a.z.row<const T>(b, row), c, a.dim);
-        }
-        // hv: the state behind each step, from 0 in front of the wave
-#pragma unroll
-        for (int t = 0; t < STEPS; ++t) {
-#pragma unroll
-            for (int j = 0; j < C; ++j) {
-                const GatedStep g(k[j], (float)x[t].v[j], (float)r[t].v[j], (float)i[t].v[j]);
-                av[t][j] = t0 + t < len ? g.a : 1.0f;
-                hv[t][j] = t0 + t < len ? g.b : 0.0f;       // (the input until the state in front is known)
-                H[j] = __builtin_fmaf(av[t][j], H[j], hv[t][j]);
-                A[j] *= av[t][j];
-            }
-        }
-        // G: a g of the wave's first step, from 0 behind it
+    // hv: what a step adds, first; G: a g of the wave's first step, from 0 behind the wave
+    const auto load = [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        in.template load<FULL>(a, at, t0, c);
+        Inputs::template load_one<FULL>(dy, a, a.y, at, t0, c);
+        if (a.z.p) Inputs::template load_one<FULL>(z, a, a.z, at, t0, c);
+        decays<C, FULL>(a, c, k);
+        in.template steps<FULL>(a, at, t0, k, av, hv, A, H, m2);
+        if (!FULL && t0 >= at.len) return;
 #pragma unroll
         for (int t = STEPS - 1; t >= 0; --t) {
 #pragma unroll
             for (int j = 0; j < C; ++j) {
                 float dh = (float)dy[t].v[j];
                 if (a.z.p) dh *= silu((float)z[t].v[j]);
-                G[j] = t0 + t < len ? av[t][j] * (dh + G[j]) : G[j];
+                G[j] = FULL || t0 + t < at.len ? av[t][j] * (dh + G[j]) : G[j];
             }
         }
-    }
-    float h[C], carry[C];
+    };
+    if (at.full)
+        load(std::true_type{});
+    else
+        load(std::false_type{});
     if constexpr (WAVES > 1) {
         // the states in front of the waves, then the gradients behind them
 #pragma unroll
@@ -420,13 +473,6 @@ __device__ __forceinline__ void gated_backward(const GatedArgs &a, GatedLds<C, W
             s.h[wave][lane * C + j] = H[j];
         }
         __syncthreads();
-    }
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-        carry[j] = 0.0f;
-        h[j] = FULL || c + j < a.dim ? a.saved[kept + c + j] : 0.0f;
-    }
-    if constexpr (WAVES > 1) {
         for (int w = 0; w < wave; ++w) {
 #pragma unroll
             for (int j = 0; j < C; ++j) h[j] = __builtin_fmaf(s.a[w][lane * C + j], h[j], s.h[w][lane * C + j]);
@@ -436,18 +482,17 @@ __device__ __forceinline__ void gated_backward(const GatedArgs &a, GatedLds<C, W
         for (int j = 0; j < C; ++j) s.h[wave][lane * C + j] = G[j];
         __syncthreads();
         const float none[C] = {};
-        if constexpr (MANY) join_chunks<C, WAVES, true>(a, s, b, last - at.chunk, at.chunk > 0, c, none, carry);
+        if constexpr (MANY)
+            if (work) join_chunks<C, WAVES, true>(a, s, b, (at.len - 1) / CHUNK - at.chunk, at.chunk > 0, (int)c, none, carry);
         for (int w = WAVES - 1; w > wave; --w) {
 #pragma unroll
             for (int j = 0; j < C; ++j) carry[j] = __builtin_fmaf(s.a[w][lane * C + j], carry[j], s.h[w][lane * C + j]);
         }
     }
-    float sum[C];
-#pragma unroll
-    for (int j = 0; j < C; ++j) sum[j] = 0.0f;
-    if (t0 < len) {
-        // hv: the state in front of each step
-        float behind[C];
+    const auto finish = [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        if (!FULL && t0 >= at.len) return;
+        // hv: the state in front of each step; h: behind the last
 #pragma unroll
         for (int t = 0; t < STEPS; ++t) {
 #pragma unroll
@@ -457,49 +502,49 @@ __device__ __forceinline__ void gated_backward(const GatedArgs &a, GatedLds<C, W
                 hv[t][j] = was;
             }
         }
+        Cursor<T> xo(a.dx, b, t0 + STEPS - 1), ro(a.dr, b, t0 + STEPS - 1), io(a.di, b, t0 + STEPS - 1), zo(a.dz, b, t0 + STEPS - 1);
 #pragma unroll
-        for (int j = 0; j < C; ++j) behind[j] = h[j];
+        for (int t = STEPS - 1; t >= 0; --t, xo.back(), ro.back(), io.back(), zo.back()) {
+            if (!FULL && t0 + t >= at.len) continue;
+            Packed<T, C> dx, dr, di, dz;
 #pragma unroll
-        for (int t = STEPS - 1; t >= 0; --t) {
-            if (t0 + t >= a.len) continue;
-            Packed<T, C> dx = zero, dr = zero, di = zero, dz = zero;
-            if (t0 + t < len) {
-#pragma unroll
-                for (int j = 0; j < C; ++j) {
-                    const float xf = (float)x[t].v[j];
-                    const GatedStep st(k[j], xf, (float)r[t].v[j], (float)i[t].v[j]);
-                    float dh = (float)dy[t].v[j];
-                    if (a.z.p) {
-                        const float zf = (float)z[t].v[j], sz = sigmoid(zf), act = silu(zf);
-                        dz.v[j] = (T)(dh * behind[j] * __builtin_fmaf(act, 1.0f - sz, sz));
-                        dh *= act;
-                    }
-                    const float g = dh + carry[j];
-                    // (the hardware root takes a subnormal for 0, its reciprocal is infinite there)
-                    const float inv = st.m2 >= 0x1p-126f ? __builtin_amdgcn_rsqf(st.m2) : 0.0f, m = st.m2 * inv;
-                    const float p = g * (st.q * xf * st.a * st.a * (st.n * inv) - st.n * st.a * hv[t][j]);
-                    dx.v[j] = (T)(g * m * st.q);
-                    di.v[j] = (T)(g * st.b * (1.0f - st.q));
-                    dr.v[j] = (T)(p * (1.0f - st.s));
-                    sum[j] += p;
-                    carry[j] = st.a * g;
-                    behind[j] = hv[t][j];
+            for (int j = 0; j < C; ++j) {
+                const float xf = (float)in.x[t].v[j], sr = sigmoid((float)in.r[t].v[j]), si = sigmoid((float)in.i[t].v[j]);
+                const float n = k[j] * sr, av_ = av[t][j];
+                float dh = (float)dy[t].v[j];
+                if (a.z.p) {
+                    const float zf = (float)z[t].v[j], sz = sigmoid(zf), act = zf * sz;
+                    dz.v[j] = (T)(dh * h[j] * __builtin_fmaf(act, 1.0f - sz, sz));
+                    dh *= act;
                 }
+                const float g = dh + carry[j];
+                // (the hardware root takes a subnormal for 0, its reciprocal is infinite there)
+                const float inv = m2[t][j] >= 0x1p-126f ? __builtin_amdgcn_rsqf(m2[t][j]) : 0.0f, gx = g * m2[t][j] * inv * si;
+                const float p = g * n * (si * xf * av_ * av_ * inv - av_ * hv[t][j]);
+                dx.v[j] = (T)gx;
+                di.v[j] = (T)(gx * xf * (1.0f - si));
+                dr.v[j] = (T)(p * (1.0f - sr));
+                sum[j] += p;
+                carry[j] = av_ * g;
+                h[j] = hv[t][j];
             }
-            store(a.dx, t0 + t, dx);
-            store(a.dr, t0 + t, dr);
-            store(a.di, t0 + t, di);
-            store(a.dz, t0 + t, dz);
+            if (a.dx.p) xo.template store<C, FULL>(c, a.dim, dx);
+            if (a.dr.p) ro.template store<C, FULL>(c, a.dim, dr);
+            if (a.di.p) io.template store<C, FULL>(c, a.dim, di);
+            if (a.dz.p) zo.template store<C, FULL>(c, a.dim, dz);
         }
-    } else {
+    };
+    if (at.full)
+        finish(std::true_type{});
+    else {
+        finish(std::false_type{});
+        // zeros past the sequence
+        Packed<T, C> zero;
 #pragma unroll
-        for (int t = 0; t < STEPS; ++t)
-            if (t0 + t < a.len) {
-                store(a.dx, t0 + t, zero);
-                store(a.dr, t0 + t, zero);
-                store(a.di, t0 + t, zero);
-                store(a.dz, t0 + t, zero);
-            }
+        for (int j = 0; j < C; ++j) zero.v[j] = T(0);
+        for (int t = max(at.len - t0, 0); t < STEPS && t0 + t < a.len; ++t)
+            for (const GatedRows &to : {a.dx, a.dr, a.di, a.dz})
+                if (to.p) Cursor<T>(to, b, t0 + t).template store<C, false>(c, a.dim, zero);
     }
     if constexpr (WAVES > 1) {
         __syncthreads();
@@ -507,27 +552,17 @@ __device__ __forceinline__ void gated_backward(const GatedArgs &a, GatedLds<C, W
         for (int j = 0; j < C; ++j) s.h[wave][lane * C + j] = sum[j];
         __syncthreads();
     }
-    if (wave != 0) return;
+    if (wave == 0) {
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-        if constexpr (WAVES > 1)
-            for (int w = 1; w < WAVES; ++w) sum[j] += s.h[w][lane * C + j];
-        if (FULL || c + j < a.dim) {
-            a.sums[kept + c + j] = sum[j];
-            if (a.dh_in && at.chunk == 0) a.dh_in[(int64_t)b * a.dim + c + j] = carry[j];
+        for (int j = 0; j < C; ++j) {
+            if constexpr (WAVES > 1)
+                for (int w = 1; w < WAVES; ++w) sum[j] += s.h[w][lane * C + j];
+            if (has(j)) {
+                a.sums[((int64_t)b * a.chunks + at.chunk) * a.dim + c + j] = sum[j];
+                if (a.dh_in && at.chunk == 0) a.dh_in[(int64_t)b * a.dim + c + j] = carry[j];
+            }
         }
     }
-}
-
-template <class T, int C, int STEPS, int WAVES, bool MANY>
-__global__ __launch_bounds__(WAVES * 64) void gated_scan_backward_kernel(GatedArgs a) {
-    __shared__ GatedLds<C, WAVES, MANY> s;
-    __shared__ uint32_t ticket;
-    const GatedBlock at = gated_block<MANY>(a, &ticket);
-    if ((at.group + 1) * 64 * C <= a.dim)
-        gated_backward<T, C, STEPS, WAVES, MANY, true>(a, s, at);
-    else
-        gated_backward<T, C, STEPS, WAVES, MANY, false>(a, s, at);
 }
 
 // ddecay from the sums of p over the chunks: 16 waves share them.
@@ -535,8 +570,17 @@ __global__ __launch_bounds__(1024) void gated_decay_kernel(const float *sums, co
     __shared__ float part[16][64];
     const int lane = threadIdx.x & 63, wave = wave_id(), c = blockIdx.x * 64 + lane;
     float s = 0.0f;
-    if (c < dim)
-        for (int64_t j = wave; j < rows; j += 16) s += sums[j * dim + c];
+    if (c < dim) {
+        int64_t j = wave;
+        for (; j + 7 * 16 < rows; j += 8 * 16) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = sums[(j + i * 16) * dim + c];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
+        }
+        for (; j < rows; j += 16) s += sums[j * dim + c];
+    }
     part[wave][lane] = s;
     __syncthreads();
     if (wave != 0 || c >= dim) return;
@@ -552,53 +596,67 @@ mi_status gated_dims(const char *fn, int batch, int len, int dim) {
     MI_REQUIRE(batch <= 65535, MI_ERR_BAD_DIM, "%s: batch=%d must be at most 65535", fn, batch);
     MI_REQUIRE(dim <= (1 << 24), MI_ERR_BAD_DIM, "%s: dim=%d must be at most 2^24", fn, dim);
     MI_REQUIRE(len <= (1 << 30), MI_ERR_BAD_DIM, "%s: len=%d must be at most 2^30", fn, len);
-    MI_REQUIRE(((int64_t)len + kGatedChunk - 1) / kGatedChunk * batch * (((int64_t)dim + 63) / 64) < (1 << 23), MI_ERR_BAD_DIM,
-               "%s: ceil(len / %d) * batch * ceil(dim / 64) must be below 2^23", fn, kGatedChunk);
+    MI_REQUIRE(((int64_t)len + 63) / 64 * batch * (((int64_t)dim + 63) / 64) < (1 << 23), MI_ERR_BAD_DIM,
+               "%s: ceil(len / 64) * batch * ceil(dim / 64) must be below 2^23", fn);
     return MI_OK;
 }
 
-inline int gated_chunks(int len) { return max(1, (len + kGatedChunk - 1) / kGatedChunk); }
+inline int gated_chunks(int len, int chunk) { return std::max(1, (len + chunk - 1) / chunk); }
 // bytes of the words and the ticket in front of them, none for one chunk
-inline size_t gated_word_bytes(int batch, int len, int dim) {
-    const int chunks = gated_chunks(len);
-    return chunks > 1 ? 16 + GatedWords::count(batch, dim, chunks) * sizeof(uint64_t) : 0;
+inline size_t gated_word_bytes(int batch, int len, int dim, int chunk, int join) {
+    const int chunks = gated_chunks(len, chunk);
+    return chunks > 1 ? 16 + GatedWords::count(batch, dim, chunks, join) * sizeof(uint64_t) : 0;
 }
 
 // Launches F<T, C, STEPS, WAVES, MANY>: one wave with as many steps as there are up to 16,
-// blocks of 8 waves beyond.
+// blocks of more waves beyond.
 template <template <class, int, int, int, bool> class F, class T>
 void launch_gated(GatedArgs a, void *workspace, hipStream_t st) {
-    constexpr int C = 4 / sizeof(T);
+    using K = F<T, 0, 0, 0, false>;
+    constexpr int C = 1;      // channels of a lane (two of 16 bits: the registers of twice the steps, 93 us)
+    a.chunks = gated_chunks(a.len, K::kAll);
+    a.kept = gated_chunks(a.len, kChunkBack);
     a.groups = (a.dim + 64 * C - 1) / (64 * C);
-    const auto launch = [&](auto kernel, int waves) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)a.groups * (unsigned)a.batch * (unsigned)a.chunks), dim3(waves * 64), 0, st, a);
-    };
+    const unsigned tiles = (unsigned)a.groups * (unsigned)a.batch * (unsigned)a.chunks;
+    const auto launch = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, dim3(tiles), dim3(waves * 64), 0, st, a); };
     if (a.chunks > 1) {
-        const int64_t n = 2 + (int64_t)GatedWords::count(a.batch, a.dim, a.chunks);
+        const int64_t n = 2 + (int64_t)GatedWords::count(a.batch, a.dim, a.chunks, K::kLast);
         a.ticket = static_cast<uint32_t *>(workspace);
         a.words = static_cast<uint64_t *>(workspace) + 2;
-        hipLaunchKernelGGL(gated_clear_kernel, dim3((unsigned)min((n + 1023) / 1024, (int64_t)2048)), dim3(256), 0, st,
+        // (std::min: the runtime's own on the host takes ints)
+        hipLaunchKernelGGL(gated_clear_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096)), dim3(256), 0, st,
                            static_cast<uint64_t *>(workspace), n);
-        launch(F<T, C, kSteps, kWaves, true>::kernel, kWaves);
+        launch(F<T, C, K::kEach, K::kLast, true>::kernel, K::kLast);
     } else if (a.len <= 1) {
         launch(F<T, C, 1, 1, false>::kernel, 1);
     } else if (a.len <= 4) {
         launch(F<T, C, 4, 1, false>::kernel, 1);
-    } else if (a.len <= kSteps) {
-        launch(F<T, C, kSteps, 1, false>::kernel, 1);
-    } else if (a.len <= 4 * kSteps) {
-        launch(F<T, C, kSteps, 4, false>::kernel, 4);
+    } else if (a.len <= 16) {
+        launch(F<T, C, 16, 1, false>::kernel, 1);
+    } else if (K::kLast > 4 && a.len <= 64) {
+        launch(F<T, C, 16, 4, false>::kernel, 4);
     } else {
-        launch(F<T, C, kSteps, kWaves, false>::kernel, kWaves);
+        launch(F<T, C, K::kEach, K::kLast, false>::kernel, K::kLast);
     }
 }
 template <class T, int C, int STEPS, int WAVES, bool MANY>
 struct Forward {
+    static constexpr int kEach = kSteps, kLast = kWaves, kAll = kChunk;
     static constexpr auto kernel = gated_scan_kernel<T, C, STEPS, WAVES, MANY>;
 };
 template <class T, int C, int STEPS, int WAVES, bool MANY>
 struct Backward {
+    static constexpr int kEach = kStepsBack, kLast = kWavesBack, kAll = kChunkBack;
     static constexpr auto kernel = gated_scan_backward_kernel<T, C, STEPS, WAVES, MANY>;
+};
+// (the sizes alone)
+template <class T>
+struct Forward<T, 0, 0, 0, false> {
+    static constexpr int kEach = kSteps, kLast = kWaves, kAll = kChunk;
+};
+template <class T>
+struct Backward<T, 0, 0, 0, false> {
+    static constexpr int kEach = kStepsBack, kLast = kWavesBack, kAll = kChunkBack;
 };
 
 }  // namespace mi
@@ -610,9 +668,10 @@ extern "C" mi_status mi_gated_scan_sizes(int batch, int len, int dim, size_t *fo
     clear_error();
     MI_REQUIRE(forward_bytes && backward_bytes && saved_bytes, MI_ERR_NULL_POINTER, "mi_gated_scan_sizes: the sizes are required");
     if (const mi_status st = gated_dims("mi_gated_scan_sizes", batch, len, dim)) return st;
-    *forward_bytes = gated_word_bytes(batch, len, dim);
-    *backward_bytes = gated_word_bytes(batch, len, dim) + (size_t)batch * gated_chunks(len) * dim * sizeof(float);
-    *saved_bytes = len ? (size_t)batch * gated_chunks(len) * dim * sizeof(float) : 0;
+    const size_t rows = (size_t)batch * gated_chunks(len, kChunkBack) * dim * sizeof(float);
+    *forward_bytes = gated_word_bytes(batch, len, dim, kChunk, kWaves);
+    *backward_bytes = gated_word_bytes(batch, len, dim, kChunkBack, kWavesBack) + rows;
+    *saved_bytes = len ? rows : 0;
     return MI_OK;
 }
 
@@ -634,8 +693,8 @@ extern "C" mi_status mi_gated_scan(const void *x, int64_t ldx, int64_t bsx, cons
     GatedArgs a{};
     a.x = in(x, ldx, bsx), a.r = in(r, ldr, bsr), a.i = in(i, ldi, bsi), a.z = in(z, ldz, bsz), a.y = {y, ldy, bsy};
     a.decay = decay, a.h_in = h_in, a.h_out = h_out, a.saved = len ? saved : nullptr, a.lens = lens, a.rate = rate;
-    a.batch = batch, a.len = len, a.dim = dim, a.chunks = gated_chunks(len);
-    const size_t need = gated_word_bytes(batch, len, dim);
+    a.batch = batch, a.len = len, a.dim = dim;
+    const size_t need = gated_word_bytes(batch, len, dim, kChunk, kWaves);
     MI_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), MI_ERR_BAD_ARG,
                "mi_gated_scan: the workspace has %zu bytes, %zu are needed", workspace_bytes, need);
     MI_REQUIRE(need == 0 || aligned(workspace, 16), MI_ERR_BAD_ALIGNMENT, "mi_gated_scan: the workspace must be 16-byte aligned");
@@ -671,12 +730,12 @@ extern "C" mi_status mi_gated_scan_backward(const void *dy, int64_t ldy, int64_t
     a.x = in(x, ldx, bsx), a.r = in(r, ldr, bsr), a.i = in(i, ldi, bsi), a.z = in(z, ldz, bsz), a.y = in(dy, ldy, bsy);
     a.dx = {dx, dim, bs}, a.dr = {dr, dim, bs}, a.di = {di, dim, bs}, a.dz = {dz, dim, bs};
     a.decay = decay, a.saved = const_cast<float *>(saved), a.dh_in = dh_in, a.lens = lens;
-    a.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + gated_word_bytes(batch, len, dim));
-    a.rate = rate, a.batch = batch, a.len = len, a.dim = dim, a.chunks = gated_chunks(len);
+    a.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + gated_word_bytes(batch, len, dim, kChunkBack, kWavesBack));
+    a.rate = rate, a.batch = batch, a.len = len, a.dim = dim;
     const hipStream_t st = as_stream(stream);
     if (batch > 0) with_type(type, [&](auto t) { launch_gated<Backward, decltype(t)>(a, workspace, st); });
     if (ddecay)
         hipLaunchKernelGGL(gated_decay_kernel, dim3((unsigned)((dim + 63) / 64)), dim3(1024), 0, st, a.sums, decay, ddecay,
-                           (int64_t)batch * a.chunks, dim);
+                           (int64_t)batch * gated_chunks(len, kChunkBack), dim);
     return check_launch("mi_gated_scan_backward");
 }

@@ -62,6 +62,7 @@ void call(mi_status st) {
 void gated() {
     Pool p;
     const int t = uni(0, 2), e = t ? 2 : 4, B = logu(1, 4), L = uni(0, 3) ? logu(1, 2600) : uni(0, 20), D = logu(1, L > 400 ? 140 : 400);
+    host_cus = uni(0, 1) ? 256 : 1;
     const View x = rows(p, B, L, D, e), r = rows(p, B, L, D, e), i = rows(p, B, L, D, e), z = rows(p, B, L, D, e), y = rows(p, B, L, D, e, true),
                dy = rows(p, B, L, D, e);
     size_t forward = 0, backward = 0, saved = 0;
@@ -108,7 +109,7 @@ void limits() {
     host_dry = 1;
     for (int t : {0, 1}) {
         const struct { int B, L, D; } sizes[] = {{65535, 1, 64}, {65535, 1, 64 * 127}, {65535, 2, 64 * 127}, {65535, 16, 64 * 127},
-                                                 {65535, 17, 64 * 127}, {65535, 128, 64 * 127}, {1, (1 << 30) - 128, 1}, {1, 1, 1 << 24}, {8, 1 << 20, 6400}};
+                                                 {65535, 17, 64 * 127}, {65535, 64, 64 * 127}, {1, (1 << 29) - 64, 1}, {1, 1, 1 << 24}, {8, 1 << 19, 6400}};
         for (const auto &s : sizes) {
             size_t w[3];
             call(mi_gated_scan_sizes(s.B, s.L, s.D, w, w + 1, w + 2));
