@@ -66,7 +66,8 @@ def check(s, got):
 
 SHAPES = [(1, 1, 1, 1, 1, 1), (8, 1, 64, 64, 8, 4), (5, 1, 100, 70, 5, 3), (3, 1, 2048, 768, 16, 9), (2, 3, 33, 17, 3, 2),
           (2, 16, 64, 128, 16, 2), (3, 17, 130, 65, 12, 5), (1, 64, 256, 192, 32, 1), (2, 65, 96, 200, 64, 3), (2, 31, 200, 1108, 7, 4),
-          (1, 130, 1000, 129, 128, 2), (1, 40, 72, 96, 33, 2), (4, 8, 4100, 48, 4, 4), (70, 1, 40, 300, 2, 128)]
+          (1, 130, 1000, 129, 128, 2), (1, 40, 72, 96, 33, 2), (4, 8, 4100, 48, 4, 4), (70, 1, 40, 300, 2, 128),
+          (2, 20, 72, 100, 80, 2), (3, 9, 31, 15, 17, 2), (1, 300, 520, 260, 24, 2)]
 
 
 @pytest.mark.parametrize("x_type", R.TYPES + [torch.int8])
