@@ -26,6 +26,7 @@ struct AdapterArgs {
     const int32_t *ids, *lens;
     void *t;                   // rows: float [rows, rank]; tiles: bf16 [3, rows, ranks]
     int batch, len, k, n, rank, ranks, bank;
+    int up_tokens;             // of a block of the second kernel, a multiple of 16 UT
 };
 
 // The adapter of a sequence, -1 for none; tokens of it.
@@ -166,14 +167,16 @@ __device__ __forceinline__ v4f product(const Parts<P> &a, const Parts<Q> &b, v4f
     return d;
 }
 
-// t of 16 MT tokens: 8 waves share the columns, 32 at a time, and join in LDS.  Operands as
+// t of 16 MT tokens: 8 waves share the columns, 64 at a time (a line
+// of 16-bit x; 32 where that takes too many registers), and join in LDS.  Operands as
 // the instruction takes them: lane 16 g + r has columns 8 g .. + 7 of row r, of A for the
 // result's rows (ranks), of x for its columns (tokens), so a lane gets four adjacent ranks of
 // a token.  Every load is 16 bytes (32 of float32) of one row.
 constexpr int kDownWaves = 8;
 template <class X, class W, int MT, int NT>
 __global__ __launch_bounds__(kDownWaves * 64) void adapter_down_tiles_kernel(AdapterArgs a) {
-    __shared__ v4f sums[kDownWaves][MT * NT][64];
+    constexpr int S = sizeof(X) == 4 || NT * sizeof(W) > 8 ? 1 : 2;
+    __shared__ v4f sums[kDownWaves / 2][MT * NT][64];
     const int b = blockIdx.y, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, wave = wave_id();
     const int id = adapter_of(a, b), tokens = tokens_of(a, b), t0 = (int)blockIdx.x * 16 * MT;
     if (id < 0 || t0 >= tokens) return;
@@ -188,36 +191,73 @@ __global__ __launch_bounds__(kDownWaves * 64) void adapter_down_tiles_kernel(Ada
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n) d[m][n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    const auto step = [&](int c, auto load) {
-        Packed<X, 8> xv[MT];
-        Packed<W, 8> wv[NT];
+    // a turn's operands: S times 32 columns
+    struct Turn {
+        Packed<X, 8> x[S][MT];
+        Packed<W, 8> w[S][NT];
+    } turn[2];
+    const auto load = [&](int c, Turn &to, auto with) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) xv[m] = load(x[m], c);
+        for (int s = 0; s < S; ++s) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) wv[n] = load(w[n], c);
-        Parts<parts_of<X>()> xp[MT];
+            for (int m = 0; m < MT; ++m) to.x[s][m] = with(x[m], c + 32 * s + 8 * g);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) xp[m] = parts(xv[m]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const auto wp = parts(wv[n]);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) d[m][n] = product(wp, xp[m], d[m][n]);
+            for (int n = 0; n < NT; ++n) to.w[s][n] = with(w[n], c + 32 * s + 8 * g);
         }
     };
-    int c = wave * 32;
-#pragma unroll 2
-    for (; c + 32 <= a.k; c += kDownWaves * 32) step(c + 8 * g, [](const auto *p, int at) { return load_packed<8>(p + at); });
-    if (c < a.k) step(c + 8 * g, [&](const auto *p, int at) { return load8(p, at, a.k); });
+    const auto whole = [](const auto *p, int at) { return load_packed<8>(p + at); };
+    const auto add = [&](const Turn &of) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+        for (int s = 0; s < S; ++s) {
+            Parts<parts_of<X>()> xp[MT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sums[wave][m * NT + n][lane] = d[m][n];
+            for (int m = 0; m < MT; ++m) xp[m] = parts(of.x[s][m]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const auto wp = parts(of.w[s][n]);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) d[m][n] = product(wp, xp[m], d[m][n]);
+            }
+        }
+    };
+    // whole turns, the next one's loads in flight over the products
+    constexpr int kStride = kDownWaves * 32 * S;
+    int c = wave * 32 * S, turns = (a.k - c) / (32 * S) > 0 ? ((a.k - c) / (32 * S) + kDownWaves - 1) / kDownWaves : 0;
+    if (turns > 0) load(c, turn[0], whole);
+    for (int i = 0; i < turns; i += 2) {
+        if (i + 1 < turns) load(c + kStride, turn[1], whole);
+        add(turn[0]);
+        if (i + 2 < turns) load(c + 2 * kStride, turn[0], whole);
+        if (i + 1 < turns) add(turn[1]);
+        c += 2 * kStride;
+    }
+    c = wave * 32 * S + turns * kStride;
+    if (c < a.k) {
+        load(c, turn[0], [&](const auto *p, int at) { return load8(p, at, a.k); });
+        add(turn[0]);
+    }
+    // the second half of the waves to the first, then those
+    constexpr int HALF = kDownWaves / 2;
+    const auto put = [&](int at) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sums[at][m * NT + n][lane] = d[m][n];
+    };
+    if (wave >= HALF) put(wave - HALF);
+    __syncthreads();
+    if (wave < HALF) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) d[m][n] += sums[wave][m * NT + n][lane];
+        put(wave);
+    }
     __syncthreads();
     for (int tile = wave; tile < MT * NT; tile += kDownWaves) {
         v4f s = sums[0][tile][lane];
 #pragma unroll
-        for (int v = 1; v < kDownWaves; ++v) s += sums[v][tile][lane];
+        for (int v = 1; v < HALF; ++v) s += sums[v][tile][lane];
         const int token = t0 + tile / NT * 16 + r, rank = tile % NT * 16 + 4 * g;
         if (token >= tokens) continue;
         const int64_t row = (int64_t)b * a.len + token;
@@ -247,20 +287,19 @@ __global__ __launch_bounds__(kDownWaves * 64) void adapter_down_tiles_kernel(Ada
     }
 }
 
-// out of kUpTokens tokens and 16 NT columns a wave, 4 waves side by side.  B's operands stay in
-// registers, a tile of 16 tokens after the other brings t's three parts and y.  A lane gets
+// out of up_tokens tokens and 16 NT columns a wave, 4 waves side by side.  B's operands stay in
+// registers, 16 UT tokens after the other bring t's three parts and y (a turn ahead).  A lane gets
 // four adjacent columns of a token from a tile of the result, so B's rows go to tiles such
 // that the lane's tiles (two of them for 16-bit y) are 16 adjacent bytes.
-constexpr int kUpTokens = 128;
-template <class Y, class W, int KS, int NT>
+template <class Y, class W, int KS, int NT, int UT>
 __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
     constexpr int PAIR = sizeof(Y) == 4 ? 1 : 2, V = 4 * PAIR;
     const int b = blockIdx.z, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int id = adapter_of(a, b), tokens = id < 0 ? 0 : tokens_of(a, b), t0 = (int)blockIdx.y * kUpTokens;
+    const int id = adapter_of(a, b), tokens = id < 0 ? 0 : tokens_of(a, b), t0 = (int)blockIdx.y * a.up_tokens;
     const int n0 = ((int)blockIdx.x * 4 + wave_id()) * 16 * NT;
     const bool in_place = a.out == a.y;
     if (n0 >= a.n || (in_place && t0 >= tokens)) return;
-    const int end = min(t0 + kUpTokens, in_place ? tokens : a.len);
+    const int end = min(t0 + a.up_tokens, in_place ? tokens : a.len);
     const bool whole = n0 + 16 * NT <= a.n;
     // the column of element i of this lane's vector h
     const auto column = [&](int h) { return n0 + h * 16 * PAIR + g * V; };
@@ -275,7 +314,7 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
             for (int s = 0; s < KS; ++s) w[n][s] = parts(load8(p, 32 * s + 8 * g, a.rank));
         }
     }
-    Packed<Y, V> y[2][NT / PAIR];
+    Packed<Y, V> y[2][UT][NT / PAIR];
     const auto load_y = [&](int t, Packed<Y, V> *to) {
         const Y *p = static_cast<const Y *>(a.y) + (b * a.bsy + min(t + r, a.len - 1) * a.ldy);
 #pragma unroll
@@ -324,13 +363,22 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
             }
         }
     };
-    load_y(t0, y[0]);
-    for (int t = t0; t < end; t += 32) {
-        if (t + 16 < end) load_y(t + 16, y[1]);
-        tile(t, y[0]);
-        if (t + 16 >= end) break;
-        if (t + 32 < end) load_y(t + 32, y[0]);
-        tile(t + 16, y[1]);
+    const auto load = [&](int t, auto &to) {
+#pragma unroll
+        for (int u = 0; u < UT; ++u)
+            if (t + 16 * u < end) load_y(t + 16 * u, to[u]);
+    };
+    const auto turn = [&](int t, const auto &yv) {
+#pragma unroll
+        for (int u = 0; u < UT; ++u)
+            if (t + 16 * u < end) tile(t + 16 * u, yv[u]);
+    };
+    load(t0, y[0]);
+    for (int t = t0; t < end; t += 32 * UT) {
+        load(t + 16 * UT, y[1]);
+        turn(t, y[0]);
+        load(t + 32 * UT, y[0]);
+        turn(t + 16 * UT, y[1]);
     }
 }
 
@@ -355,34 +403,51 @@ void launch_adapter_rows(const AdapterArgs &a, bool work, hipStream_t st) {
     hipLaunchKernelGGL((adapter_up_kernel<Y, W>), dim3(rows, (unsigned)((a.n + 255) / 256)), dim3(256), 0, st, a);
 }
 
-// Tiles of 32 tokens for up to 64 ranks (16 above: the sums of 8 waves would not fit).
+// The first kernel's tiles have 64 tokens (A is read once for them: 16384 x 4096 of rank 32 in
+// bf16 31 us, with 32 tokens 40, with 16 51; a row maximum of the same x 30) where that leaves a
+// block for every CU, else 16.
 template <class X, class Y, class W>
 void launch_adapter_tiles(const AdapterArgs &a, bool work, hipStream_t st) {
+    const bool many = (int64_t)((a.len + 63) / 64) * a.batch >= device_cus();
     const auto down = [&](auto kernel, int mt) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)((a.len + 16 * mt - 1) / (16 * mt)), (unsigned)a.batch), dim3(kDownWaves * 64), 0, st, a);
     };
-    const auto up = [&](auto kernel, int nt) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.n + 64 * nt - 1) / (64 * nt)), (unsigned)((a.len + kUpTokens - 1) / kUpTokens),
-                                        (unsigned)a.batch), dim3(256), 0, st, a);
+    const auto up = [&](auto kernel, int nt, int ut) {
+        AdapterArgs b = a;
+        const int64_t columns = (a.n + 64 * nt - 1) / (64 * nt);
+        // as many tokens a block as leave 1024 blocks, 64 at most while the grid has room (8 x 2048
+        // -> 2048 in bf16: 33.8 us, 128 tokens 35.5; 8 tiles of columns a wave 44)
+        b.up_tokens = a.len <= 64 * 65535 ? 64 : 128;
+        while (b.up_tokens > 16 * ut && columns * a.batch * ((a.len + b.up_tokens - 1) / b.up_tokens) < 1024) b.up_tokens /= 2;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)columns, (unsigned)((a.len + b.up_tokens - 1) / b.up_tokens), (unsigned)a.batch),
+                           dim3(256), 0, st, b);
     };
     if (work) {
+        const auto ranks = [&](auto nt) {
+            constexpr int NT = decltype(nt)::value, P = std::max(parts_of<X>(), parts_of<W>());
+            constexpr int MT = NT < 4 ? 4 : NT == 4 ? (P == 1 ? 4 : 2) : P == 1 ? 2 : 1;      // (registers)
+            if (many)
+                down(adapter_down_tiles_kernel<X, W, MT, NT>, MT);
+            else
+                down(adapter_down_tiles_kernel<X, W, 1, NT>, 1);
+        };
         if (a.rank <= 16)
-            down(adapter_down_tiles_kernel<X, W, 2, 1>, 2);
+            ranks(std::integral_constant<int, 1>{});
         else if (a.rank <= 32)
-            down(adapter_down_tiles_kernel<X, W, 2, 2>, 2);
+            ranks(std::integral_constant<int, 2>{});
         else if (a.rank <= 64)
-            down(adapter_down_tiles_kernel<X, W, 2, 4>, 2);
+            ranks(std::integral_constant<int, 4>{});
         else
-            down(adapter_down_tiles_kernel<X, W, 1, 8>, 1);
+            ranks(std::integral_constant<int, 8>{});
     }
     // B's parts in registers: 16 a tile of columns for 32 ranks and part
-    constexpr int P = parts_of<W>();
+    constexpr int P = parts_of<W>(), UT = sizeof(Y) == 4 ? 1 : 2;
     if (a.rank <= 32)
-        up(adapter_up_tiles_kernel<Y, W, 1, 4>, 4);
+        up(adapter_up_tiles_kernel<Y, W, 1, 4, UT>, 4, UT);
     else if (a.rank <= 64)
-        up(adapter_up_tiles_kernel<Y, W, 2, P < 3 ? 4 : 2>, P < 3 ? 4 : 2);
+        up(adapter_up_tiles_kernel<Y, W, 2, P < 3 ? 4 : 2, UT>, P < 3 ? 4 : 2, UT);
     else
-        up(adapter_up_tiles_kernel<Y, W, 4, P < 2 ? 4 : 2>, P < 2 ? 4 : 2);
+        up(adapter_up_tiles_kernel<Y, W, 4, P < 2 ? 4 : 2, 1>, P < 2 ? 4 : 2, 1);
 }
 
 }  // namespace mi
@@ -424,7 +489,7 @@ extern "C" mi_status mi_adapter_add(const void *x, int x_type, int64_t ldx, int6
     MI_REQUIRE(y && out && ids, MI_ERR_NULL_POINTER, "mi_adapter_add: y, out and ids are required");
     MI_REQUIRE(out != y || (ldo == ldy && bso == bsy), MI_ERR_BAD_ARG, "mi_adapter_add: in place, out has y's strides");
     const AdapterArgs args{x, y, out, ldx, bsx, ldy, bsy, ldo, bso, x_scale, a, b, scales, ids, lens,
-                           workspace, batch, len, k, n, k ? rank : 0, adapter_ranks(rank), bank};
+                           workspace, batch, len, k, n, k ? rank : 0, adapter_ranks(rank), bank, 0};
     const bool work = args.rank && bank;
     if (!work && out == y) return MI_OK;
     MI_REQUIRE(!work || (x && a && b), MI_ERR_NULL_POINTER, "mi_adapter_add: x, a and b are required");
