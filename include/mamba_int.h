@@ -624,7 +624,7 @@ mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const uint8_t *pack
  * logprob 0.  A NaN or -inf is never drawn; a row of nothing else has id -1 and
  * logprob -inf.  Where the largest logit is +inf, the tokens with +inf have e =
  * 1 and the others 0.  Sums are exact: a token's mass is e as a 64-bit
- * integer in units of 2^-(62 - ceil(log2 vocab)), at least 2^-52 (an e below
+ * integer in units of 2^-(62 - ceil(log2 vocab)), at least 2^-51 (an e below
  * half a unit is 0), so a row's token depends on nothing but the row.
  *   logits  rows of type MI_F32, MI_BF16, MI_F16 or MI_I32, ld elements from
  *           one to the next; scale in (0, 1e30];

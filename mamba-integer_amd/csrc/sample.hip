@@ -12,6 +12,8 @@
 // integer, so every sum is exact, in any order.  The kept tokens are a beginning of the
 // order, so one 64-bit number (the key of l above the token's complement) tells them
 // from the rest.
+#include <type_traits>
+
 #include "float_ops.hpp"
 
 namespace mi {
@@ -19,9 +21,10 @@ namespace mi {
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWaves = kSampleThreads / 64;
 constexpr int kSampleBins = 2048;
-constexpr int kSampleList = 1024;           // candidates whose ranks are counted pairwise
+constexpr int kSampleNear = 256;            // candidates whose ranks are counted pairwise
+constexpr int kSampleList = 2048;           // candidates of a small top_k, all in LDS
 constexpr int kSampleMaxVocab = 1 << 24;
-constexpr double kSampleRange = 40.0;       // e^-40 * 2^52 rounds to a mass of 0
+constexpr double kSampleRange = 40.0;       // e^-40 * 2^51 rounds to a mass of 0
 
 struct SampleArgs {
     const void *logits;
@@ -49,26 +52,63 @@ using Logit = std::conditional_t<std::is_same<T, int32_t>::value, int32_t, float
 
 // The key above the token's complement: larger is earlier in the order; never 0.
 __device__ __forceinline__ uint64_t order_of(uint32_t key, int token) { return (uint64_t)key << 32 | (uint32_t)~token; }
+__device__ __forceinline__ int token_of(uint64_t place) { return (int)~(uint32_t)place; }
+// The logit of a key.
+template <class L>
+__device__ __forceinline__ L value_of(uint32_t key) {
+    if constexpr (std::is_same<L, int32_t>::value)
+        return (int32_t)(key ^ 0x80000000u);
+    else
+        return __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
 
-struct SampleLds {
-    uint32_t count[kSampleBins];
-    uint64_t mass[kSampleBins];
-    uint64_t list[kSampleList], list_mass[kSampleList];
-    uint64_t wave_mass[kSampleWaves], threshold;
-    uint32_t wave_count[kSampleWaves], found, lo, hi;
-    uint64_t above_mass;
-    uint32_t above_count;
-    int bin, token;
+// 2^(j / 64).
+__constant__ const double kExpTable[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
 };
 
+struct SampleLds {
+    double table[64];
+    uint32_t count[kSampleBins];
+    uint64_t mass[kSampleBins];
+    uint64_t list[kSampleList];               // places of the candidates of a small top_k
+    uint64_t near[kSampleNear], near_mass[kSampleNear];
+    uint64_t wave_mass[kSampleWaves], lo, hi, above_mass, last;
+    uint32_t wave_count[kSampleWaves], above_count, found;
+    int bin;
+};
+
+// (of two 64-bit types that differ in name, min and max are those of 32 bits)
+__device__ __forceinline__ uint64_t less(uint64_t a, uint64_t b) { return a < b ? a : b; }
+__device__ __forceinline__ uint64_t more(uint64_t a, uint64_t b) { return a < b ? b : a; }
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
     return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)v, o);
 }
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int o) {
     return (uint64_t)(uint32_t)__shfl_up((int)(v >> 32), o) << 32 | (uint32_t)__shfl_up((int)(uint32_t)v, o);
 }
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
+__device__ __forceinline__ uint64_t block_sum(SampleLds &s, uint64_t v) {
     for (int o = 32; o > 0; o >>= 1) v += shfl_xor64(v, o);
+    if ((threadIdx.x & 63) == 0) s.wave_mass[wave_id()] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < kSampleWaves; ++w) v += s.wave_mass[w];
+    __syncthreads();
     return v;
 }
 
@@ -76,23 +116,86 @@ __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
 template <class T>
 struct SampleRow {
     const T *p;
-    double scale, top, inv_t, unit;
-    uint32_t top_key;
+    const double *table;
+    double top, factor, unit;      // the largest logit; scale / temperature; 2^bits
     int vocab;
 
-    // 0 for the largest logit (an infinite one too), below 0 for others, -inf or NaN far below
-    __device__ __forceinline__ double below(Logit<T> v) const {
-        return order_key(v) == top_key ? 0.0 : ((double)v * scale - top) * inv_t;
+    // l - max l over the temperature: 0 for the largest (an infinite one too), -inf or NaN far below
+    __device__ __forceinline__ double below(Logit<T> v) const { return (double)v == top ? 0.0 : ((double)v - top) * factor; }
+    // exp(d) of d in (-40, 0] to 2 of its last places, 0 below: 2^(n / 64) exp(r) with |r| < ln 2 / 128
+    __device__ __forceinline__ double e(double d) const {
+        const double n = __builtin_rint(d * 0x1.71547652b82fep+6);
+        const double r = __builtin_fma(n, -0x1.9ef35793c7673p-47, __builtin_fma(n, -0x1.62e42fefa2000p-7, d));
+        double q = __builtin_fma(r, 1.0 / 120.0, 1.0 / 24.0);
+        q = __builtin_fma(r, q, 1.0 / 6.0);
+        q = __builtin_fma(r, q, 0.5);
+        q = __builtin_fma(r * r, q, r);
+        const int k = d > -kSampleRange ? (int)n : 0;
+        const double t = table[k & 63];
+        return d > -kSampleRange ? __builtin_ldexp(__builtin_fma(t, q, t), k >> 6) : 0.0;
     }
-    __device__ __forceinline__ static double e(double d) { return d > -kSampleRange ? exp(d) : 0.0; }
-    __device__ __forceinline__ uint64_t mass(double e) const { return (uint64_t)__builtin_rint(e * unit); }
+    // e * 2^bits as an integer (bits <= 51): the mantissa of its sum with 2^52
+    __device__ __forceinline__ uint64_t mass(double e) const {
+        return __builtin_bit_cast(uint64_t, __builtin_fma(e, unit, 0x1p52)) - __builtin_bit_cast(uint64_t, 0x1p52);
+    }
     __device__ __forceinline__ static int bin(double d) {
         return d > -kSampleRange ? min((int)(d * (-kSampleBins / kSampleRange)), kSampleBins - 1) : kSampleBins - 1;
     }
 };
 
+// 16 bytes of a row from token i on, zeros from `end` on.
+template <class T, int N = 16 / sizeof(T)>
+__device__ __forceinline__ Packed<T, N> load_logits(const T *p, int i, int end) {
+    if (i + N <= end) return load_packed<N>(p + i);
+    Packed<T, N> v;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v.v[e] = i + e < end ? p[i + e] : T(0);
+    return v;
+}
+
+// Calls f(logit, token) for every token that may be drawn, by all threads, in no order.
+template <class T, class F>
+__device__ __forceinline__ void each_logit(const SampleRow<T> &r, F &&f) {
+    constexpr int N = 16 / sizeof(T), STEP = kSampleThreads * N;
+    int i = (int)threadIdx.x * N;
+    Packed<T, N> next;
+    if (i < r.vocab) next = load_logits(r.p, i, r.vocab);
+    for (; i < r.vocab; i += STEP) {
+        const Packed<T, N> now = next;
+        if (i + STEP < r.vocab) next = load_logits(r.p, i + STEP, r.vocab);
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (i + e < r.vocab && drawable((Logit<T>)now.v[e])) f((Logit<T>)now.v[e], i + e);
+    }
+}
+
+// Calls f(logits, first token, how many of them) over a wave's share of the row, in the order of
+// tokens, N adjacent ones a lane, with all lanes active, until f says true (the same for all).
+template <class T, class F>
+__device__ __forceinline__ void wave_share(const SampleRow<T> &r, int wave, F &&f) {
+    constexpr int N = 16 / sizeof(T), STEP = 64 * N;
+    const int share = (r.vocab + kSampleWaves * STEP - 1) / (kSampleWaves * STEP) * STEP;
+    const int end = min((wave + 1) * share, r.vocab), lane = (int)threadIdx.x & 63;
+    Packed<T, N> next;
+    int base = wave * share;
+    if (base < end) next = load_logits(r.p, base + lane * N, end);
+    for (; base < end; base += STEP) {
+        const Packed<T, N> now = next;
+        if (base + STEP < end) next = load_logits(r.p, base + STEP + lane * N, end);
+        const int i = base + lane * N;
+        if (f(now, i, min(max(end - i, 0), N))) break;
+    }
+}
+
+__device__ __forceinline__ void clear_bins(SampleLds &s) {
+    for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) {
+        s.count[i] = 0;
+        s.mass[i] = 0;
+    }
+}
+
 // The first of the bins, from 0 on, at which the counts reach `count` or the masses reach
-// `mass`, and what lies in the bins before it.  All threads; the bins hold them by then.
+// `mass`, and what lies in the bins before it; the last bin if none.  All threads.
 __device__ __forceinline__ void cut_bin(SampleLds &s, uint32_t count, uint64_t mass) {
     constexpr int PER = kSampleBins / kSampleThreads;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
@@ -141,241 +244,257 @@ __device__ __forceinline__ void cut_bin(SampleLds &s, uint32_t count, uint64_t m
     __syncthreads();
 }
 
-// Calls f(logit, token, on) over a wave's share of the row, in the order of tokens, 64 at a time,
-// with all lanes active (`on`: the lane has a token), until f says true (the same for all lanes).
-template <class T, class F>
-__device__ __forceinline__ void wave_share(const SampleRow<T> &r, int wave, F &&f) {
-    const int share = ((r.vocab + kSampleWaves - 1) / kSampleWaves + 63) / 64 * 64;
-    const int end = min((wave + 1) * share, r.vocab);
-    for (int base = wave * share; base < end; base += 64) {
-        const int i = base + (threadIdx.x & 63);
-        const Logit<T> v = i < end ? (Logit<T>)r.p[i] : Logit<T>(0);
-        if (f(v, i, i < end && drawable(v))) break;
-    }
-}
-
-// Of the tokens in bin s.bin (by `below`) whose place in the order is at least `from`:
-// keeps the first ones while fewer than `count` of them and less than `mass` lie before.
-// Returns the last kept one's place.  All threads; the bins count these tokens.
-template <class T>
-__device__ uint64_t cut_in_bin(const SampleRow<T> &r, SampleLds &s, uint64_t from, uint32_t count, uint64_t mass) {
-    const int tid = threadIdx.x, bin = s.bin;
-    uint32_t n = s.count[bin];
+// Of n candidates in the order of their places, larger first: the place of the last one that
+// has fewer than `count` and less than `mass` in front of it (there is one: neither is 0).
+// visit(f) calls f(place, d) for each candidate, by all threads, in any order; no two places
+// are alike.  Too many candidates are parted by place until few enough share a part.  All
+// threads.
+template <class T, class V>
+__device__ __forceinline__ uint64_t cut_among(const SampleRow<T> &r, SampleLds &s, uint32_t n, uint32_t count, uint64_t mass, V &&visit) {
+    const int tid = threadIdx.x;
+    const bool by_mass = mass != ~0ull;
+    uint64_t lo = 0, hi = ~0ull;
     __syncthreads();
     if (tid == 0) {
-        s.lo = 0xffffffffu;
+        s.lo = ~0ull;
         s.hi = 0;
         s.found = 0;
-        s.threshold = ~0ull;
+        s.last = ~0ull;
     }
-    __syncthreads();
-    {
-        uint32_t lo = 0xffffffffu, hi = 0;
-        for (int i = tid; i < r.vocab; i += kSampleThreads) {
-            const Logit<T> v = (Logit<T>)r.p[i];
-            if (!drawable(v) || order_of(order_key(v), i) < from) continue;
-            const double d = r.below(v);
-            if (SampleRow<T>::bin(d) != bin) continue;
-            lo = min(lo, order_key(v));
-            hi = max(hi, order_key(v));
-        }
-        if (lo <= hi) {
-            atomicMin(&s.lo, lo);
-            atomicMax(&s.hi, hi);
-        }
-    }
-    __syncthreads();
-    uint32_t lo = s.lo, hi = s.hi;
-    // The keys in [lo, hi] are the candidates: too many are parted by key.
-    while (n > kSampleList && lo != hi) {
-        const uint64_t span = (uint64_t)hi - lo + 1;
-        for (int i = tid; i < kSampleBins; i += kSampleThreads) {
-            s.count[i] = 0;
-            s.mass[i] = 0;
-        }
+    if (n > kSampleNear) {
         __syncthreads();
-        for (int i = tid; i < r.vocab; i += kSampleThreads) {
-            const Logit<T> v = (Logit<T>)r.p[i];
-            const uint32_t key = order_key(v);
-            if (!drawable(v) || key < lo || key > hi || order_of(key, i) < from) continue;
-            const int at = (int)((uint64_t)(hi - key) * kSampleBins / span);
-            atomicAdd(&s.count[at], 1u);
-            atomicAdd((unsigned long long *)&s.mass[at], (unsigned long long)r.mass(r.e(r.below(v))));
-        }
-        __syncthreads();
-        cut_bin(s, count, mass);
-        const uint64_t at = (uint64_t)s.bin;
-        // hi - key in [ceil(at * span / bins), ceil((at + 1) * span / bins))
-        const uint64_t first = (at * span + kSampleBins - 1) / kSampleBins, end = ((at + 1) * span + kSampleBins - 1) / kSampleBins;
-        n = s.count[s.bin];
-        count -= s.above_count;
-        mass -= s.above_mass;
-        lo = hi - (uint32_t)(end - 1);
-        hi = hi - (uint32_t)first;
-        __syncthreads();
-    }
-    if (n <= kSampleList) {
-        for (int i = tid; i < r.vocab; i += kSampleThreads) {
-            const Logit<T> v = (Logit<T>)r.p[i];
-            const uint32_t key = order_key(v);
-            if (!drawable(v) || key < lo || key > hi || order_of(key, i) < from) continue;
-            const uint32_t at = atomicAdd(&s.found, 1u);
-            if (at < kSampleList) {
-                s.list[at] = order_of(key, i);
-                s.list_mass[at] = r.mass(r.e(r.below(v)));
-            }
-        }
-        __syncthreads();
-        if (tid < (int)n) {
-            const uint64_t mine = s.list[tid];
-            uint32_t c = 0;
-            uint64_t m = 0;
-            for (int j = 0; j < (int)n; ++j) {
-                const bool earlier = s.list[j] > mine;
-                c += earlier ? 1u : 0u;
-                m += earlier ? s.list_mass[j] : 0ull;
-            }
-            if (c < count && m < mass) atomicMin((unsigned long long *)&s.threshold, (unsigned long long)mine);
-        }
-    } else {
-        // one key: the first tokens of it, in their order
-        const int wave = wave_id(), lane = tid & 63;
-        uint64_t each = 0;
-        uint32_t mine = 0;
-        wave_share(r, wave, [&](Logit<T> v, int i, bool on) {
-            mine += __popcll(__ballot(on && order_key(v) == lo && order_of(lo, i) >= from));
-            return false;
+        uint64_t least = ~0ull, most = 0;
+        visit([&](uint64_t place, double) {
+            least = less(least, place);
+            most = more(most, place);
         });
-        if (lane == 0) s.wave_count[wave] = mine;
-        wave_share(r, wave, [&](Logit<T> v, int, bool on) {     // the mass that each has
-            const bool is = on && order_key(v) == lo;
-            if (is) s.list_mass[0] = r.mass(r.e(r.below(v)));
-            return __any(is) != 0;
-        });
+        for (int o = 32; o > 0; o >>= 1) {
+            least = less(least, shfl_xor64(least, o));
+            most = more(most, shfl_xor64(most, o));
+        }
+        if ((tid & 63) == 0) {
+            atomicMin((unsigned long long *)&s.lo, (unsigned long long)least);
+            atomicMax((unsigned long long *)&s.hi, (unsigned long long)most);
+        }
         __syncthreads();
-        each = s.list_mass[0];
-        uint64_t keep = min((uint64_t)count, (uint64_t)n);
-        if (each != 0) keep = min(keep, (mass - 1) / each + 1);
-        uint32_t seen = 0;
-        for (int w = 0; w < wave; ++w) seen += s.wave_count[w];
-        if (seen < keep && seen + mine >= keep)
-            wave_share(r, wave, [&](Logit<T> v, int i, bool on) {
-                const bool is = on && order_key(v) == lo && order_of(lo, i) >= from;
-                const uint64_t votes = __ballot(is);
-                const uint32_t rank = seen + __popcll(votes & ((1ull << lane) - 1));
-                if (is && rank + 1 == keep) s.threshold = order_of(lo, i);
-                seen += __popcll(votes);
-                return seen >= keep;
+        lo = s.lo;
+        hi = s.hi;
+        while (n > kSampleNear) {
+            const int shift = max(0, 64 - __builtin_clzll((hi - lo) | 1) - 11);      // (hi - lo) >> shift is a bin
+            clear_bins(s);
+            __syncthreads();
+            visit([&](uint64_t place, double d) {
+                if (place < lo || place > hi) return;
+                const int at = (int)((hi - place) >> shift);
+                atomicAdd(&s.count[at], 1u);
+                if (by_mass) atomicAdd((unsigned long long *)&s.mass[at], (unsigned long long)r.mass(r.e(d)));
             });
+            __syncthreads();
+            cut_bin(s, count, mass);
+            n = s.count[s.bin];
+            count -= s.above_count;
+            if (by_mass) mass -= s.above_mass;
+            hi -= (uint64_t)s.bin << shift;
+            lo = more(lo, hi - (((uint64_t)1 << shift) - 1));
+            __syncthreads();
+        }
     }
     __syncthreads();
-    return s.threshold;
+    visit([&](uint64_t place, double d) {
+        if (place < lo || place > hi) return;
+        const uint32_t at = atomicAdd(&s.found, 1u);
+        if (at < kSampleNear) {
+            s.near[at] = place;
+            s.near_mass[at] = by_mass ? r.mass(r.e(d)) : 0;
+        }
+    });
+    __syncthreads();
+    if (tid < (int)n) {
+        const uint64_t mine = s.near[tid];
+        uint32_t c = 0;
+        uint64_t m = 0;
+        for (int j = 0; j < (int)n; ++j) {
+            const bool earlier = s.near[j] > mine;
+            c += earlier ? 1u : 0u;
+            m += earlier ? s.near_mass[j] : 0ull;
+        }
+        if (c < count && m < mass) atomicMin((unsigned long long *)&s.last, (unsigned long long)mine);
+    }
+    __syncthreads();
+    return s.last;
 }
 
 template <class T>
 __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     __shared__ SampleLds s;
+    constexpr int N = 16 / sizeof(T);
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const int64_t row = blockIdx.x;
     SampleRow<T> r;
     r.p = static_cast<const T *>(a.logits) + row * a.ld;
+    r.table = s.table;
     r.vocab = a.vocab;
-    r.scale = a.scale;
 
     // the first of the order
-    uint64_t best = 0;
-    for (int i = tid; i < r.vocab; i += kSampleThreads) {
-        const Logit<T> v = (Logit<T>)r.p[i];
-        if (drawable(v)) best = max(best, order_of(order_key(v), i));
-    }
-    for (int o = 32; o > 0; o >>= 1) best = max(best, shfl_xor64(best, o));
+    Logit<T> most{};
+    int first = -1;
+    each_logit(r, [&](Logit<T> v, int i) {
+        if (first < 0 || v > most) {
+            most = v;
+            first = i;
+        }
+    });
+    uint64_t best = first < 0 ? 0 : order_of(order_key(most), first);
+    for (int o = 32; o > 0; o >>= 1) best = more(best, shfl_xor64(best, o));
     if (lane == 0) s.wave_mass[wave] = best;
-    for (int i = tid; i < kSampleBins; i += kSampleThreads) {
-        s.count[i] = 0;
-        s.mass[i] = 0;
-    }
+    if (tid < 64) s.table[tid] = kExpTable[tid];
+    clear_bins(s);
     __syncthreads();
-    for (int w = 0; w < kSampleWaves; ++w) best = max(best, s.wave_mass[w]);
+    for (int w = 0; w < kSampleWaves; ++w) best = more(best, s.wave_mass[w]);
     const float temperature = a.temperature ? a.temperature[row] : a.temperature_all;
     if (best == 0 || !(temperature > 0.0f)) {     // nothing to draw from, or the first
         if (tid == 0) {
-            a.ids[row] = best ? (int64_t)(uint32_t)~(uint32_t)best : -1;
+            a.ids[row] = best ? (int64_t)token_of(best) : -1;
             if (a.logprob) a.logprob[row] = best ? 0.0f : -__builtin_inff();
         }
         return;
     }
-    r.top_key = (uint32_t)(best >> 32);
-    r.top = (double)(Logit<T>)r.p[(uint32_t)~(uint32_t)best] * a.scale;
-    r.inv_t = 1.0 / (double)temperature;
+    r.top = (double)(Logit<T>)r.p[token_of(best)];
+    r.factor = a.scale / (double)temperature;
     r.unit = (double)(1ull << a.bits);
 
     const int32_t k = a.top_k ? a.top_k[row] : a.top_k_all;
     const float p = a.top_p ? a.top_p[row] : a.top_p_all, least = a.min_p ? a.min_p[row] : a.min_p_all;
-    const bool by_k = k > 0 && k < r.vocab, by_p = p < 1.0f;
+    bool by_k = k > 0 && k < r.vocab;
+    const bool by_p = p < 1.0f;
     uint64_t threshold = 0;
+    uint32_t listed = 0;       // tokens in the list: all that top_k may keep
+    const auto in_list = [&](auto &&f) {
+        for (uint32_t i = tid; i < listed; i += kSampleThreads) f(s.list[i], r.below(value_of<Logit<T>>((uint32_t)(s.list[i] >> 32))));
+    };
+    const auto in_row = [&](auto &&f) { each_logit(r, [&](Logit<T> v, int i) { f(order_of(order_key(v), i), r.below(v)); }); };
+    const auto left = [&](auto &&f) {      // the tokens that the filters so far have left
+        const auto one = [&](uint64_t place, double d) {
+            if (place >= threshold) f(place, d);
+        };
+        if (listed)
+            in_list(one);
+        else
+            in_row(one);
+    };
+    const auto of_bin = [&](int bin) {
+        return [&, bin](auto &&f) {
+            left([&](uint64_t place, double d) {
+                if (SampleRow<T>::bin(d) == bin) f(place, d);
+            });
+        };
+    };
     __syncthreads();
-    if (by_k || by_p) {
-        for (int i = tid; i < r.vocab; i += kSampleThreads) {
-            const Logit<T> v = (Logit<T>)r.p[i];
-            if (!drawable(v)) continue;
-            const double d = r.below(v);
-            const int at = SampleRow<T>::bin(d);
-            atomicAdd(&s.count[at], 1u);
-            if (by_p) {
-                const uint64_t m = r.mass(r.e(d));
-                if (m) atomicAdd((unsigned long long *)&s.mass[at], (unsigned long long)m);
-            }
-        }
+    if (by_k) {
+        each_logit(r, [&](Logit<T> v, int) {
+            const int at = SampleRow<T>::bin(r.below(v));
+            if (at != kSampleBins - 1) atomicAdd(&s.count[at], 1u);
+        });
         __syncthreads();
+        cut_bin(s, (uint32_t)k, ~0ull);
+        const int bin = s.bin;
+        by_k = bin != kSampleBins - 1;      // (the last bin has no mass: a cut in it takes nothing away)
         if (by_k) {
-            cut_bin(s, (uint32_t)k, ~0ull);
-            // (the last bin has no mass: a cut in it takes nothing away)
-            if (s.bin != kSampleBins - 1) threshold = cut_in_bin(r, s, 0, (uint32_t)k - s.above_count, ~0ull);
-        }
-        if (by_p) {
-            // the bins again, of what top_k left: its cut has used them
-            for (int i = tid; i < kSampleBins; i += kSampleThreads) {
-                s.count[i] = 0;
-                s.mass[i] = 0;
+            const uint32_t above = s.above_count, n = s.count[bin];
+            if (above + n <= kSampleList) {
+                if (tid == 0) s.found = 0;
+                __syncthreads();
+                each_logit(r, [&](Logit<T> v, int i) {
+                    if (SampleRow<T>::bin(r.below(v)) <= bin) {
+                        const uint32_t at = atomicAdd(&s.found, 1u);
+                        if (at < kSampleList) s.list[at] = order_of(order_key(v), i);
+                    }
+                });
+                listed = above + n;
+                __syncthreads();
             }
-            __syncthreads();
-            uint64_t sum = 0;
-            for (int i = tid; i < r.vocab; i += kSampleThreads) {
-                const Logit<T> v = (Logit<T>)r.p[i];
-                if (!drawable(v) || order_of(order_key(v), i) < threshold) continue;
-                const double d = r.below(v);
-                const uint64_t m = r.mass(r.e(d));
-                atomicAdd(&s.count[SampleRow<T>::bin(d)], 1u);
-                atomicAdd((unsigned long long *)&s.mass[SampleRow<T>::bin(d)], (unsigned long long)m);
-                sum += m;
-            }
-            sum = wave_sum64(sum);
-            if (lane == 0) s.wave_mass[wave] = sum;
-            __syncthreads();
-            sum = 0;
-            for (int w = 0; w < kSampleWaves; ++w) sum += s.wave_mass[w];
-            __syncthreads();
-            uint64_t mass = p > 0.0f ? (uint64_t)ceil((double)p * (double)sum) : 1;
-            mass = max(mass, (uint64_t)1);
-            cut_bin(s, ~0u, mass);
-            threshold = max(threshold, cut_in_bin(r, s, threshold, ~0u, mass - s.above_mass));
+            threshold = cut_among(r, s, n, (uint32_t)k - above, ~0ull, of_bin(bin));
         }
     }
+    if (by_p) {
+        __syncthreads();
+        clear_bins(s);
+        __syncthreads();
+        uint64_t sum = 0;
+        left([&](uint64_t, double d) {
+            const int at = SampleRow<T>::bin(d);
+            const uint64_t m = r.mass(r.e(d));
+            if (m == 0) return;
+            atomicAdd(&s.count[at], 1u);
+            atomicAdd((unsigned long long *)&s.mass[at], (unsigned long long)m);
+            sum += m;
+        });
+        sum = block_sum(s, sum);
+        const uint64_t mass = more(p > 0.0f ? (uint64_t)ceil((double)p * (double)sum) : 1, 1);
+        cut_bin(s, ~0u, mass);
+        const int bin = s.bin;
+        const uint32_t n = s.count[bin];
+        const uint64_t before = s.above_mass;
+        threshold = more(threshold, cut_among(r, s, n, ~0u, mass - before, [&](auto &&f) {
+            of_bin(bin)([&](uint64_t place, double d) {
+                if (r.mass(r.e(d)) != 0) f(place, d);
+            });
+        }));
+    }
 
+    // a token's mass, 0 for one that is not kept
+    const auto kept = [&](uint64_t place, double d) -> uint64_t {
+        if (place < threshold) return 0;
+        const double e = r.e(d);
+        return e >= (double)least || place == best || !(least > 0.0f) ? r.mass(e) : 0;
+    };
+    const auto target_of = [&](uint64_t total) {
+        const double at = (double)a.u[row] * (double)total;
+        return at > 0.0 ? less((uint64_t)fmin(at, 9e18), total - 1) : (uint64_t)0;
+    };
+    const auto write = [&](int token, uint64_t total) {
+        a.ids[row] = token;
+        if (a.logprob) a.logprob[row] = (float)(r.below((Logit<T>)r.p[token]) - log((double)total / r.unit));
+    };
+    if (listed) {
+        // of the kept ones by token, the last one with no more than the target in front of it
+        uint64_t sum = 0;
+        uint64_t n = 0;
+        const auto by_token = [&](auto &&f) {
+            in_list([&](uint64_t place, double d) {
+                if (kept(place, d) != 0) f((uint64_t)(uint32_t)place, d);
+            });
+        };
+        in_list([&](uint64_t place, double d) {
+            const uint64_t m = kept(place, d);
+            sum += m;
+            n += m != 0 ? 1 : 0;
+        });
+        sum = block_sum(s, sum);
+        n = block_sum(s, n);
+        const uint64_t at = cut_among(r, s, (uint32_t)n, ~0u, target_of(sum) + 1, by_token);
+        if (tid == 0) write(token_of(at), sum);
+        return;
+    }
     // the kept mass of each wave's share of the row, in the order of tokens
-    auto kept = [&](Logit<T> v, int i, bool on) -> uint64_t {
-        if (!on) return 0;
-        const uint64_t at = order_of(order_key(v), i);
-        if (at < threshold) return 0;
-        const double e = r.e(r.below(v));
-        return e >= (double)least || at == best || !(least > 0.0f) ? r.mass(e) : 0;
+    const auto masses = [&](const Packed<T, N> &v, int i, int n, uint64_t *m) {
+        uint64_t sum = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const Logit<T> l = (Logit<T>)v.v[e];
+            m[e] = e < n && drawable(l) ? kept(order_of(order_key(l), i + e), r.below(l)) : 0;
+            sum += m[e];
+        }
+        return sum;
     };
     uint64_t sum = 0;
-    wave_share(r, wave, [&](Logit<T> v, int i, bool on) {
-        sum += kept(v, i, on);
+    wave_share(r, wave, [&](const Packed<T, N> &v, int i, int n) {
+        uint64_t m[N];
+        sum += masses(v, i, n, m);
         return false;
     });
-    sum = wave_sum64(sum);
+    for (int o = 32; o > 0; o >>= 1) sum += shfl_xor64(sum, o);
+    __syncthreads();
     if (lane == 0) s.wave_mass[wave] = sum;
     __syncthreads();
     uint64_t total = 0, before = 0;
@@ -383,13 +502,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
         before += w < wave ? s.wave_mass[w] : 0;
         total += s.wave_mass[w];
     }
-    const float u = a.u[row];
-    const double at = (double)u * (double)total;
-    const uint64_t target = at > 0.0 ? min((uint64_t)fmin(at, 9e18), total - 1) : 0;
+    const uint64_t target = target_of(total);
     if (!(before <= target && target < before + sum)) return;
-    wave_share(r, wave, [&](Logit<T> v, int i, bool on) {
-        const uint64_t m = kept(v, i, on);
-        uint64_t run = m;
+    wave_share(r, wave, [&](const Packed<T, N> &v, int i, int n) {
+        uint64_t m[N], run = masses(v, i, n, m);
+        const uint64_t mine = run;
         for (int o = 1; o < 64; o <<= 1) {
             const uint64_t up = shfl_up64(run, o);
             if (lane >= o) run += up;
@@ -397,8 +514,12 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
         const uint64_t votes = __ballot(before + run > target);
         if (votes != 0) {
             if (lane == __ffsll((unsigned long long)votes) - 1) {
-                a.ids[row] = i;
-                if (a.logprob) a.logprob[row] = (float)(r.below(v) - log((double)total / r.unit));
+                uint64_t at = before + run - mine;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    if (at <= target && target < at + m[e]) write(i + e, total);
+                    at += m[e];
+                }
             }
             return true;
         }
@@ -432,7 +553,7 @@ extern "C" mi_status mi_sample_tokens(const void *logits, int type, int64_t ld, 
     while ((1 << log2v) < vocab) ++log2v;
     // the masses of a row sum to 2^62 at most
     const SampleArgs a{logits, ld, scale, u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all,
-                       ids, logprob, vocab, min(52, 62 - log2v)};
+                       ids, logprob, vocab, min(51, 62 - log2v)};
     const hipStream_t st = as_stream(stream);
     const auto launch = [&](auto t) {
         hipLaunchKernelGGL((sample_kernel<decltype(t)>), dim3((unsigned)rows), dim3(kSampleThreads), 0, st, a);
