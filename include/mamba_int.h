@@ -632,11 +632,14 @@ mi_status mi_w4_matvec(const void *x, int64_t ldx, int type, const uint8_t *pack
  *   temperature, top_k, top_p, min_p   [rows], or NULL for the one value
  *           *_all of every row (which must be a number);
  *   ids int64, logprob fp32 [rows].
+ *   workspace   16-byte aligned, mi_sample_workspace_size bytes (0: may be NULL).
  * vocab in [1, 2^24], rows < 2^22. */
+mi_status mi_sample_workspace_size(int rows, int vocab, size_t *bytes);
 mi_status mi_sample_tokens(const void *logits, int type, int64_t ld, double scale, const float *u,
                            const float *temperature, float temperature_all, const int32_t *top_k, int top_k_all,
                            const float *top_p, float top_p_all, const float *min_p, float min_p_all,
-                           int64_t *ids, float *logprob, int rows, int vocab, void *stream);
+                           int64_t *ids, float *logprob, int rows, int vocab, void *workspace, size_t workspace_bytes,
+                           void *stream);
 
 /* Low-rank adapters beside a shared projection, each sequence with its own of
  * a bank:

@@ -31,6 +31,7 @@ decltype(&mi_causal_conv) g_conv;
 decltype(&mi_selective_scan) g_scan;
 decltype(&mi_selective_scan_workspace_size) g_scan_size;
 decltype(&mi_w4_matvec) g_w4;
+decltype(&mi_sample_workspace_size) g_sample_size;
 decltype(&mi_sample_tokens) g_sample;
 decltype(&mi_adapter_workspace_size) g_adapter_size;
 decltype(&mi_adapter_add) g_adapter;
@@ -396,8 +397,13 @@ PyObject *sample_tokens(PyObject *const *a, Py_ssize_t n) {
     int64_t *ip = vec<int64_t>(ids.p, {B}, at::kLong, "out");
     Ref lp(with_logprob ? empty({B}, x, at::kFloat) : (Py_INCREF(Py_None), Py_None));
     float *lpp = with_logprob ? static_cast<float *>(THPVariable_Unpack(lp.p).data_ptr()) : nullptr;
-    check("mi_sample_tokens", g_sample(xr.p, code, xr.ld, scale, u, t, t_all, k, k_all, p, p_all, least, min_all, ip, lpp,
-                                       size_of(B, "rows"), size_of(V, "vocab"), stream));
+    const int bi = size_of(B, "rows"), vi = size_of(V, "vocab");
+    size_t bytes = 0;
+    check("mi_sample_workspace_size", g_sample_size(bi, vi, &bytes));
+    Tensor ws;
+    if (bytes) ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    check("mi_sample_tokens", g_sample(xr.p, code, xr.ld, scale, u, t, t_all, k, k_all, p, p_all, least, min_all, ip, lpp, bi, vi,
+                                       bytes ? ws.data_ptr() : nullptr, bytes, stream));
     written(a[9]);
     return with_logprob ? Py_BuildValue("(NN)", ids.release(), lp.release()) : ids.release();
 }
@@ -551,19 +557,20 @@ PyObject *check_accumulator(PyObject *const *a, Py_ssize_t n) {
 // (MIError, addresses of the entry points)
 PyObject *init(PyObject *const *a, Py_ssize_t n) {
     const auto entry = [&](int i, auto &f) { f = reinterpret_cast<std::decay_t<decltype(f)>>(address(a[i])); };
-    count(n, 13, "init");
+    count(n, 14, "init");
     entry(1, g_norm);
     entry(2, g_conv);
     entry(3, g_scan_size);
     entry(4, g_scan);
     entry(5, g_w4);
-    entry(6, g_sample);
-    entry(7, g_adapter_size);
-    entry(8, g_adapter);
-    entry(9, g_gated_sizes);
-    entry(10, g_gated);
-    entry(11, g_gated_backward);
-    entry(12, g_last_error);
+    entry(6, g_sample_size);
+    entry(7, g_sample);
+    entry(8, g_adapter_size);
+    entry(9, g_adapter);
+    entry(10, g_gated_sizes);
+    entry(11, g_gated);
+    entry(12, g_gated_backward);
+    entry(13, g_last_error);
     Py_INCREF(a[0]);
     Py_XDECREF(g_mi_error);
     g_mi_error = a[0];

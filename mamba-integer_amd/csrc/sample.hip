@@ -12,6 +12,7 @@
 // integer, so every sum is exact, in any order.  The kept tokens are a beginning of the
 // order, so one 64-bit number (the key of l above the token's complement) tells them
 // from the rest.
+#include <algorithm>
 #include <type_traits>
 
 #include "float_ops.hpp"
@@ -22,7 +23,8 @@ constexpr int kSampleThreads = 1024;
 constexpr int kSampleWaves = kSampleThreads / 64;
 constexpr int kSampleBins = 2048;
 constexpr int kSampleNear = 256;            // candidates whose ranks are counted pairwise
-constexpr int kSampleList = 2048;           // candidates of a small top_k, all in LDS
+constexpr int kSampleList = 8192;           // candidates of a row that are listed
+constexpr int kSampleSlices = 64;           // of a row, at most
 constexpr int kSampleMaxVocab = 1 << 24;
 constexpr double kSampleRange = 40.0;       // e^-40 * 2^51 rounds to a mass of 0
 
@@ -37,6 +39,18 @@ struct SampleArgs {
     int64_t *ids;
     float *logprob;
     int vocab, bits;
+    int slices, slice;      // of a row, and tokens of one
+    char *workspace;
+};
+
+// What the kernels of a row pass on, in the workspace.
+struct SampleShared {
+    uint64_t best[kSampleSlices];            // the first of the order in a slice
+    uint64_t slice_mass[kSampleSlices];      // the mass of a slice that is surely kept
+    uint64_t mass[kSampleBins];
+    uint32_t count[kSampleBins];
+    uint32_t found, unused;
+    uint64_t list[kSampleList];              // places of candidates
 };
 
 // A logit's place in the order: larger for larger logits, 0 and -0 alike.
@@ -86,7 +100,6 @@ struct SampleLds {
     double table[64];
     uint32_t count[kSampleBins];
     uint64_t mass[kSampleBins];
-    uint64_t list[kSampleList];               // places of the candidates of a small top_k
     uint64_t near[kSampleNear], near_mass[kSampleNear];
     uint64_t wave_mass[kSampleWaves], lo, hi, above_mass, last;
     uint32_t wave_count[kSampleWaves], above_count, found;
@@ -118,7 +131,7 @@ struct SampleRow {
     const T *p;
     const double *table;
     double top, factor, unit;      // the largest logit; scale / temperature; 2^bits
-    int vocab;
+    int begin, end;                // the tokens that the passes go over
 
     // l - max l over the temperature: 0 for the largest (an infinite one too), -inf or NaN far below
     __device__ __forceinline__ double below(Logit<T> v) const { return (double)v == top ? 0.0 : ((double)v - top) * factor; }
@@ -157,15 +170,15 @@ __device__ __forceinline__ Packed<T, N> load_logits(const T *p, int i, int end) 
 template <class T, class F>
 __device__ __forceinline__ void each_logit(const SampleRow<T> &r, F &&f) {
     constexpr int N = 16 / sizeof(T), STEP = kSampleThreads * N;
-    int i = (int)threadIdx.x * N;
+    int i = r.begin + (int)threadIdx.x * N;
     Packed<T, N> next;
-    if (i < r.vocab) next = load_logits(r.p, i, r.vocab);
-    for (; i < r.vocab; i += STEP) {
+    if (i < r.end) next = load_logits(r.p, i, r.end);
+    for (; i < r.end; i += STEP) {
         const Packed<T, N> now = next;
-        if (i + STEP < r.vocab) next = load_logits(r.p, i + STEP, r.vocab);
+        if (i + STEP < r.end) next = load_logits(r.p, i + STEP, r.end);
 #pragma unroll
         for (int e = 0; e < N; ++e)
-            if (i + e < r.vocab && drawable((Logit<T>)now.v[e])) f((Logit<T>)now.v[e], i + e);
+            if (i + e < r.end && drawable((Logit<T>)now.v[e])) f((Logit<T>)now.v[e], i + e);
     }
 }
 
@@ -174,10 +187,10 @@ __device__ __forceinline__ void each_logit(const SampleRow<T> &r, F &&f) {
 template <class T, class F>
 __device__ __forceinline__ void wave_share(const SampleRow<T> &r, int wave, F &&f) {
     constexpr int N = 16 / sizeof(T), STEP = 64 * N;
-    const int share = (r.vocab + kSampleWaves * STEP - 1) / (kSampleWaves * STEP) * STEP;
-    const int end = min((wave + 1) * share, r.vocab), lane = (int)threadIdx.x & 63;
+    const int share = (r.end - r.begin + kSampleWaves * STEP - 1) / (kSampleWaves * STEP) * STEP;
+    const int end = min(r.begin + (wave + 1) * share, r.end), lane = (int)threadIdx.x & 63;
     Packed<T, N> next;
-    int base = wave * share;
+    int base = r.begin + wave * share;
     if (base < end) next = load_logits(r.p, base + lane * N, end);
     for (; base < end; base += STEP) {
         const Packed<T, N> now = next;
@@ -324,18 +337,9 @@ __device__ __forceinline__ uint64_t cut_among(const SampleRow<T> &r, SampleLds &
     return s.last;
 }
 
+// The first of the order among the row's tokens in [begin, end), by all threads.
 template <class T>
-__global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
-    __shared__ SampleLds s;
-    constexpr int N = 16 / sizeof(T);
-    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
-    const int64_t row = blockIdx.x;
-    SampleRow<T> r;
-    r.p = static_cast<const T *>(a.logits) + row * a.ld;
-    r.table = s.table;
-    r.vocab = a.vocab;
-
-    // the first of the order
+__device__ __forceinline__ uint64_t first_of(const SampleRow<T> &r, SampleLds &s) {
     Logit<T> most{};
     int first = -1;
     each_logit(r, [&](Logit<T> v, int i) {
@@ -346,77 +350,233 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     });
     uint64_t best = first < 0 ? 0 : order_of(order_key(most), first);
     for (int o = 32; o > 0; o >>= 1) best = more(best, shfl_xor64(best, o));
-    if (lane == 0) s.wave_mass[wave] = best;
+    if ((threadIdx.x & 63) == 0) s.wave_mass[wave_id()] = best;
+    __syncthreads();
+    for (int w = 0; w < kSampleWaves; ++w) best = more(best, s.wave_mass[w]);
+    return best;
+}
+
+// A row's parameters.
+struct SampleFilters {
+    float temperature, p, least;
+    int32_t k;
+    bool by_k, by_p;
+    __device__ __forceinline__ SampleFilters(const SampleArgs &a, int64_t row) {
+        temperature = a.temperature ? a.temperature[row] : a.temperature_all;
+        k = a.top_k ? a.top_k[row] : a.top_k_all;
+        p = a.top_p ? a.top_p[row] : a.top_p_all;
+        least = a.min_p ? a.min_p[row] : a.min_p_all;
+        by_k = k > 0 && k < a.vocab;
+        by_p = p < 1.0f;
+    }
+    // the least mass that top_p keeps of `sum`
+    __device__ __forceinline__ uint64_t mass_of(uint64_t sum) const {
+        return more(p > 0.0f ? (uint64_t)ceil((double)p * (double)sum) : 1, 1);
+    }
+};
+template <class T>
+__device__ __forceinline__ SampleRow<T> sample_row(const SampleArgs &a, const SampleLds &s, int64_t row, int begin, int end) {
+    SampleRow<T> r;
+    r.p = static_cast<const T *>(a.logits) + row * a.ld;
+    r.table = s.table;
+    r.begin = begin;
+    r.end = end;
+    return r;
+}
+template <class T>
+__device__ __forceinline__ void scale_by(SampleRow<T> &r, const SampleArgs &a, uint64_t best, float temperature) {
+    r.top = (double)(Logit<T>)r.p[token_of(best)];
+    r.factor = a.scale / (double)temperature;
+    r.unit = (double)(1ull << a.bits);
+}
+
+// ------------------------------------------------------------------ slices
+// Few rows of many tokens: a row's passes are shared by `slices` blocks, in a kernel each
+// (the first of the order; the bins; what the bins leave), and the last kernel draws.
+__device__ __forceinline__ SampleShared &shared_of(const SampleArgs &a, int64_t row) {
+    return reinterpret_cast<SampleShared *>(a.workspace)[row];
+}
+__device__ __forceinline__ uint64_t best_of(const SampleArgs &a, const SampleShared &g) {
+    uint64_t best = 0;
+    for (int i = 0; i < a.slices; ++i) best = more(best, g.best[i]);
+    return best;
+}
+
+template <class T>
+__global__ __launch_bounds__(kSampleThreads) void sample_first_kernel(SampleArgs a) {
+    __shared__ SampleLds s;
+    const int64_t row = blockIdx.y;
+    const int slice = blockIdx.x;
+    SampleShared &g = shared_of(a, row);
+    for (int i = slice * kSampleThreads + (int)threadIdx.x; i < kSampleBins; i += a.slices * kSampleThreads) {
+        g.count[i] = 0;
+        g.mass[i] = 0;
+    }
+    const SampleRow<T> r = sample_row<T>(a, s, row, slice * a.slice, min((slice + 1) * a.slice, a.vocab));
+    const uint64_t best = first_of(r, s);
+    if (threadIdx.x == 0) {
+        g.best[slice] = best;
+        if (slice == 0) g.found = 0;
+    }
+}
+
+// Counts, for top_k, or masses, for top_p alone, added to the row's bins.
+template <class T>
+__global__ __launch_bounds__(kSampleThreads) void sample_bins_kernel(SampleArgs a) {
+    __shared__ SampleLds s;
+    const int64_t row = blockIdx.y;
+    const int slice = blockIdx.x, tid = threadIdx.x;
+    SampleShared &g = shared_of(a, row);
+    const SampleFilters f(a, row);
+    const uint64_t best = best_of(a, g);
+    if (best == 0 || !(f.temperature > 0.0f) || !(f.by_k || f.by_p)) return;
+    SampleRow<T> r = sample_row<T>(a, s, row, slice * a.slice, min((slice + 1) * a.slice, a.vocab));
+    scale_by(r, a, best, f.temperature);
     if (tid < 64) s.table[tid] = kExpTable[tid];
     clear_bins(s);
     __syncthreads();
-    for (int w = 0; w < kSampleWaves; ++w) best = more(best, s.wave_mass[w]);
-    const float temperature = a.temperature ? a.temperature[row] : a.temperature_all;
-    if (best == 0 || !(temperature > 0.0f)) {     // nothing to draw from, or the first
+    if (f.by_k)
+        each_logit(r, [&](Logit<T> v, int) {
+            const int at = SampleRow<T>::bin(r.below(v));
+            if (at != kSampleBins - 1) atomicAdd(&s.count[at], 1u);
+        });
+    else
+        each_logit(r, [&](Logit<T> v, int) {
+            const double d = r.below(v);
+            const int at = SampleRow<T>::bin(d);
+            const uint64_t m = r.mass(r.e(d));
+            if (m == 0) return;
+            atomicAdd(&s.count[at], 1u);
+            atomicAdd((unsigned long long *)&s.mass[at], (unsigned long long)m);
+        });
+    __syncthreads();
+    for (int i = tid; i < kSampleBins; i += kSampleThreads) {
+        if (s.count[i]) atomicAdd(&g.count[i], s.count[i]);
+        if (s.mass[i]) atomicAdd((unsigned long long *)&g.mass[i], (unsigned long long)s.mass[i]);
+    }
+}
+
+// What the bins say: the bin in which the first filter cuts, how many tokens are candidates
+// (top_k: all that it may keep; top_p alone: those of the bin), or that the row has to be gone
+// over as a whole.  LDS has the row's bins then.  All threads.
+struct SampleCut {
+    bool whole;
+    int bin;
+    uint32_t listed;
+    uint64_t mass;      // top_p alone: what is kept of the bin's mass, at least
+};
+__device__ __forceinline__ SampleCut cut_row(const SampleShared &g, SampleLds &s, const SampleFilters &f) {
+    for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) {
+        s.count[i] = g.count[i];
+        s.mass[i] = g.mass[i];
+    }
+    __syncthreads();
+    SampleCut c{};
+    if (f.by_k) {
+        cut_bin(s, (uint32_t)f.k, ~0ull);
+        c.bin = s.bin;
+        c.listed = c.bin == kSampleBins - 1 ? 0 : s.above_count + s.count[c.bin];
+        c.whole = c.bin == kSampleBins - 1 || c.listed > kSampleList;
+    } else {
+        uint64_t sum = 0;
+        for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) sum += s.mass[i];
+        const uint64_t mass = f.mass_of(block_sum(s, sum));
+        cut_bin(s, ~0u, mass);
+        c.bin = s.bin;
+        c.listed = s.count[c.bin];
+        c.whole = c.listed > kSampleList;
+        c.mass = mass - s.above_mass;
+    }
+    return c;
+}
+
+template <class T>
+__global__ __launch_bounds__(kSampleThreads) void sample_gather_kernel(SampleArgs a) {
+    __shared__ SampleLds s;
+    const int64_t row = blockIdx.y;
+    const int slice = blockIdx.x, tid = threadIdx.x;
+    SampleShared &g = shared_of(a, row);
+    const SampleFilters f(a, row);
+    const uint64_t best = best_of(a, g);
+    if (best == 0 || !(f.temperature > 0.0f)) return;
+    SampleCut c{};
+    c.bin = kSampleBins;      // (without top_k and top_p every token is surely kept)
+    if (f.by_k || f.by_p) c = cut_row(g, s, f);
+    if (c.whole) return;
+    SampleRow<T> r = sample_row<T>(a, s, row, slice * a.slice, min((slice + 1) * a.slice, a.vocab));
+    scale_by(r, a, best, f.temperature);
+    if (tid < 64) s.table[tid] = kExpTable[tid];
+    __syncthreads();
+    uint64_t sum = 0;
+    const auto list = [&](Logit<T> v, int i) {
+        const uint32_t at = atomicAdd(&g.found, 1u);
+        if (at < kSampleList) g.list[at] = order_of(order_key(v), i);
+    };
+    if (f.by_k)
+        each_logit(r, [&](Logit<T> v, int i) {
+            if (SampleRow<T>::bin(r.below(v)) <= c.bin) list(v, i);
+        });
+    else
+        each_logit(r, [&](Logit<T> v, int i) {
+            const double d = r.below(v);
+            const int at = SampleRow<T>::bin(d);
+            if (at > c.bin) return;
+            const double e = r.e(d);
+            if (at == c.bin) {
+                if (r.mass(e) != 0) list(v, i);      // (as the bins count)
+            } else if (e >= (double)f.least || !(f.least > 0.0f) || order_of(order_key(v), i) == best) {
+                sum += r.mass(e);
+            }
+        });
+    sum = block_sum(s, sum);
+    if (tid == 0) g.slice_mass[slice] = sum;
+}
+
+// A block a row: all of it, or after the kernels above.
+template <class T, bool SLICES>
+__global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
+    __shared__ SampleLds s;
+    constexpr int N = 16 / sizeof(T);
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+    const int64_t row = blockIdx.x;
+    SampleRow<T> r = sample_row<T>(a, s, row, 0, a.vocab);
+    SampleShared &g = shared_of(a, row);
+    const SampleFilters f(a, row);
+    const uint64_t best = SLICES ? best_of(a, g) : first_of(r, s);
+    if (tid < 64) s.table[tid] = kExpTable[tid];
+    clear_bins(s);
+    if (best == 0 || !(f.temperature > 0.0f)) {     // nothing to draw from, or the first
         if (tid == 0) {
             a.ids[row] = best ? (int64_t)token_of(best) : -1;
             if (a.logprob) a.logprob[row] = best ? 0.0f : -__builtin_inff();
         }
         return;
     }
-    r.top = (double)(Logit<T>)r.p[token_of(best)];
-    r.factor = a.scale / (double)temperature;
-    r.unit = (double)(1ull << a.bits);
-
-    const int32_t k = a.top_k ? a.top_k[row] : a.top_k_all;
-    const float p = a.top_p ? a.top_p[row] : a.top_p_all, least = a.min_p ? a.min_p[row] : a.min_p_all;
-    bool by_k = k > 0 && k < r.vocab;
-    const bool by_p = p < 1.0f;
+    scale_by(r, a, best, f.temperature);
     uint64_t threshold = 0;
-    uint32_t listed = 0;       // tokens in the list: all that top_k may keep
-    const auto in_list = [&](auto &&f) {
-        for (uint32_t i = tid; i < listed; i += kSampleThreads) f(s.list[i], r.below(value_of<Logit<T>>((uint32_t)(s.list[i] >> 32))));
+    const uint64_t *listed = nullptr;      // tokens that may be left, if they are few
+    uint32_t n_listed = 0;
+    const auto in_list = [&](auto &&fn) {
+        for (uint32_t i = tid; i < n_listed; i += kSampleThreads) fn(listed[i], r.below(value_of<Logit<T>>((uint32_t)(listed[i] >> 32))));
     };
-    const auto in_row = [&](auto &&f) { each_logit(r, [&](Logit<T> v, int i) { f(order_of(order_key(v), i), r.below(v)); }); };
-    const auto left = [&](auto &&f) {      // the tokens that the filters so far have left
+    const auto in_row = [&](auto &&fn) { each_logit(r, [&](Logit<T> v, int i) { fn(order_of(order_key(v), i), r.below(v)); }); };
+    const auto left = [&](auto &&fn) {      // the tokens that the filters so far have left
         const auto one = [&](uint64_t place, double d) {
-            if (place >= threshold) f(place, d);
+            if (place >= threshold) fn(place, d);
         };
-        if (listed)
+        if (SLICES && listed)
             in_list(one);
         else
             in_row(one);
     };
     const auto of_bin = [&](int bin) {
-        return [&, bin](auto &&f) {
+        return [&, bin](auto &&fn) {
             left([&](uint64_t place, double d) {
-                if (SampleRow<T>::bin(d) == bin) f(place, d);
+                if (SampleRow<T>::bin(d) == bin && r.mass(r.e(d)) != 0) fn(place, d);
             });
         };
     };
-    __syncthreads();
-    if (by_k) {
-        each_logit(r, [&](Logit<T> v, int) {
-            const int at = SampleRow<T>::bin(r.below(v));
-            if (at != kSampleBins - 1) atomicAdd(&s.count[at], 1u);
-        });
-        __syncthreads();
-        cut_bin(s, (uint32_t)k, ~0ull);
-        const int bin = s.bin;
-        by_k = bin != kSampleBins - 1;      // (the last bin has no mass: a cut in it takes nothing away)
-        if (by_k) {
-            const uint32_t above = s.above_count, n = s.count[bin];
-            if (above + n <= kSampleList) {
-                if (tid == 0) s.found = 0;
-                __syncthreads();
-                each_logit(r, [&](Logit<T> v, int i) {
-                    if (SampleRow<T>::bin(r.below(v)) <= bin) {
-                        const uint32_t at = atomicAdd(&s.found, 1u);
-                        if (at < kSampleList) s.list[at] = order_of(order_key(v), i);
-                    }
-                });
-                listed = above + n;
-                __syncthreads();
-            }
-            threshold = cut_among(r, s, n, (uint32_t)k - above, ~0ull, of_bin(bin));
-        }
-    }
-    if (by_p) {
+    const auto cut_mass = [&] {      // top_p of what is left
         __syncthreads();
         clear_bins(s);
         __syncthreads();
@@ -429,24 +589,64 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
             atomicAdd((unsigned long long *)&s.mass[at], (unsigned long long)m);
             sum += m;
         });
-        sum = block_sum(s, sum);
-        const uint64_t mass = more(p > 0.0f ? (uint64_t)ceil((double)p * (double)sum) : 1, 1);
+        const uint64_t mass = f.mass_of(block_sum(s, sum));
         cut_bin(s, ~0u, mass);
         const int bin = s.bin;
         const uint32_t n = s.count[bin];
         const uint64_t before = s.above_mass;
-        threshold = more(threshold, cut_among(r, s, n, ~0u, mass - before, [&](auto &&f) {
-            of_bin(bin)([&](uint64_t place, double d) {
-                if (r.mass(r.e(d)) != 0) f(place, d);
+        threshold = more(threshold, cut_among(r, s, n, ~0u, mass - before, of_bin(bin)));
+    };
+    __syncthreads();
+    bool by_slices = SLICES;       // the row's mass is known by slices, but for the listed tokens
+    if (SLICES && (f.by_k || f.by_p)) {
+        const SampleCut c = cut_row(g, s, f);
+        by_slices = !c.whole && !f.by_k;
+        if (!c.whole) {
+            listed = g.list;
+            n_listed = c.listed;
+            if (f.by_k) {
+                const uint32_t n = s.count[c.bin];
+                threshold = cut_among(r, s, n, (uint32_t)f.k - (c.listed - n), ~0ull, [&](auto &&fn) {
+                    in_list([&](uint64_t place, double d) {
+                        if (SampleRow<T>::bin(d) == c.bin) fn(place, d);
+                    });
+                });
+                if (f.by_p) cut_mass();
+            } else {
+                threshold = cut_among(r, s, c.listed, ~0u, c.mass, in_list);
+            }
+        }
+    }
+    if (!listed && !by_slices) {
+        if (f.by_k) {
+            __syncthreads();
+            clear_bins(s);
+            __syncthreads();
+            each_logit(r, [&](Logit<T> v, int) {
+                const int at = SampleRow<T>::bin(r.below(v));
+                if (at != kSampleBins - 1) atomicAdd(&s.count[at], 1u);
             });
-        }));
+            __syncthreads();
+            cut_bin(s, (uint32_t)f.k, ~0ull);
+            const int bin = s.bin;
+            // (the last bin has no mass: a cut in it takes nothing away)
+            if (bin != kSampleBins - 1) {
+                const uint32_t above = s.above_count, n = s.count[bin];
+                threshold = cut_among(r, s, n, (uint32_t)f.k - above, ~0ull, [&](auto &&fn) {
+                    in_row([&](uint64_t place, double d) {
+                        if (SampleRow<T>::bin(d) == bin) fn(place, d);
+                    });
+                });
+            }
+        }
+        if (f.by_p) cut_mass();
     }
 
     // a token's mass, 0 for one that is not kept
     const auto kept = [&](uint64_t place, double d) -> uint64_t {
         if (place < threshold) return 0;
         const double e = r.e(d);
-        return e >= (double)least || place == best || !(least > 0.0f) ? r.mass(e) : 0;
+        return e >= (double)f.least || place == best || !(f.least > 0.0f) ? r.mass(e) : 0;
     };
     const auto target_of = [&](uint64_t total) {
         const double at = (double)a.u[row] * (double)total;
@@ -456,15 +656,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
         a.ids[row] = token;
         if (a.logprob) a.logprob[row] = (float)(r.below((Logit<T>)r.p[token]) - log((double)total / r.unit));
     };
-    if (listed) {
+    uint64_t total = 0, before = 0, target = 0;
+    if (SLICES && listed && f.by_k) {
         // of the kept ones by token, the last one with no more than the target in front of it
-        uint64_t sum = 0;
-        uint64_t n = 0;
-        const auto by_token = [&](auto &&f) {
-            in_list([&](uint64_t place, double d) {
-                if (kept(place, d) != 0) f((uint64_t)(uint32_t)place, d);
-            });
-        };
+        uint64_t sum = 0, n = 0;
         in_list([&](uint64_t place, double d) {
             const uint64_t m = kept(place, d);
             sum += m;
@@ -472,11 +667,32 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
         });
         sum = block_sum(s, sum);
         n = block_sum(s, n);
-        const uint64_t at = cut_among(r, s, (uint32_t)n, ~0u, target_of(sum) + 1, by_token);
+        const uint64_t at = cut_among(r, s, (uint32_t)n, ~0u, target_of(sum) + 1, [&](auto &&fn) {
+            in_list([&](uint64_t place, double d) {
+                if (kept(place, d) != 0) fn((uint64_t)(uint32_t)place, d);
+            });
+        });
         if (tid == 0) write(token_of(at), sum);
         return;
     }
-    // the kept mass of each wave's share of the row, in the order of tokens
+    if (SLICES && by_slices) {
+        // the slices' kept masses, and the slice that the target lies in
+        __syncthreads();
+        for (int i = tid; i < a.slices; i += kSampleThreads) s.mass[i] = g.slice_mass[i];
+        __syncthreads();
+        in_list([&](uint64_t place, double d) {
+            const uint64_t m = kept(place, d);
+            if (m) atomicAdd((unsigned long long *)&s.mass[token_of(place) / a.slice], (unsigned long long)m);
+        });
+        __syncthreads();
+        for (int i = 0; i < a.slices; ++i) total += s.mass[i];
+        target = target_of(total);
+        int slice = 0;
+        for (; before + s.mass[slice] <= target; ++slice) before += s.mass[slice];
+        r.begin = slice * a.slice;
+        r.end = min(r.begin + a.slice, a.vocab);
+    }
+    // the kept mass of each wave's share of the row, or slice, in the order of tokens
     const auto masses = [&](const Packed<T, N> &v, int i, int n, uint64_t *m) {
         uint64_t sum = 0;
 #pragma unroll
@@ -497,12 +713,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     __syncthreads();
     if (lane == 0) s.wave_mass[wave] = sum;
     __syncthreads();
-    uint64_t total = 0, before = 0;
-    for (int w = 0; w < kSampleWaves; ++w) {
-        before += w < wave ? s.wave_mass[w] : 0;
-        total += s.wave_mass[w];
+    for (int w = 0; w < wave; ++w) before += s.wave_mass[w];
+    if (!(SLICES && by_slices)) {
+        for (int w = 0; w < kSampleWaves; ++w) total += s.wave_mass[w];
+        target = target_of(total);
     }
-    const uint64_t target = target_of(total);
     if (!(before <= target && target < before + sum)) return;
     wave_share(r, wave, [&](const Packed<T, N> &v, int i, int n) {
         uint64_t m[N], run = masses(v, i, n, m);
@@ -528,14 +743,31 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     });
 }
 
+// Slices of a row: 4096 tokens or more, and at most 512 blocks of all rows.
+inline int sample_slices(int rows, int vocab) {
+    const int n = std::min((vocab + 4095) / 4096, kSampleSlices);
+    return std::max(1, std::min(n, 512 / std::max(rows, 1)));
+}
+
 }  // namespace mi
 
 using namespace mi;
 
+extern "C" mi_status mi_sample_workspace_size(int rows, int vocab, size_t *bytes) {
+    clear_error();
+    MI_REQUIRE(bytes, MI_ERR_NULL_POINTER, "mi_sample_workspace_size: bytes is required");
+    MI_REQUIRE(rows >= 0 && rows < (1 << 22), MI_ERR_BAD_DIM, "mi_sample_workspace_size: rows=%d must be in [0, %d)", rows, 1 << 22);
+    MI_REQUIRE(vocab >= 1 && vocab <= kSampleMaxVocab, MI_ERR_BAD_DIM, "mi_sample_workspace_size: vocab=%d must be in [1, %d]", vocab,
+               kSampleMaxVocab);
+    *bytes = sample_slices(rows, vocab) > 1 ? (size_t)rows * sizeof(SampleShared) : 0;
+    return MI_OK;
+}
+
 extern "C" mi_status mi_sample_tokens(const void *logits, int type, int64_t ld, double scale, const float *u,
                                       const float *temperature, float temperature_all, const int32_t *top_k, int top_k_all,
                                       const float *top_p, float top_p_all, const float *min_p, float min_p_all, int64_t *ids,
-                                      float *logprob, int rows, int vocab, void *stream) {
+                                      float *logprob, int rows, int vocab, void *workspace, size_t workspace_bytes,
+                                      void *stream) {
     clear_error();
     MI_REQUIRE(rows >= 0, MI_ERR_BAD_DIM, "mi_sample_tokens: negative rows");
     MI_REQUIRE(rows < (1 << 22), MI_ERR_BAD_DIM, "mi_sample_tokens: rows=%d must be below %d", rows, 1 << 22);
@@ -549,14 +781,32 @@ extern "C" mi_status mi_sample_tokens(const void *logits, int type, int64_t ld, 
                "mi_sample_tokens: top_p or min_p is not a number");
     if (rows == 0) return MI_OK;
     MI_REQUIRE(logits && u && ids, MI_ERR_NULL_POINTER, "mi_sample_tokens: logits, u and ids are required");
+    const int slices = sample_slices(rows, vocab);
+    const size_t need = slices > 1 ? (size_t)rows * sizeof(SampleShared) : 0;
+    MI_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), MI_ERR_BAD_ARG,
+               "mi_sample_tokens: the workspace has %zu bytes, %zu are needed", workspace_bytes, need);
+    MI_REQUIRE(need == 0 || aligned(workspace, 16), MI_ERR_BAD_ALIGNMENT, "mi_sample_tokens: the workspace must be 16-byte aligned");
     int log2v = 0;
     while ((1 << log2v) < vocab) ++log2v;
-    // the masses of a row sum to 2^62 at most
-    const SampleArgs a{logits, ld, scale, u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all,
-                       ids, logprob, vocab, min(51, 62 - log2v)};
+    // the masses of a row sum to 2^62 at most; a slice has whole vectors of 16 bytes
+    SampleArgs a{logits, ld, scale, u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all,
+                 ids, logprob, vocab, std::min(51, 62 - log2v), slices, ((vocab + slices - 1) / slices + 7) / 8 * 8,
+                 static_cast<char *>(workspace)};
+    a.slices = (vocab + a.slice - 1) / a.slice;      // (none without tokens)
     const hipStream_t st = as_stream(stream);
     const auto launch = [&](auto t) {
-        hipLaunchKernelGGL((sample_kernel<decltype(t)>), dim3((unsigned)rows), dim3(kSampleThreads), 0, st, a);
+        using T = decltype(t);
+        const dim3 each((unsigned)a.slices, (unsigned)rows), block(kSampleThreads);
+        if (need == 0) {
+            hipLaunchKernelGGL((sample_kernel<T, false>), dim3((unsigned)rows), block, 0, st, a);
+            return;
+        }
+        hipLaunchKernelGGL((sample_first_kernel<T>), each, block, 0, st, a);
+        // (without the filters there is nothing to bin)
+        if (top_k || top_p || (top_k_all > 0 && top_k_all < vocab) || top_p_all < 1.0f)
+            hipLaunchKernelGGL((sample_bins_kernel<T>), each, block, 0, st, a);
+        hipLaunchKernelGGL((sample_gather_kernel<T>), each, block, 0, st, a);
+        hipLaunchKernelGGL((sample_kernel<T, true>), dim3((unsigned)rows), block, 0, st, a);
     };
     if (type == MI_I32)
         launch(int32_t{});

@@ -71,7 +71,8 @@ SIGNATURES = {
                           P, I64, I64, I, I, I, I, I, I, P, SZ, P],
     "mi_pack_w4": [P, P, I, P, P, P, P, I, I, I, P],
     "mi_w4_matvec": [P, I64, I, P, P, I, P, P, P, I64, I, I, I, I, P],
-    "mi_sample_tokens": [P, I, I64, D, P, P, F, P, I, P, F, P, F, P, P, I, I, P],
+    "mi_sample_workspace_size": [I, I, P],
+    "mi_sample_tokens": [P, I, I64, D, P, P, F, P, I, P, F, P, F, P, P, I, I, P, SZ, P],
     "mi_adapter_workspace_size": [I, I, I, P],
     "mi_adapter_add": [P, I, I64, I64, P, P, P, I, P, P, P, P, I64, I64, P, I64, I64, I, I, I, I, I, I, I, P, SZ, P],
     "mi_gated_scan_sizes": [I, I, I, P, P, P],

@@ -492,7 +492,7 @@ def _calls():
         raise ImportError("the module of the float operators' calls is not built; build the library where torch, a C++ "
                           "compiler and Python's headers are") from e
     entries = ("mi_add_rms_norm", "mi_causal_conv", "mi_selective_scan_workspace_size", "mi_selective_scan",
-               "mi_w4_matvec", "mi_sample_tokens", "mi_adapter_workspace_size", "mi_adapter_add", "mi_gated_scan_sizes", "mi_gated_scan",
+               "mi_w4_matvec", "mi_sample_workspace_size", "mi_sample_tokens", "mi_adapter_workspace_size", "mi_adapter_add", "mi_gated_scan_sizes", "mi_gated_scan",
                "mi_gated_scan_backward", "mi_last_error_string")
     _float_calls.init(_lib.MIError, *(ctypes.cast(getattr(lib, e), ctypes.c_void_p).value for e in entries))
     return _float_calls

@@ -211,3 +211,15 @@ def test_refusals(cuda):
         ops.sample_tokens(x, u[:2])
     with pytest.raises(ValueError, match="forward only"):
         ops.sample_tokens(x.requires_grad_(), u)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_row_alone_and_among_many(cuda, dtype):
+    """Few rows are shared by several blocks, many are not: a row's token is the same."""
+    logits, _, u = make(5, 40000, dtype, 11, spread=0.7)
+    many = logits.repeat(120, 1)
+    for par in (dict(), dict(top_p=0.9), dict(top_k=300, top_p=0.8), dict(top_k=20000), dict(top_p=0.5, min_p=0.01), dict(min_p=0.3)):
+        got, lp = run(cuda, logits, u, **par)
+        check(logits, u, got, lp, **par)
+        all_, lps = run(cuda, many, u.repeat(120), **par)
+        assert torch.equal(all_, got.repeat(120)) and torch.equal(lps, lp.repeat(120))

@@ -13,8 +13,8 @@ A = ctypes.c_void_p(0x100000)     # never dereferenced: every call below fails v
 F, D = ctypes.c_float, ctypes.c_double
 
 
-def sample(x=A, t=0, ld=8, scale=1.0, u=A, ta=1.0, pa=1.0, ma=0.0, ids=A, B=2, V=8):
-    return ("mi_sample_tokens", x, t, ld, D(scale), u, None, F(ta), None, 0, None, F(pa), None, F(ma), ids, None, B, V, None)
+def sample(x=A, t=0, ld=8, scale=1.0, u=A, ta=1.0, pa=1.0, ma=0.0, ids=A, B=2, V=8, ws=None, wsb=0):
+    return ("mi_sample_tokens", x, t, ld, D(scale), u, None, F(ta), None, 0, None, F(pa), None, F(ma), ids, None, B, V, ws, wsb, None)
 
 
 @pytest.mark.parametrize("call,status,needle", [
@@ -22,7 +22,8 @@ def sample(x=A, t=0, ld=8, scale=1.0, u=A, ta=1.0, pa=1.0, ma=0.0, ids=A, B=2, V
     (sample(t=4), 4, "type"), (sample(t=-1), 4, "type"), (sample(ld=-8), 2, "stride"), (sample(scale=0.0), 4, "scale"),
     (sample(scale=math.nan), 4, "scale"), (sample(scale=math.inf), 4, "scale"), (sample(ta=math.nan), 4, "temperature"),
     (sample(pa=math.nan), 4, "top_p"), (sample(ma=math.nan), 4, "min_p"), (sample(x=None), 1, "required"),
-    (sample(u=None), 1, "required"), (sample(ids=None), 1, "required")])
+    (sample(u=None), 1, "required"), (sample(ids=None), 1, "required"), (sample(V=40000), 4, "workspace"),
+    (sample(V=40000, ws=A, wsb=99), 4, "workspace"), (sample(V=40000, ws=ctypes.c_void_p(0x100004), wsb=1 << 30), 3, "aligned")])
 def test_argument_validation(call, status, needle):
     from mamba_int import _lib
     assert _lib.raw(*call) == status and needle in _lib.last_error()
@@ -31,6 +32,17 @@ def test_argument_validation(call, status, needle):
 def test_no_rows_is_a_noop():
     from mamba_int import _lib
     assert _lib.raw(*sample(B=0, x=None, u=None, ids=None)) == 0
+
+
+def test_workspace_size():
+    from mamba_int import _lib
+    n = ctypes.c_size_t(9)
+    assert _lib.raw("mi_sample_workspace_size", 512, 100000, ctypes.byref(n)) == 0 and n.value == 0
+    assert _lib.raw("mi_sample_workspace_size", 3, 1000, ctypes.byref(n)) == 0 and n.value == 0
+    assert _lib.raw("mi_sample_workspace_size", 3, 100000, ctypes.byref(n)) == 0 and n.value > 0
+    assert _lib.raw("mi_sample_workspace_size", 3, 0, ctypes.byref(n)) == 2
+    assert _lib.raw("mi_sample_workspace_size", -3, 8, ctypes.byref(n)) == 2
+    assert _lib.raw("mi_sample_workspace_size", 3, 8, None) == 1
 
 
 def test_integers_stay_out_of_the_other_operators():
