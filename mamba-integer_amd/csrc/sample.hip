@@ -25,6 +25,7 @@ constexpr int kSampleBins = 2048;
 constexpr int kSampleNear = 256;            // candidates whose ranks are counted pairwise
 constexpr int kSampleList = 8192;           // candidates of a row that are listed
 constexpr int kSampleSlices = 64;           // of a row, at most
+constexpr int kSampleBlocks = 512;          // of the slices of all rows, at most
 constexpr int kSampleMaxVocab = 1 << 24;
 constexpr double kSampleRange = 40.0;       // e^-40 * 2^51 rounds to a mass of 0
 
@@ -47,6 +48,7 @@ struct SampleArgs {
 struct SampleShared {
     uint64_t best[kSampleSlices];            // the first of the order in a slice
     uint64_t slice_mass[kSampleSlices];      // the mass of a slice that is surely kept
+    uint64_t slice_bins[kSampleSlices][kSampleBins];      // top_p alone: a slice's masses
     uint64_t mass[kSampleBins];
     uint32_t count[kSampleBins];
     uint32_t found, unused;
@@ -96,11 +98,15 @@ __constant__ const double kExpTable[64] = {
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
 };
 
+struct alignas(16) Candidate {
+    uint64_t place, mass;
+};
+
 struct SampleLds {
     double table[64];
     uint32_t count[kSampleBins];
     uint64_t mass[kSampleBins];
-    uint64_t near[kSampleNear], near_mass[kSampleNear];
+    Candidate near[kSampleNear];
     uint64_t wave_mass[kSampleWaves], lo, hi, above_mass, last;
     uint32_t wave_count[kSampleWaves], above_count, found;
     int bin;
@@ -257,6 +263,17 @@ __device__ __forceinline__ void cut_bin(SampleLds &s, uint32_t count, uint64_t m
     __syncthreads();
 }
 
+// How many of the n candidates in LDS have a larger place than `mine`, and their mass.
+__device__ __forceinline__ void in_front(const SampleLds &s, int n, uint64_t mine, uint32_t &c, uint64_t &m) {
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+        const Candidate o = s.near[j];
+        const bool earlier = o.place > mine;
+        c += earlier ? 1u : 0u;
+        m += earlier ? o.mass : 0ull;
+    }
+}
+
 // Of n candidates in the order of their places, larger first: the place of the last one that
 // has fewer than `count` and less than `mass` in front of it (there is one: neither is 0).
 // visit(f) calls f(place, d) for each candidate, by all threads, in any order; no two places
@@ -317,20 +334,15 @@ __device__ __forceinline__ uint64_t cut_among(const SampleRow<T> &r, SampleLds &
         if (place < lo || place > hi) return;
         const uint32_t at = atomicAdd(&s.found, 1u);
         if (at < kSampleNear) {
-            s.near[at] = place;
-            s.near_mass[at] = by_mass ? r.mass(r.e(d)) : 0;
+            s.near[at] = {place, by_mass ? r.mass(r.e(d)) : 0};
         }
     });
     __syncthreads();
     if (tid < (int)n) {
-        const uint64_t mine = s.near[tid];
+        const uint64_t mine = s.near[tid].place;
         uint32_t c = 0;
         uint64_t m = 0;
-        for (int j = 0; j < (int)n; ++j) {
-            const bool earlier = s.near[j] > mine;
-            c += earlier ? 1u : 0u;
-            m += earlier ? s.near_mass[j] : 0ull;
-        }
+        in_front(s, (int)n, mine, c, m);
         if (c < count && m < mass) atomicMin((unsigned long long *)&s.last, (unsigned long long)mine);
     }
     __syncthreads();
@@ -396,9 +408,11 @@ __device__ __forceinline__ void scale_by(SampleRow<T> &r, const SampleArgs &a, u
 __device__ __forceinline__ SampleShared &shared_of(const SampleArgs &a, int64_t row) {
     return reinterpret_cast<SampleShared *>(a.workspace)[row];
 }
+// (a slice's a lane: one after the other they took a load's latency each)
 __device__ __forceinline__ uint64_t best_of(const SampleArgs &a, const SampleShared &g) {
-    uint64_t best = 0;
-    for (int i = 0; i < a.slices; ++i) best = more(best, g.best[i]);
+    const int lane = threadIdx.x & 63;
+    uint64_t best = lane < a.slices ? g.best[lane] : 0;
+    for (int o = 32; o > 0; o >>= 1) best = more(best, shfl_xor64(best, o));
     return best;
 }
 
@@ -452,7 +466,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_bins_kernel(SampleArgs 
     __syncthreads();
     for (int i = tid; i < kSampleBins; i += kSampleThreads) {
         if (s.count[i]) atomicAdd(&g.count[i], s.count[i]);
+        if (f.by_k) continue;
         if (s.mass[i]) atomicAdd((unsigned long long *)&g.mass[i], (unsigned long long)s.mass[i]);
+        g.slice_bins[slice][i] = s.mass[i];
     }
 }
 
@@ -493,6 +509,7 @@ __device__ __forceinline__ SampleCut cut_row(const SampleShared &g, SampleLds &s
 template <class T>
 __global__ __launch_bounds__(kSampleThreads) void sample_gather_kernel(SampleArgs a) {
     __shared__ SampleLds s;
+    __shared__ uint64_t own[kSampleList];      // the slice's candidates (a global counter for each took 52 us where this takes 14)
     const int64_t row = blockIdx.y;
     const int slice = blockIdx.x, tid = threadIdx.x;
     SampleShared &g = shared_of(a, row);
@@ -506,30 +523,80 @@ __global__ __launch_bounds__(kSampleThreads) void sample_gather_kernel(SampleArg
     SampleRow<T> r = sample_row<T>(a, s, row, slice * a.slice, min((slice + 1) * a.slice, a.vocab));
     scale_by(r, a, best, f.temperature);
     if (tid < 64) s.table[tid] = kExpTable[tid];
+    if (tid == 0) s.found = 0;
     __syncthreads();
     uint64_t sum = 0;
     const auto list = [&](Logit<T> v, int i) {
-        const uint32_t at = atomicAdd(&g.found, 1u);
-        if (at < kSampleList) g.list[at] = order_of(order_key(v), i);
+        const uint32_t at = atomicAdd(&s.found, 1u);
+        if (at < kSampleList) own[at] = order_of(order_key(v), i);
     };
     if (f.by_k)
         each_logit(r, [&](Logit<T> v, int i) {
             if (SampleRow<T>::bin(r.below(v)) <= c.bin) list(v, i);
         });
-    else
+    else if (f.by_p && !(f.least > 0.0f)) {
+        // (the bins in front of the cut are kept as they are)
+        for (int i = tid; i < c.bin; i += kSampleThreads) sum += g.slice_bins[slice][i];
+        each_logit(r, [&](Logit<T> v, int i) {
+            const double d = r.below(v);
+            if (SampleRow<T>::bin(d) == c.bin) list(v, i);
+        });
+    } else
         each_logit(r, [&](Logit<T> v, int i) {
             const double d = r.below(v);
             const int at = SampleRow<T>::bin(d);
             if (at > c.bin) return;
             const double e = r.e(d);
             if (at == c.bin) {
-                if (r.mass(e) != 0) list(v, i);      // (as the bins count)
+                list(v, i);
             } else if (e >= (double)f.least || !(f.least > 0.0f) || order_of(order_key(v), i) == best) {
                 sum += r.mass(e);
             }
         });
     sum = block_sum(s, sum);
-    if (tid == 0) g.slice_mass[slice] = sum;
+    const uint32_t n = s.found;
+    if (tid == 0) {
+        g.slice_mass[slice] = sum;
+        s.above_count = n ? atomicAdd(&g.found, n) : 0;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += kSampleThreads)
+        if (i < kSampleList && s.above_count + i < kSampleList) g.list[s.above_count + i] = own[i];
+}
+
+// The draw from the few candidates of a top_k, a thread each: its place among them and the
+// mass in front of it by looking at them all, in the order and then by token.
+template <class T>
+__device__ __forceinline__ void draw_listed(const SampleArgs &a, const SampleRow<T> &r, SampleLds &s, const SampleFilters &f, int64_t row,
+                                            const uint64_t *list, int n) {
+    const int tid = threadIdx.x;
+    uint64_t place = 0, mass = 0;
+    double d = 0.0, e = 0.0;
+    if (tid < n) {
+        place = list[tid];
+        d = r.below(value_of<Logit<T>>((uint32_t)(place >> 32)));
+        e = r.e(d);
+        mass = r.mass(e);
+        s.near[tid] = {place, mass};
+    }
+    __syncthreads();
+    uint32_t c = 0;
+    uint64_t m = 0;
+    if (tid < n) in_front(s, n, place, c, m);
+    const bool in_k = tid < n && c < (uint32_t)f.k;
+    const uint64_t sum = block_sum(s, in_k ? mass : 0);
+    const bool keep = in_k && (!f.by_p || m < f.mass_of(sum)) && (e >= (double)f.least || c == 0 || !(f.least > 0.0f));
+    if (!keep) mass = 0;
+    if (tid < n) s.near[tid] = {(uint64_t)(uint32_t)place, mass};      // (the complement of the token)
+    const uint64_t total = block_sum(s, mass);
+    const double at = (double)a.u[row] * (double)total;
+    const uint64_t target = at > 0.0 ? less((uint64_t)fmin(at, 9e18), total - 1) : (uint64_t)0;
+    m = 0;
+    if (tid < n) in_front(s, n, (uint64_t)(uint32_t)place, c, m);
+    if (m <= target && target < m + mass) {
+        a.ids[row] = token_of(place);
+        if (a.logprob) a.logprob[row] = (float)(d - log((double)total / r.unit));
+    }
 }
 
 // A block a row: all of it, or after the kernels above.
@@ -600,10 +667,17 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     bool by_slices = SLICES;       // the row's mass is known by slices, but for the listed tokens
     if (SLICES && (f.by_k || f.by_p)) {
         const SampleCut c = cut_row(g, s, f);
-        by_slices = !c.whole && !f.by_k;
-        if (!c.whole) {
+        // (top_p's bin is listed with the tokens in it that have no mass, which the bins do not count)
+        const uint32_t found = f.by_k ? c.listed : g.found;
+        const bool whole = c.whole || found > kSampleList;
+        by_slices = !whole && !f.by_k;
+        if (!whole) {
             listed = g.list;
-            n_listed = c.listed;
+            n_listed = found;
+            if (f.by_k && n_listed <= kSampleNear) {
+                draw_listed(a, r, s, f, row, g.list, (int)n_listed);
+                return;
+            }
             if (f.by_k) {
                 const uint32_t n = s.count[c.bin];
                 threshold = cut_among(r, s, n, (uint32_t)f.k - (c.listed - n), ~0ull, [&](auto &&fn) {
@@ -613,7 +687,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
                 });
                 if (f.by_p) cut_mass();
             } else {
-                threshold = cut_among(r, s, c.listed, ~0u, c.mass, in_list);
+                threshold = cut_among(r, s, c.listed, ~0u, c.mass, [&](auto &&fn) {
+                    in_list([&](uint64_t place, double d) {
+                        if (r.mass(r.e(d)) != 0) fn(place, d);
+                    });
+                });
             }
         }
     }
@@ -743,10 +821,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     });
 }
 
-// Slices of a row: 4096 tokens or more, and at most 512 blocks of all rows.
+// Slices of a row: of 8192 tokens or so (each block has the row's bins to read first: 64 rows
+// of 32000 in slices of 4000 49 us, of 8000 42), 512 blocks at most.
 inline int sample_slices(int rows, int vocab) {
-    const int n = std::min((vocab + 4095) / 4096, kSampleSlices);
-    return std::max(1, std::min(n, 512 / std::max(rows, 1)));
+    const int n = std::min((vocab + 8191) / 8192, kSampleSlices);
+    return std::max(1, std::min(n, kSampleBlocks / std::max(rows, 1)));
 }
 
 }  // namespace mi
