@@ -13,6 +13,15 @@ exponential decays, SiLU) on BitLinear projections, with a head in 4-bit weights
     ...
     logits = W4 rms_norm(r + x)                        ops.add_rms_norm, ops.w4_matvec
 
+A layer may have a gated linear recurrence in the scan's place, one state a channel:
+
+    [r | i] = BitLinear(u)                             ops.bitlinear_f32
+    y = gated scan(u, r, i, decay) * silu(z)           ops.gated_scan
+
+Requests of one batch may each have a low-rank adapter beside the input and output
+projections (``Adapters``, ops.adapter_add) and draw their tokens with parameters of
+their own (``Sampling``, ops.sample_tokens).
+
 The residual r and every row between the kernels is float32.  Prompts of unequal
 lengths run as one padded batch; the state of a sequence is its last conv inputs and
 its scan state, and a decode step is the same path over one token.
@@ -23,14 +32,16 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import List, Optional, Tuple
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import ops
 from .params import ModelDims
+from .sampling import Sampling
 
 HEAD_GROUP = 64      # weights of the head that share a scale
+GATED_RATE = 8.0     # of a gated layer's log decay
 
 
 @dataclass
@@ -56,17 +67,41 @@ class SelectiveLayer:
 
 
 @dataclass
+class GatedLayer:
+    norm: torch.Tensor        # float32 [d_model]
+    w_in: Projection          # d_model -> 2 d_inner: [u | z]
+    conv_w: torch.Tensor      # float32 [d_inner, width]
+    conv_b: torch.Tensor
+    w_gates: Projection       # d_inner -> 2 d_inner: [r | i]
+    decay: torch.Tensor       # float32 [d_inner]
+    w_out: Projection         # d_inner -> d_model
+
+
+@dataclass
+class Adapters:
+    """Low-rank adapters of a model: for every layer the bank beside w_in, (a [bank, rank, d_model],
+    b [bank, 2 d_inner, rank]), and the one beside w_out, (a [bank, rank, d_inner], b [bank, d_model,
+    rank]), either may be None; scales float32 [bank] (None: 1).  ``ids`` int32 [B]: each
+    sequence's adapter, outside [0, bank) for none."""
+    w_in: List[Optional[Tuple[torch.Tensor, torch.Tensor]]]
+    w_out: List[Optional[Tuple[torch.Tensor, torch.Tensor]]]
+    ids: torch.Tensor
+    scales: Optional[torch.Tensor] = None
+
+
+@dataclass
 class SelectiveParams:
     dims: ModelDims
     emb: torch.Tensor         # float32 [vocab, d_model]
-    layers: List[SelectiveLayer]
+    layers: List[Union[SelectiveLayer, GatedLayer]]
     norm_f: torch.Tensor
     head: Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]   # ops.pack_w4's [vocab, d_model]
 
 
 @dataclass
 class SelectiveState:
-    """Per layer: the last conv inputs float32 [B, width - 1, d_inner], scan state float32 [B, d_inner, d_state]."""
+    """Per layer: the last conv inputs float32 [B, width - 1, d_inner], scan state float32 [B, d_inner, d_state]
+    ([B, d_inner] of a gated layer)."""
     conv: List[torch.Tensor]
     h: List[torch.Tensor]
 
@@ -96,9 +131,10 @@ def quantize_w4(w: torch.Tensor, group: int = HEAD_GROUP):
     return ops.pack_w4(codes, scale, group, zeros=zero.to(torch.uint8))
 
 
-def random_params(dims: ModelDims, seed: int, device: str = "cuda", width: int = 4) -> SelectiveParams:
+def random_params(dims: ModelDims, seed: int, device: str = "cuda", width: int = 4, gated: Sequence[int] = ()) -> SelectiveParams:
     """A synthetic model: normal weights (quantized as above), steps between 0.001 and 0.1
-    at dt = 0, decays of 1 .. d_state."""
+    at dt = 0, decays of 1 .. d_state.  ``gated``: the layers with the gated recurrence,
+    whose channels' decays lie between 0.9 and 0.999 where the gate is open."""
     g = torch.Generator(device=device)
     g.manual_seed(seed)
     d, D, N, R = dims.d_model, dims.d_inner, dims.d_state, dims.dt_rank
@@ -107,7 +143,15 @@ def random_params(dims: ModelDims, seed: int, device: str = "cuda", width: int =
         return torch.randn(shape, generator=g, device=device)
 
     layers = []
-    for _ in range(dims.n_layer):
+    for i in range(dims.n_layer):
+        if i in gated:
+            a = 0.9 + 0.099 * torch.rand(D, generator=g, device=device)
+            layers.append(GatedLayer(
+                norm=torch.ones(d, device=device), w_in=ternary(randn(2 * D, d) / math.sqrt(d)),
+                conv_w=randn(D, width) / math.sqrt(width), conv_b=0.1 * randn(D),
+                w_gates=ternary(randn(2 * D, D) / math.sqrt(D)), decay=torch.log(torch.expm1(-torch.log(a) / GATED_RATE)),
+                w_out=ternary(randn(d, D) / math.sqrt(D * 2 * dims.n_layer))))
+            continue
         step = torch.exp(torch.rand(D, generator=g, device=device) * math.log(100.0) + math.log(1e-3))
         layers.append(SelectiveLayer(
             norm=torch.ones(d, device=device), w_in=ternary(randn(2 * D, d) / math.sqrt(d)),
@@ -135,13 +179,16 @@ class SelectiveRunner:
         D, N = self.dims.d_inner, self.dims.d_state
         width = self.params.layers[0].conv_w.shape[1]
         return SelectiveState([torch.zeros((batch, width - 1, D), device=self.device) for _ in self.params.layers],
-                              [torch.zeros((batch, D, N), device=self.device) for _ in self.params.layers])
+                              [torch.zeros((batch, D) if isinstance(ly, GatedLayer) else (batch, D, N), device=self.device)
+                               for ly in self.params.layers])
 
     @torch.no_grad()
-    def forward(self, ids: torch.Tensor, state: SelectiveState, lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def forward(self, ids: torch.Tensor, state: SelectiveState, lens: Optional[torch.Tensor] = None,
+                adapters: Optional[Adapters] = None) -> torch.Tensor:
         """Logits float32 [B, vocab] of each sequence's last token; ids int64 [B, L], state is
         updated in place.  lens int32 [B]: tokens of each sequence, taken as within [0, L] (the
-        rest of its row is padding); one of no tokens has logits of zero."""
+        rest of its row is padding); one of no tokens has logits of zero.  ``adapters``: each
+        sequence's own beside the projections."""
         B, L = ids.shape
         if L < 1:
             raise ValueError("ids must hold at least one token a sequence")
@@ -154,14 +201,27 @@ class SelectiveRunner:
             else:
                 q, s, _ = ops.add_rms_norm_quant(x, ly.norm, residual=r, residual_out=r)
             uz = ops.bitlinear(q, ly.w_in.packed, ops.OUT_FLOAT, 2 * D, x_scale=s, w_scale=ly.w_in.scale).view(B, L, 2 * D)
+            if adapters is not None and adapters.w_in[i] is not None:
+                a, b = adapters.w_in[i]
+                ops.adapter_add(uz, q.view(B, L, -1)[..., :dims.d_model], a, b, adapters.ids, scales=adapters.scales,
+                                x_scale=s.view(B, L), lens=lens, out=uz)
             u = ops.causal_conv(uz[..., :D], ly.conv_w, bias=ly.conv_b, state_in=state.conv[i], state_out=state.conv[i],
                                 lens=lens)
-            xp = ops.bitlinear_f32(u.view(B * L, D), ly.w_x.packed, ly.w_x.scale)
-            dt = ops.bitlinear_f32(xp[:, :R].contiguous(), ly.w_dt.packed, ly.w_dt.scale).view(B, L, D)
-            xp = xp.view(B, L, R + 2 * N)
-            y = ops.selective_scan(u, dt, ly.a, xp[..., R:R + N], xp[..., R + N:], d_skip=ly.d, z=uz[..., D:],
-                                   dt_bias=ly.dt_bias, h_in=state.h[i], h_out=state.h[i], lens=lens)
+            if isinstance(ly, GatedLayer):
+                ri = ops.bitlinear_f32(u.view(B * L, D), ly.w_gates.packed, ly.w_gates.scale).view(B, L, 2 * D)
+                y = ops.gated_scan(u, ri[..., :D], ri[..., D:], ly.decay, z=uz[..., D:], rate=GATED_RATE, h_in=state.h[i],
+                                   h_out=state.h[i], lens=lens)
+            else:
+                xp = ops.bitlinear_f32(u.view(B * L, D), ly.w_x.packed, ly.w_x.scale)
+                dt = ops.bitlinear_f32(xp[:, :R].contiguous(), ly.w_dt.packed, ly.w_dt.scale).view(B, L, D)
+                xp = xp.view(B, L, R + 2 * N)
+                y = ops.selective_scan(u, dt, ly.a, xp[..., R:R + N], xp[..., R + N:], d_skip=ly.d, z=uz[..., D:],
+                                       dt_bias=ly.dt_bias, h_in=state.h[i], h_out=state.h[i], lens=lens)
             x = ops.bitlinear_f32(y.view(B * L, D), ly.w_out.packed, ly.w_out.scale)
+            if adapters is not None and adapters.w_out[i] is not None:
+                a, b = adapters.w_out[i]
+                rows = x.view(B, L, -1)
+                ops.adapter_add(rows, y, a, b, adapters.ids, scales=adapters.scales, lens=lens, out=rows)
         # a row of its own sequence, whatever lens holds
         last = (lens.clamp(1, L).long() if lens is not None else torch.full((B,), L, device=self.device)) - 1
         rows = last + L * torch.arange(B, device=self.device)
@@ -172,14 +232,16 @@ class SelectiveRunner:
         return ops.w4_matvec(y, packed, scales, dims.vocab_size, HEAD_GROUP, zeros=zeros)
 
     @torch.no_grad()
-    def generate(self, ids: torch.Tensor, steps: int, lens: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Greedy tokens int64 [B, steps] after the prompts."""
+    def generate(self, ids: torch.Tensor, steps: int, lens: Optional[torch.Tensor] = None, sampling: Optional[Sampling] = None,
+                 adapters: Optional[Adapters] = None) -> torch.Tensor:
+        """Tokens int64 [B, steps] after the prompts: the largest logit's, or drawn as ``sampling``
+        says."""
         state = self.new_state(ids.shape[0])
-        out, logits = [], self.forward(ids, state, lens)
+        out, logits = [], self.forward(ids, state, lens, adapters)
         for i in range(steps):
-            out.append(logits.argmax(-1, keepdim=True))
+            out.append((sampling.draw(logits) if sampling is not None else logits.argmax(-1)).unsqueeze(-1))
             if i + 1 < steps:
-                logits = self.forward(out[-1], state)
+                logits = self.forward(out[-1], state, adapters=adapters)
         return torch.cat(out, 1) if out else ids.new_empty((ids.shape[0], 0))
 
 

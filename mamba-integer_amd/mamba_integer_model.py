@@ -34,6 +34,7 @@ from mamba_int import checkpoint, ops
 from mamba_int.model import IntegerMambaRunner
 from mamba_int.params import (DECAY_SHIFT, LayerParams, ModelDims, ModelParams,
                               init_random_params, requant_shift, synthetic_out_clamp)
+from mamba_int.sampling import Sampling
 
 
 class DyadicScanFunction:
@@ -276,10 +277,20 @@ class MambaIntegerModel(nn.Module):
         return self.runner(input_ids.device).forward_float(input_ids, self.logit_scale)
 
     @torch.no_grad()
-    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, use_graph: bool = True) -> torch.Tensor:
-        """Greedy generation: returns input_ids extended by max_new_tokens ids."""
-        new = self.runner(input_ids.device).generate(input_ids, max_new_tokens, use_graph=use_graph)
-        return torch.cat([input_ids, new], dim=1)
+    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, use_graph: bool = True,
+                 sampling: Optional[Sampling] = None) -> torch.Tensor:
+        """Returns input_ids extended by max_new_tokens ids: the largest logits', or drawn from the
+        logits as ``sampling`` says, step by step (the reference draws at a temperature of 0.8,
+        ``scripts/inference.py:157-158``)."""
+        runner = self.runner(input_ids.device)
+        if sampling is None or max_new_tokens == 0:
+            new = runner.generate(input_ids, max_new_tokens, use_graph=use_graph)
+            return torch.cat([input_ids, new], dim=1)
+        logits, state = runner.prefill(input_ids)
+        new = [sampling.draw(logits, self.logit_scale)]
+        while len(new) < max_new_tokens:
+            new.append(sampling.draw(runner.decode_step(new[-1], state), self.logit_scale))
+        return torch.cat([input_ids, torch.stack(new, dim=1)], dim=1)
 
 
 __all__ = ["MambaIntegerModel", "MambaIntegerBlock", "MambaIntegerBlockV2", "BitShiftNorm", "BitShiftNormV2",
