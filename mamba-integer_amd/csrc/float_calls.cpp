@@ -14,11 +14,14 @@
 #include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include <stdarg.h>
+
+#include <array>
 
 #include "mamba_int.h"
 
@@ -484,54 +487,149 @@ struct Gated {
     }
 };
 
-// (stream, x, r, i, decay, z, rate, h_in, h_out, lens, out, save): y, or (y, what the backward pass reads)
+// (stream, x, r, i, decay, z, rate, h_in, h_out, lens, out): y, or None where autograd records an input
 PyObject *gated_scan(PyObject *const *a, Py_ssize_t n) {
-    count(n, 12, "gated_scan");
+    count(n, 11, "gated_scan");
     void *stream = stream_of(a[0]);
+    if (c10::GradMode::is_enabled())
+        for (const int k : {1, 2, 3, 4, 5, 7})
+            if (THPVariable_Check(a[k]) && THPVariable_Unpack(a[k]).requires_grad()) Py_RETURN_NONE;
     const Gated g(a[1], a[2], a[3], a[4], a[5], a[6], a[9]);
     const Tensor &x = THPVariable_Unpack(a[1]);
     const float *h_in = vec<float>(a[7], {g.B, g.D}, at::kFloat, "h_in");
     float *h_out = vec<float>(a[8], {g.B, g.D}, at::kFloat, "h_out");
-    const bool save = a[11] == Py_True;
     Ref y(output(a[10], x.sizes(), x));
     const Rows yr = rows(y.p, x.sizes(), g.type, "out", true);
-    Ref saved(save ? empty({(int64_t)(g.saved_bytes / sizeof(float))}, x, at::kFloat) : (Py_INCREF(Py_None), Py_None));
     Tensor ws;
     if (g.forward_bytes) ws = at::empty({(int64_t)g.forward_bytes}, x.options().dtype(at::kByte));
     check("mi_gated_scan",
           g_gated(g.x.p, g.x.ld, g.x.bs, g.r.p, g.r.ld, g.r.bs, g.i.p, g.i.ld, g.i.bs, g.decay, g.rate, g.z.p, g.z.ld, g.z.bs, h_in,
-                  h_out, g.lens, yr.p, yr.ld, yr.bs, save ? static_cast<float *>(THPVariable_Unpack(saved.p).data_ptr()) : nullptr,
-                  g.code, g.bi, g.li, g.di, g.forward_bytes ? ws.data_ptr() : nullptr, g.forward_bytes, stream));
+                  h_out, g.lens, yr.p, yr.ld, yr.bs, nullptr, g.code, g.bi, g.li, g.di, g.forward_bytes ? ws.data_ptr() : nullptr,
+                  g.forward_bytes, stream));
     written(a[8]);
     written(a[10]);
-    return save ? Py_BuildValue("(NN)", y.release(), saved.release()) : y.release();
+    return y.release();
 }
 
-// (stream, dy, x, r, i, decay, z, rate, lens, saved, needs): the gradients of x, r, i, decay, z and
-// h_in, None where `needs`, a tuple of six truth values, has a false one.
-PyObject *gated_scan_backward(PyObject *const *a, Py_ssize_t n) {
-    count(n, 11, "gated_scan_backward");
+// ------------------------------------------------ the gated recurrence under autograd
+// In C++ on both sides: through Python the two passes of a small training step took 60 us of
+// host time more than their kernels.  Nothing below touches Python (the backward pass runs on
+// the engine's threads); what is wrong raises a C++ error, which torch hands on.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void require(mi_status st, const char *fn) {
+    TORCH_CHECK(st == MI_OK, fn, " failed with status ", (int)st, ": ", g_last_error());
+}
+Rows rows_of(const Tensor &t) { return t.defined() ? Rows{t.data_ptr(), t.stride(1), t.stride(0)} : Rows{}; }
+int code_of(const Tensor &t) { return t.scalar_type() == at::kFloat ? MI_F32 : t.scalar_type() == at::kBFloat16 ? MI_BF16 : MI_F16; }
+Tensor bytes_of(size_t n, const Tensor &like) {
+    return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
+}
+void *pointer(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+using Maybe = std::optional<Tensor>;
+Maybe maybe(const Tensor &t) { return t.defined() ? Maybe(t) : std::nullopt; }
+
+// What was recorded, of tensors that the call has checked; `stream`: a backward pass runs on the
+// forward pass's.
+variable_list gated_gradients(const Tensor &grad, const variable_list &in, double rate, int64_t stream, const std::array<bool, 6> &needs) {
+    const Tensor &x = in[0], &r = in[1], &i = in[2], &decay = in[3], &z = in[4], &lens = in[5], &saved = in[6];
+    // (contiguous() keeps an empty tensor's strides)
+    const Tensor dy = grad.stride(2) != 1 || grad.is_neg() ? grad.clone(at::MemoryFormat::Contiguous) : grad;
+    const int B = (int)x.size(0), L = (int)x.size(1), D = (int)x.size(2);
+    size_t forward = 0, backward = 0, keep = 0;
+    require(g_gated_sizes(B, L, D, &forward, &backward, &keep), "mi_gated_scan_sizes");
+    const auto like_x = [&](bool on) { return on ? at::empty(x.sizes(), x.options()) : Tensor(); };
+    const auto floats = [&](bool on, at::IntArrayRef shape) { return on ? at::empty(shape, x.options().dtype(at::kFloat)) : Tensor(); };
+    variable_list out{like_x(needs[0]),       like_x(needs[1]), like_x(needs[2]), floats(needs[3], {x.size(2)}), like_x(needs[4]),
+                      floats(needs[5], {x.size(0), x.size(2)})};
+    const Tensor ws = bytes_of(backward, x);
+    const Rows dr = rows_of(dy), xr = rows_of(x), rr = rows_of(r), ir = rows_of(i), zr = rows_of(z);
+    require(g_gated_backward(dr.p, dr.ld, dr.bs, xr.p, xr.ld, xr.bs, rr.p, rr.ld, rr.bs, ir.p, ir.ld, ir.bs,
+                             static_cast<const float *>(decay.data_ptr()), (float)rate, zr.p, zr.ld, zr.bs,
+                             static_cast<const int32_t *>(pointer(lens)), static_cast<const float *>(saved.data_ptr()), pointer(out[0]),
+                             pointer(out[1]), pointer(out[2]), pointer(out[4]), static_cast<float *>(pointer(out[3])),
+                             static_cast<float *>(pointer(out[5])), code_of(x), B, L, D, pointer(ws), backward,
+                             reinterpret_cast<void *>(stream)),
+            "mi_gated_scan_backward");
+    return out;
+}
+
+// The gradients as a node whose own gradient is an error: a second derivative that leaves this
+// part out would be wrong without one.
+struct GatedGradients : torch::autograd::Function<GatedGradients> {
+    static variable_list forward(AutogradContext *, const Tensor &dy, const Tensor &x, const Tensor &r, const Tensor &i,
+                                 const Tensor &decay, const Maybe &z, const Maybe &lens, const Tensor &saved, double rate,
+                                 int64_t stream, std::array<bool, 6> needs) {
+        variable_list out;      // (those there are)
+        for (const Tensor &v : gated_gradients(dy, {x, r, i, decay, z.value_or(Tensor()), lens.value_or(Tensor()), saved}, rate, stream, needs))
+            if (v.defined()) out.push_back(v);
+        return out;
+    }
+    static variable_list backward(AutogradContext *, const variable_list &) { TORCH_CHECK(false, "gated_scan is differentiable once"); }
+};
+
+struct GatedScan : torch::autograd::Function<GatedScan> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &r, const Tensor &i, const Tensor &decay, const Maybe &gate,
+                          const Maybe &first, const Maybe &lengths, double rate, int64_t stream) {
+        const Tensor z = gate.value_or(Tensor()), h_in = first.value_or(Tensor()), lens = lengths.value_or(Tensor());
+        const int B = (int)x.size(0), L = (int)x.size(1), D = (int)x.size(2);
+        size_t forward = 0, backward = 0, keep = 0;
+        require(g_gated_sizes(B, L, D, &forward, &backward, &keep), "mi_gated_scan_sizes");
+        const Tensor y = at::empty(x.sizes(), x.options()), saved = at::empty({(int64_t)(keep / sizeof(float))}, x.options().dtype(at::kFloat)),
+                     ws = bytes_of(forward, x);
+        const Rows xr = rows_of(x), rr = rows_of(r), ir = rows_of(i), zr = rows_of(z), yr = rows_of(y);
+        require(g_gated(xr.p, xr.ld, xr.bs, rr.p, rr.ld, rr.bs, ir.p, ir.ld, ir.bs, static_cast<const float *>(decay.data_ptr()),
+                        (float)rate, zr.p, zr.ld, zr.bs, static_cast<const float *>(pointer(h_in)), nullptr,
+                        static_cast<const int32_t *>(pointer(lens)), yr.p, std::max(yr.ld, x.size(2)), yr.bs,
+                        static_cast<float *>(saved.data_ptr()), code_of(x), B, L, D, pointer(ws), forward, reinterpret_cast<void *>(stream)),
+                "mi_gated_scan");
+        ctx->save_for_backward({x, r, i, decay, z, lens, saved});
+        ctx->saved_data["rate"] = rate;
+        ctx->saved_data["stream"] = stream;
+        ctx->saved_data["state"] = h_in.defined();
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        variable_list out(9);
+        if (!grads[0].defined()) return out;
+        const variable_list in = ctx->get_saved_variables();
+        const double rate = ctx->saved_data["rate"].toDouble();
+        const int64_t stream = ctx->saved_data["stream"].toInt();
+        // (tensors that were not given are not counted among the node's inputs)
+        const bool z = in[4].defined(), state = ctx->saved_data["state"].toBool();
+        const std::array<bool, 6> needs{ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2),
+                                        ctx->needs_input_grad(3), z && ctx->needs_input_grad(4),
+                                        state && ctx->needs_input_grad(z ? 5 : 4)};
+        if (!c10::GradMode::is_enabled()) {
+            const variable_list got = gated_gradients(grads[0], in, rate, stream, needs);
+            std::copy(got.begin(), got.end(), out.begin());
+            return out;
+        }
+        const variable_list got =
+            GatedGradients::apply(grads[0], in[0], in[1], in[2], in[3], maybe(in[4]), maybe(in[5]), in[6], rate, stream, needs);
+        for (int k = 0, at = 0; k < 6; ++k)
+            if (needs[k]) out[k] = got[at++];
+        return out;
+    }
+};
+
+// (stream, x, r, i, decay, z, rate, h_in, lens): y, recorded
+PyObject *gated_scan_recorded(PyObject *const *a, Py_ssize_t n) {
+    count(n, 9, "gated_scan_recorded");
     void *stream = stream_of(a[0]);
-    const Gated g(a[2], a[3], a[4], a[5], a[6], a[7], a[8]);
-    const Tensor &x = THPVariable_Unpack(a[2]);
-    const Rows dy = rows(a[1], x.sizes(), g.type, "dy");
-    const float *saved = vec<float>(a[9], {(int64_t)(g.saved_bytes / sizeof(float))}, at::kFloat, "saved");
-    if (!PyTuple_Check(a[10]) || PyTuple_GET_SIZE(a[10]) != 6) raise(PyExc_TypeError, "needs must be a tuple of six");
-    const int64_t row[1] = {g.D}, state[2] = {g.B, g.D};
-    const auto grad = [&](int k, at::IntArrayRef shape, at::ScalarType type) {
-        return PyTuple_GET_ITEM(a[10], k) == Py_True ? empty(shape, x, type) : (Py_INCREF(Py_None), Py_None);
-    };
-    Ref dx(grad(0, x.sizes(), g.type)), dr(grad(1, x.sizes(), g.type)), di(grad(2, x.sizes(), g.type)), dd(grad(3, row, at::kFloat)),
-        dz(grad(4, x.sizes(), g.type)), dh(grad(5, state, at::kFloat));
-    const auto at_ = [](const Ref &t) { return t.p == Py_None ? nullptr : THPVariable_Unpack(t.p).data_ptr(); };
-    Tensor ws;
-    if (g.backward_bytes) ws = at::empty({(int64_t)g.backward_bytes}, x.options().dtype(at::kByte));
-    check("mi_gated_scan_backward",
-          g_gated_backward(dy.p, dy.ld, dy.bs, g.x.p, g.x.ld, g.x.bs, g.r.p, g.r.ld, g.r.bs, g.i.p, g.i.ld, g.i.bs, g.decay, g.rate,
-                           g.z.p, g.z.ld, g.z.bs, g.lens, saved, at_(dx), at_(dr), at_(di), at_(dz), static_cast<float *>(at_(dd)),
-                           static_cast<float *>(at_(dh)), g.code, g.bi, g.li, g.di, g.backward_bytes ? ws.data_ptr() : nullptr,
-                           g.backward_bytes, stream));
-    return Py_BuildValue("(NNNNNN)", dx.release(), dr.release(), di.release(), dd.release(), dz.release(), dh.release());
+    double rate;
+    {
+        const c10::AutoGradMode none(false);
+        const Gated g(a[1], a[2], a[3], a[4], a[5], a[6], a[8]);
+        vec<float>(a[7], {g.B, g.D}, at::kFloat, "h_in");
+        rate = PyFloat_AsDouble(a[6]);
+    }
+    const auto some = [](PyObject *o) { return o == Py_None ? Maybe() : Maybe(THPVariable_Unpack(o)); };
+    return THPVariable_Wrap(GatedScan::apply(THPVariable_Unpack(a[1]), THPVariable_Unpack(a[2]), THPVariable_Unpack(a[3]),
+                                             THPVariable_Unpack(a[4]), some(a[5]), some(a[7]), some(a[8]), rate,
+                                             reinterpret_cast<int64_t>(stream)));
 }
 
 // (stream, name, tensor): raises where the tensor is a leaf whose gradient another live graph
@@ -583,6 +681,8 @@ PyObject *guarded(PyObject *, PyObject *const *a, Py_ssize_t n) {
     try {
         return F(a, n);
     } catch (const Raised &) {
+    } catch (const c10::Error &e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
     } catch (const std::exception &e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
     } catch (...) {
@@ -593,7 +693,7 @@ PyObject *guarded(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 #define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<f>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(init),           METHOD(add_rms_norm), METHOD(causal_conv),
-                         METHOD(selective_scan), METHOD(w4_matvec),    METHOD(sample_tokens), METHOD(adapter_add), METHOD(gated_scan), METHOD(gated_scan_backward), METHOD(check_accumulator), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(selective_scan), METHOD(w4_matvec),    METHOD(sample_tokens), METHOD(adapter_add), METHOD(gated_scan), METHOD(gated_scan_recorded), METHOD(check_accumulator), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_float_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

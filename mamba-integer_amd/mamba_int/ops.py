@@ -617,38 +617,6 @@ def adapter_add(y, x, a, b, ids, scales=None, x_scale=None, lens=None, out=None)
     return _calls().adapter_add(_here(), y, x, a, b, ids, scales, x_scale, lens, out)
 
 
-class _GatedScanGrad(torch.autograd.Function):
-    """gated_scan's gradients, as a node whose own gradient is an error: a second derivative
-    that leaves this part out would be wrong without one."""
-
-    @staticmethod
-    def forward(ctx, dy, x, r, i, decay, z, rate, lens, saved, needs):
-        return _calls().gated_scan_backward(_here(), dy, x, r, i, decay, z, rate, lens, saved, needs)
-
-    @staticmethod
-    def backward(ctx, *_):
-        raise RuntimeError("gated_scan is differentiable once")
-
-
-class _GatedScan(torch.autograd.Function):
-    """gated_scan while autograd records."""
-
-    @staticmethod
-    def forward(ctx, x, r, i, decay, z, h_in, rate, lens):
-        y, saved = _calls().gated_scan(_here(), x, r, i, decay, z, rate, h_in, None, lens, None, True)
-        ctx.save_for_backward(x, r, i, decay, z, lens, saved)
-        ctx.rate = rate
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, r, i, decay, z, lens, saved = ctx.saved_tensors
-        if dy.stride(-1) != 1 or dy.is_neg():
-            dy = dy.clone(memory_format=torch.contiguous_format)    # (contiguous() keeps an empty tensor's strides)
-        grads = _GatedScanGrad.apply(dy, x, r, i, decay, z, ctx.rate, lens, saved, ctx.needs_input_grad[:6])
-        return (*grads, None, None)
-
-
 def gated_scan(x, r, i, decay, z=None, rate: float = 8.0, h_in=None, h_out=None, lens=None, out=None):
     """Gated linear recurrence: with s = sigmoid(r), a = exp(-rate * softplus(decay) * s),
     h = a * h + sqrt(1 - a^2) * sigmoid(i) * x,  y = h (* silu(z)).
@@ -659,14 +627,14 @@ def gated_scan(x, r, i, decay, z=None, rate: float = 8.0, h_in=None, h_out=None,
     Differentiable, once, in x, r, i, decay, z and h_in; while autograd records one of them,
     out and h_out cannot be given.  In a graph's capture no other live graph may hold such a
     leaf from another stream."""
-    if torch.is_grad_enabled():
-        leaves = [(n, t) for n, t in (("x", x), ("r", r), ("i", i), ("decay", decay), ("z", z), ("h_in", h_in))
-                  if isinstance(t, torch.Tensor) and t.requires_grad]
-        if leaves:
-            if out is not None or h_out is not None:
-                raise ValueError("out and h_out cannot be given while autograd records the inputs")
-            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-                for n, t in leaves:
-                    _calls().check_accumulator(_here(), n, t)
-            return _GatedScan.apply(x, r, i, decay, z, h_in, rate, lens)
-    return _calls().gated_scan(_here(), x, r, i, decay, z, rate, h_in, h_out, lens, out, False)
+    y = _calls().gated_scan(_here(), x, r, i, decay, z, rate, h_in, h_out, lens, out)
+    if y is not None:
+        return y
+    # autograd records an input
+    if out is not None or h_out is not None:
+        raise ValueError("out and h_out cannot be given while autograd records the inputs")
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        for name, t in (("x", x), ("r", r), ("i", i), ("decay", decay), ("z", z), ("h_in", h_in)):
+            if isinstance(t, torch.Tensor):
+                _calls().check_accumulator(_here(), name, t)
+    return _calls().gated_scan_recorded(_here(), x, r, i, decay, z, rate, h_in, lens)
