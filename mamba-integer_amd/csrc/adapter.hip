@@ -295,7 +295,7 @@ template <class Y, class W, int KS, int NT, int UT>
 __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
     constexpr int PAIR = sizeof(Y) == 4 ? 1 : 2, V = 4 * PAIR;
     const int b = blockIdx.z, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int id = adapter_of(a, b), tokens = id < 0 ? 0 : tokens_of(a, b), t0 = (int)blockIdx.y * a.up_tokens;
+    const int id = adapter_of(a, b), tokens = id < 0 || a.rank == 0 ? 0 : tokens_of(a, b), t0 = (int)blockIdx.y * a.up_tokens;
     const int n0 = ((int)blockIdx.x * 4 + wave_id()) * 16 * NT;
     const bool in_place = a.out == a.y;
     if (n0 >= a.n || (in_place && t0 >= tokens)) return;

@@ -85,7 +85,7 @@ void gated() {
 void adapter() {
     Pool p;
     const int t = uni(0, 2), w = uni(0, 2), ew = w ? 2 : 4, xt = uni(0, 2) ? t : 4, ex = xt == 4 ? 1 : xt ? 2 : 4, e = t ? 2 : 4;
-    const int B = logu(1, 6), L = uni(0, 1) ? 1 : logu(1, 90), K = logu(1, 700), N = logu(1, 600), R = uni(0, 4) ? logu(1, 40) : uni(0, 128),
+    const int B = logu(1, 6), L = uni(0, 1) ? 1 : logu(1, 90), K = uni(0, 15) ? logu(1, 700) : 0, N = logu(1, 600), R = uni(0, 4) ? logu(1, 40) : uni(0, 2) ? uni(0, 128) : 0,
               bank = logu(1, 5);
     const View x = rows(p, B, L, K, ex), y = rows(p, B, L, N, e, true), o = rows(p, B, L, N, e, true);
     size_t bytes = 0;

@@ -165,6 +165,16 @@ def test_empty(cuda):
         assert torch.equal(run(dict(s, a=a.contiguous(), b=b.contiguous(), scales=sc), cuda).cpu(), s["y"])
 
 
+def test_no_ranks_and_no_columns(cuda):
+    """Nothing to add: y in a new tensor, for rows and for tiles."""
+    for L in (2, 50):
+        s = make(3, L, 16, 12, 4, 2, torch.float16, torch.float16, 6, none=0.0)
+        none = dict(s, a=s["a"][:, :0].contiguous(), b=s["b"][:, :, :0].contiguous())
+        assert torch.equal(run(none, cuda).cpu(), s["y"])
+        none = dict(s, a=s["a"][:, :, :0].contiguous(), x=s["x"][..., :0].contiguous())
+        assert torch.equal(run(none, cuda).cpu(), s["y"])
+
+
 def test_nan_stays_in_its_row(cuda):
     for L in (1, 40):
         s = make(3, L, 64, 64, 8, 2, torch.float32, torch.float32, 7, none=0.0)
