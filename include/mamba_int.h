@@ -508,12 +508,13 @@ mi_status mi_decode_step_static(const mi_model_params *params, int m, const int6
                                 int32_t *logits, int ld_logits, int8_t *const *conv_state,
                                 int32_t *const *h_state, void *stream);
 
-/* ------------------------------------------- float operators (forward only) */
+/* ---------------------------------------------------------- float operators */
 /* The float layer around the ternary projections, for models whose recurrence
  * was trained in floating point: residual addition + RMS norm (float rows, or
  * the 8-bit rows and scales that mi_bitlinear MI_OUT_FLOAT reads), the short
  * causal convolution, the selective state space scan, and products of a few
- * rows with 4-bit weights.  Element types below are mi_dtype values; sums,
+ * rows with 4-bit weights; for batches of requests, token sampling, low-rank
+ * adapters, and a gated recurrence, the only one with a backward pass.  Element types below are mi_dtype values; sums,
  * statistics and states are 32-bit floats.  Row strides (ld*) and sequence
  * strides (bs*) count elements; a stride of an input may be 0 (one row for
  * all).  The elements of a row are adjacent.  Outputs must not overlap inputs

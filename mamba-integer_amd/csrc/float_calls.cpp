@@ -1,7 +1,7 @@
 // The host side of the float operators' calls (mamba_int.ops: add_rms_norm,
 // add_rms_norm_quant, causal_conv, selective_scan, w4_matvec, sample_tokens, adapter_add,
-// gated_scan): checks of the tensors, outputs, and the call of the C ABI, as a Python module.  Through ctypes
-// and checks in Python a call took 9 to 18 us of host time, several times what its
+// gated_scan): checks of the tensors, outputs, the call of the C ABI, and gated_scan's node
+// of autograd, as a Python module.  Through ctypes and checks in Python a call took 9 to 18 us of host time, several times what its
 // kernel takes on a decode step's rows.
 //
 // The entry points come as addresses (the library is loaded once, by _lib), the

@@ -12,6 +12,11 @@
 // integer, so every sum is exact, in any order.  The kept tokens are a beginning of the
 // order, so one 64-bit number (the key of l above the token's complement) tells them
 // from the rest.
+//
+// Rows in slices, a launch each for the first of the order, the bins, the candidates and the
+// draw.  1 x 32000 takes 24 us, 64 x 131072 in bf16 76 (first 7, bins 18, candidates 24, draw
+// 29), where its bytes take 3: what bounds it is the chain of loads, barriers and sums over
+// lanes in each launch, and the exponentials (11 us of the bins).
 #include <algorithm>
 #include <type_traits>
 
@@ -509,7 +514,7 @@ __device__ __forceinline__ SampleCut cut_row(const SampleShared &g, SampleLds &s
 template <class T>
 __global__ __launch_bounds__(kSampleThreads) void sample_gather_kernel(SampleArgs a) {
     __shared__ SampleLds s;
-    __shared__ uint64_t own[kSampleList];      // the slice's candidates (a global counter for each took 52 us where this takes 14)
+    __shared__ uint64_t own[kSampleList];      // the slice's candidates (a global counter for each: 64 rows of 131072 in 52 us instead of 24)
     const int64_t row = blockIdx.y;
     const int slice = blockIdx.x, tid = threadIdx.x;
     SampleShared &g = shared_of(a, row);
