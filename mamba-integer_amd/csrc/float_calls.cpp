@@ -1,8 +1,8 @@
 // The host side of the float operators' calls (mamba_int.ops: add_rms_norm,
 // add_rms_norm_quant, causal_conv, selective_scan, w4_matvec, sample_tokens, adapter_add,
 // gated_scan): checks of the tensors, outputs, the call of the C ABI, and gated_scan's node
-// of autograd, as a Python module.  Through ctypes and checks in Python a call took 9 to 18 us of host time, several times what its
-// kernel takes on a decode step's rows.
+// of autograd, as a Python module.  Through ctypes and checks in Python a call took 9 to
+// 18 us of host time, several times what its kernel takes on a decode step's rows.
 //
 // The entry points come as addresses (the library is loaded once, by _lib), the
 // stream as its handle and device.
@@ -693,7 +693,9 @@ PyObject *guarded(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 #define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<f>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(init),           METHOD(add_rms_norm), METHOD(causal_conv),
-                         METHOD(selective_scan), METHOD(w4_matvec),    METHOD(sample_tokens), METHOD(adapter_add), METHOD(gated_scan), METHOD(gated_scan_recorded), METHOD(check_accumulator), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(selective_scan), METHOD(w4_matvec),
+                         METHOD(sample_tokens), METHOD(adapter_add), METHOD(gated_scan), METHOD(gated_scan_recorded),
+                         METHOD(check_accumulator), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_float_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
