@@ -330,7 +330,9 @@ __device__ __forceinline__ uint64_t cut_among(const SampleRow<T> &r, SampleLds &
             count -= s.above_count;
             if (by_mass) mass -= s.above_mass;
             hi -= (uint64_t)s.bin << shift;
-            lo = more(lo, hi - (((uint64_t)1 << shift) - 1));
+            // (the last part is cut off at lo, which may be nearer to 0 than a part is wide)
+            const uint64_t width = ((uint64_t)1 << shift) - 1;
+            if (hi - lo > width) lo = hi - width;
             __syncthreads();
         }
     }
@@ -771,7 +773,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
         for (int i = 0; i < a.slices; ++i) total += s.mass[i];
         target = target_of(total);
         int slice = 0;
-        for (; before + s.mass[slice] <= target; ++slice) before += s.mass[slice];
+        for (; slice + 1 < a.slices && before + s.mass[slice] <= target; ++slice) before += s.mass[slice];
         r.begin = slice * a.slice;
         r.end = min(r.begin + a.slice, a.vocab);
     }
