@@ -20,7 +20,7 @@ namespace mi {
 
 // Steps of a wave and waves of a block with a whole chunk.  Forwards 16 x 16: 8 x 2048 x 1536 in
 // bf16 68.6 us, 1 x 16384 x 1536 in float32 86.6; 8 waves 69.7 and 88.3, 4 waves 93 and 111, waves
-// of 8 steps with two channels a lane 78 and 101.  A wave takes 74 registers, so a CU has one
+// of 8 steps with two channels a lane 78 and 101.  A wave takes 73 registers, so a CU has one
 // block; held to 64 for two of them it spills: 77.6 and 90.5.  What bounds it is that block's
 // chain of load, join and store (the vector units work in 37 us), in float32 HBM (4.8 TB/s).  Backwards 4 waves of 16, since a wave there
 // takes 160 registers and a block of 8 leaves no room for a second one: 133 us against 166.
@@ -81,6 +81,13 @@ __device__ __forceinline__ float one_minus_square(float n, float a) {
     return v < 0.5f ? s : __builtin_fmaf(-a, a, 1.0f);
 }
 
+// The decay of many steps goes as its root r = exp(-sum of n / 2), held at 2^-126 where it would
+// be flushed to zero: a product of the decays themselves loses a state of up to 2^128 that has
+// not decayed yet, and makes a NaN of an infinite one.  (A NaN among the n is in the sum beside.)
+constexpr float kLeastRoot = 0x1p-126f;
+__device__ __forceinline__ float decay_root(float n) { return fmaxf(__builtin_amdgcn_exp2f(-0.72134752f * n), kLeastRoot); }
+__device__ __forceinline__ float after_steps(float root, float h, float sum) { return __builtin_fmaf(root, root * h, sum); }
+
 // One step's decay and input.
 struct GatedStep {
     float s, q, n, a, m2, b;
@@ -97,7 +104,7 @@ struct GatedStep {
 // ---------------------------------------------------------------- chunks
 // A block has a chunk of a sequence's steps (16 a wave) and 64 C channels, C in a lane.  A
 // wave keeps its rows in registers, sums its steps up as one step
-// h -> A h + H, and starts from the state in front of it, which comes from the waves
+// h -> A^2 h + H, and starts from the state in front of it, which comes from the waves
 // before it through LDS, and from the chunks before through memory: every block passes
 // its chunk's (A, H) on as soon as it has them, and every kJoin-th chunk the state behind
 // it.  A block reads at most the last such state and JOIN - 1 sums, so the rows are read
@@ -233,8 +240,8 @@ __device__ __forceinline__ void join_chunks(const GatedArgs &a, GatedLds<C, WAVE
             const int v = BACKWARDS ? WAVES - 1 - w : w;
 #pragma unroll
             for (int j = 0; j < C; ++j) {
-                H[j] = __builtin_fmaf(s.a[v][lane * C + j], H[j], s.h[v][lane * C + j]);
-                A[j] *= s.a[v][lane * C + j];
+                H[j] = after_steps(s.a[v][lane * C + j], H[j], s.h[v][lane * C + j]);
+                A[j] = fmaxf(A[j] * s.a[v][lane * C + j], kLeastRoot);
             }
         }
         uint64_t *p = words.sums(b, at);
@@ -262,14 +269,14 @@ __device__ __forceinline__ void join_chunks(const GatedArgs &a, GatedLds<C, WAVE
     for (int j = 0; j < C; ++j) {
         float h = base > 0 ? s.before_h[JOIN - 1][lane * C + j] : s.before_h[0][lane * C + j];
         for (int w = base > 0 ? 0 : 1; base + w < at; ++w)
-            h = __builtin_fmaf(s.before_a[w][lane * C + j], h, s.before_h[w][lane * C + j]);
+            h = after_steps(s.before_a[w][lane * C + j], h, s.before_h[w][lane * C + j]);
         carry[j] = h;
     }
     if (wave == 0 && at % JOIN == JOIN - 1 && behind) {
         uint64_t *p = words.template state<JOIN>(b, at, a.chunks);
 #pragma unroll
         for (int j = 0; j < C; ++j)
-            if (c + j < a.dim) pass_on(p + c + j, __builtin_fmaf(A[j], carry[j], H[j]));
+            if (c + j < a.dim) pass_on(p + c + j, after_steps(A[j], carry[j], H[j]));
     }
 }
 
@@ -299,12 +306,14 @@ struct GatedInputs {
 #pragma unroll
         for (int t = 0; t < STEPS; ++t, p.next(FULL || t0 + t < at.len)) to[t] = p.template load<C, FULL>(c, a.dim);
     }
-    // Each step's decay and input, and the wave's steps as one: h -> A h + H.
+    // Each step's decay and input, and the wave's steps as one: h -> A^2 h + H.
     template <bool FULL>
     __device__ __forceinline__ void steps(const GatedArgs &a, const GatedTile &at, int t0, const float *k, float (*av)[C], float (*bv)[C],
                                           float *A, float *H, float (*m2)[C] = nullptr) const {
+        float n[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
+            n[j] = 0.0f;
             A[j] = 1.0f;
             H[j] = 0.0f;
         }
@@ -319,9 +328,11 @@ struct GatedInputs {
                 bv[t][j] = on ? g.b : 0.0f;
                 if (m2) m2[t][j] = g.m2;
                 H[j] = __builtin_fmaf(av[t][j], H[j], bv[t][j]);
-                A[j] *= av[t][j];
+                n[j] += on ? g.n : 0.0f;
             }
         }
+#pragma unroll
+        for (int j = 0; j < C; ++j) A[j] = decay_root(n[j]);
     }
 };
 
@@ -384,7 +395,7 @@ __global__ __launch_bounds__(WAVES * 64) void gated_scan_kernel(GatedArgs a) {
     if constexpr (WAVES > 1)
         for (int w = 0; w < wave; ++w) {
 #pragma unroll
-            for (int j = 0; j < C; ++j) h[j] = __builtin_fmaf(s.a[w][lane * C + j], h[j], s.h[w][lane * C + j]);
+            for (int j = 0; j < C; ++j) h[j] = after_steps(s.a[w][lane * C + j], h[j], s.h[w][lane * C + j]);
         }
     if (a.saved && t0 % kChunkBack == 0 && t0 < a.len) {
         float *p = a.saved + ((int64_t)b * a.kept + t0 / kChunkBack) * a.dim;
@@ -477,7 +488,7 @@ __global__ __launch_bounds__(WAVES * 64) void gated_scan_backward_kernel(GatedAr
         __syncthreads();
         for (int w = 0; w < wave; ++w) {
 #pragma unroll
-            for (int j = 0; j < C; ++j) h[j] = __builtin_fmaf(s.a[w][lane * C + j], h[j], s.h[w][lane * C + j]);
+            for (int j = 0; j < C; ++j) h[j] = after_steps(s.a[w][lane * C + j], h[j], s.h[w][lane * C + j]);
         }
         __syncthreads();
 #pragma unroll
@@ -488,7 +499,7 @@ __global__ __launch_bounds__(WAVES * 64) void gated_scan_backward_kernel(GatedAr
             if (work) join_chunks<C, WAVES, true>(a, s, b, (at.len - 1) / CHUNK - at.chunk, at.chunk > 0, (int)c, none, carry);
         for (int w = WAVES - 1; w > wave; --w) {
 #pragma unroll
-            for (int j = 0; j < C; ++j) carry[j] = __builtin_fmaf(s.a[w][lane * C + j], carry[j], s.h[w][lane * C + j]);
+            for (int j = 0; j < C; ++j) carry[j] = after_steps(s.a[w][lane * C + j], carry[j], s.h[w][lane * C + j]);
         }
     }
     const auto finish = [&](auto full) {
