@@ -672,8 +672,10 @@ mi_status mi_adapter_add(const void *x, int x_type, int64_t ldx, int64_t bsx, co
  * state after lens[b] tokens).  workspace (forward_bytes) and saved
  * (saved_bytes; nullable: what mi_gated_scan_backward reads of a forward pass
  * with the same inputs) as mi_gated_scan_sizes says, 16-byte aligned, of any
- * content.  Infinite values give what the formulas give, except that an
- * infinite state may become a NaN at a step whose a is below 2^-126.
+ * content.  Infinite values give what the formulas give, except that rate *
+ * softplus(decay) is the largest float where it is infinite (a closed gate, s =
+ * 0, keeps the state), and that an infinite state may become a NaN at a step
+ * whose a is below 2^-126.
  * batch <= 65535, dim <= 2^24, ceil(len / 64) * batch * ceil(dim / 64) < 2^23. */
 mi_status mi_gated_scan_sizes(int batch, int len, int dim, size_t *forward_bytes, size_t *backward_bytes,
                               size_t *saved_bytes);

@@ -57,8 +57,9 @@ __device__ __forceinline__ int gated_len(const GatedArgs &a, int b) {
 // log(1 + exp(v)) = max(v, 0) + log(w) + (e - (w - 1)) / w, e = exp(-|v|), w = 1 + e rounded: the
 // last term is what the rounding of w lost (w = 1 wherever it matters).  The exponent's
 // product with log2 e is kept in two parts, so a low v, whose value is e, has e's precision.
+// (The maximum that keeps a NaN: past -1e4 e is 0, and the parts of an infinite product none.)
 __device__ __forceinline__ float gated_softplus(float v) {
-    const float u = -fabsf(v), p = u * 1.44269504f;
+    const float u = __builtin_elementwise_maximum(-fabsf(v), -1e4f), p = u * 1.44269504f;
     const float e = __builtin_amdgcn_exp2f(p);
     const float lost = __builtin_fmaf(u, 1.44269504f, -p) + u * 1.925963033e-8f;      // log2 e's next bits
     const float f = __builtin_fmaf(e, lost * 0.693147181f, e), w = 1.0f + f;
@@ -340,10 +341,16 @@ template <int C>
 __device__ __forceinline__ uint32_t first_channel(const GatedTile &at) {
     return (uint32_t)(at.group * 64 + (int)(threadIdx.x & 63)) * C;
 }
+// rate softplus(decay), the largest float where that is infinite: a closed gate then keeps the
+// state whatever the decay is.
 template <int C, bool FULL>
 __device__ __forceinline__ void decays(const GatedArgs &a, uint32_t c, float *k) {
+    constexpr float kMost = 0x1.fffffep127f;
 #pragma unroll
-    for (int j = 0; j < C; ++j) k[j] = FULL || (int)c + j < a.dim ? a.rate * gated_softplus(a.decay[c + j]) : 0.0f;
+    for (int j = 0; j < C; ++j) {
+        const float soft = FULL || (int)c + j < a.dim ? __builtin_elementwise_minimum(gated_softplus(a.decay[c + j]), kMost) : 0.0f;
+        k[j] = __builtin_elementwise_minimum(a.rate * soft, kMost);
+    }
 }
 
 template <class T, int C, int STEPS, int WAVES, bool MANY>
@@ -533,7 +540,8 @@ __global__ __launch_bounds__(WAVES * 64) void gated_scan_backward_kernel(GatedAr
                 const float g = dh + carry[j];
                 // (the hardware root takes a subnormal for 0, its reciprocal is infinite there)
                 const float inv = m2[t][j] >= 0x1p-126f ? __builtin_amdgcn_rsqf(m2[t][j]) : 0.0f, gx = g * m2[t][j] * inv * si;
-                const float p = g * n * (si * xf * av_ * av_ * inv - av_ * hv[t][j]);
+                // (n may be the largest float, beside decays of 0)
+                const float p = g * (n * (si * xf * av_ * av_ * inv - av_ * hv[t][j]));
                 dx.v[j] = (T)gx;
                 di.v[j] = (T)(gx * xf * (1.0f - si));
                 dr.v[j] = (T)(p * (1.0f - sr));

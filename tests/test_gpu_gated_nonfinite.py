@@ -98,3 +98,40 @@ def test_gradients(cuda, L, what):
         same(g, *want["d_" + n], torch.float32)
     if what == "dy":
         assert torch.isinf(grads[0][1, :L - L // 5, 4]).all() and torch.isinf(grads[4][1, 4])
+
+
+@pytest.mark.parametrize("L", LENGTHS)
+@pytest.mark.parametrize("rate", [8.0, 0.0, 1e30])
+def test_decays_at_the_ends_of_their_range(cuda, L, rate):
+    """A decay of -inf (and what softplus makes 0) keeps the state, one of +inf leaves nothing of
+    it but where the gate is closed or the rate is 0, and both have gradients."""
+    from mamba_int import ops
+    inf = float("inf")
+    decay = torch.tensor([-inf, -3.4e38, -1e30, -2e4, inf, 3.4e38, 2.5e38, 1e30, float("nan")])
+    s = make(L, 0.0, seed=L)
+    s["decay"] = decay
+    s["r"][1] = -inf            # closed
+    dy = torch.rand(2, L, 9, generator=torch.Generator().manual_seed(L)).to(cuda)
+    y, h = forward(s, cuda, rate=rate)
+    leaf = {k: v.to(cuda).requires_grad_() for k, v in s.items()}
+    grads = dict(zip(leaf, torch.autograd.grad(ops.gated_scan(**leaf, rate=rate), list(leaf.values()), dy)))
+    assert torch.isnan(y[..., 8]).all() and not torch.isnan(y[..., :8]).any() and not torch.isnan(h[:, :8]).any()
+    x, q = s["x"].double(), torch.sigmoid(s["i"].double())
+    kept = torch.zeros(2, 8, dtype=torch.bool)
+    kept[:, :4] = True                     # a = 1, so nothing is added
+    kept[1] = True
+    kept |= rate == 0.0
+    first = s["h_in"][:, :8].double()
+    want = torch.where(kept.unsqueeze(1), first.unsqueeze(1), (q * x)[..., :8])
+    # two roundings of q, its product and h's: 8 U with the hardware's reciprocal and exponential
+    assert ((y[..., :8].cpu() - want).abs() <= 2.0 ** -21 * want.abs()).all()
+    assert torch.equal(h.cpu()[:, :8], y.cpu()[:, -1, :8])
+    g = dy.double().cpu()[..., :8]
+    sums = g.flip(1).cumsum(1).flip(1)
+    expect = {"x": torch.where(kept.unsqueeze(1), 0.0, g * q[..., :8]), "r": torch.zeros_like(g),
+              "i": torch.where(kept.unsqueeze(1), 0.0, g * (q * x * (1 - q))[..., :8]), "decay": torch.zeros(8, dtype=torch.float64),
+              "h_in": torch.where(kept, sums[:, 0], 0.0)}
+    for n, w in expect.items():
+        got = grads[n].double().cpu()[..., :8]
+        # sums of up to L gradients; 1 - q is off by two roundings of 1, against 0.26 at least
+        assert ((got - w).abs() <= (L + 64) * 2.0 ** -24 * w.abs()).all(), n
