@@ -586,11 +586,12 @@ __global__ __launch_bounds__(WAVES * 64) void gated_scan_backward_kernel(GatedAr
     }
 }
 
-// ddecay from the sums of p over the chunks: 16 waves share them.
+// ddecay from the sums of p over the chunks: 16 waves share them, in 64 bits (sequences and
+// chunks may cancel, and there may be any number of them).
 __global__ __launch_bounds__(1024) void gated_decay_kernel(const float *sums, const float *decay, float *out, int64_t rows, int dim) {
-    __shared__ float part[16][64];
+    __shared__ double part[16][64];
     const int lane = threadIdx.x & 63, wave = wave_id(), c = blockIdx.x * 64 + lane;
-    float s = 0.0f;
+    double s = 0.0;
     if (c < dim) {
         int64_t j = wave;
         for (; j + 7 * 16 < rows; j += 8 * 16) {
@@ -609,7 +610,7 @@ __global__ __launch_bounds__(1024) void gated_decay_kernel(const float *sums, co
     // sigmoid / softplus: 1 - e/2 + ... of e = exp(v) for low v
     const float v = decay[c], e = expf(v);
     const float ratio = v < -9.0f ? 1.0f - 0.5f * e : 1.0f / (1.0f + expf(-v)) / gated_softplus(v);
-    out[c] = s * ratio;
+    out[c] = (float)(s * ratio);
 }
 
 mi_status gated_dims(const char *fn, int batch, int len, int dim) {
