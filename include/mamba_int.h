@@ -651,9 +651,8 @@ mi_status mi_sample_tokens(const void *logits, int type, int64_t ld, double scal
  * n values of `type`, out may be y itself (with its strides): rows without an
  * adapter are not touched then.  A [bank,rank,k] and B [bank,n,rank] of
  * weight_type; scales fp32 [bank], nullable (1); lens int32 [batch], nullable.
- * The products and the sum with y are in 32 bits, rounded once.  A row with an
- * infinite x or adapter value may give a NaN where the formula gives an
- * infinity.  rank in [0, 128]; k and n <= 2^23; batch * len < 2^22,
+ * The products and the sum with y are in 32 bits, rounded once; infinite values
+ * give what the formula gives.  rank in [0, 128]; k and n <= 2^23; batch * len < 2^22,
  * batch <= 65535 for len >= 8.
  * workspace: 16-byte aligned, mi_adapter_workspace_size bytes. */
 mi_status mi_adapter_workspace_size(int batch, int len, int rank, size_t *bytes);

@@ -157,6 +157,14 @@ __device__ __forceinline__ Packed<T, 8> load8(const T *p, int c, int n) {
     for (int i = 0; i < 8; ++i) v.v[i] = c + i < n ? p[c + i] : T(0);
     return v;
 }
+// What the parts leave of an infinity is inf - inf, and 0 * inf with another's parts.  So a sum
+// that came out as a NaN is computed again from the values, one by one until it is one itself.
+template <class F>
+__device__ __forceinline__ float sum_again(int n, F &&term) {
+    float s = 0.0f;
+    for (int i = 0; i < n && s == s; ++i) s = term(i, s);
+    return s;
+}
 template <int P, int Q>
 __device__ __forceinline__ v4f product(const Parts<P> &a, const Parts<Q> &b, v4f d) {
     // the small ones first
@@ -262,6 +270,15 @@ __global__ __launch_bounds__(kDownWaves * 64) void adapter_down_tiles_kernel(Ada
         for (int v = 1; v < HALF; ++v) s += sums[v][tile][lane];
         const int token = t0 + tile / NT * 16 + r, rank = tile % NT * 16 + 4 * g;
         if (token >= tokens) continue;
+        if constexpr (parts_of<X>() > 1 || parts_of<W>() > 1) {
+            const X *xp = static_cast<const X *>(a.x) + (b * a.bsx + token * a.ldx);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (s[i] == s[i] || rank + i >= a.rank) continue;
+                const W *wp = static_cast<const W *>(a.a) + ((int64_t)id * a.rank + rank + i) * a.k;
+                s[i] = sum_again(a.k, [&](int c, float v) { return __builtin_fmaf((float)xp[c], (float)wp[c], v); });
+            }
+        }
         const int64_t row = (int64_t)b * a.len + token;
         float f = a.scales ? a.scales[id] : 1.0f;
         if (a.x_scale) f *= a.x_scale[row];
@@ -275,8 +292,9 @@ __global__ __launch_bounds__(kDownWaves * 64) void adapter_down_tiles_kernel(Ada
             for (int i = 0; i < 2; ++i) {
                 const uint32_t lo = __builtin_bit_cast(uint32_t, v[2 * i]), hi = __builtin_bit_cast(uint32_t, v[2 * i + 1]);
                 o[i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-                v[2 * i] -= __builtin_bit_cast(float, lo & 0xffff0000u);
-                v[2 * i + 1] -= __builtin_bit_cast(float, hi & 0xffff0000u);
+                // (an infinity is its first part alone)
+                v[2 * i] = fabsf(v[2 * i]) == __builtin_inff() ? 0.0f : v[2 * i] - __builtin_bit_cast(float, lo & 0xffff0000u);
+                v[2 * i + 1] = fabsf(v[2 * i + 1]) == __builtin_inff() ? 0.0f : v[2 * i + 1] - __builtin_bit_cast(float, hi & 0xffff0000u);
             }
             *reinterpret_cast<uint2 *>(static_cast<bf16_t *>(a.t) + (p * (int64_t)a.batch * a.len + row) * a.ranks + rank) =
                 make_uint2(o[0], o[1]);
@@ -294,7 +312,7 @@ __global__ __launch_bounds__(kDownWaves * 64) void adapter_down_tiles_kernel(Ada
 // four adjacent columns of a token from a tile of the result, so B's rows go to tiles such
 // that the lane's tiles (two of them for 16-bit y) are 16 adjacent bytes.
 template <class Y, class W, int KS, int NT, int UT>
-__global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
+__global__ __launch_bounds__(256, KS == 1 && parts_of<W>() == 1 ? 4 : 1) void adapter_up_tiles_kernel(AdapterArgs a) {
     constexpr int PAIR = sizeof(Y) == 4 ? 1 : 2, V = 4 * PAIR;
     const int b = blockIdx.z, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int id = adapter_of(a, b), tokens = id < 0 || a.rank == 0 ? 0 : tokens_of(a, b), t0 = (int)blockIdx.y * a.up_tokens;
@@ -329,6 +347,7 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
             }
         }
     };
+    uint32_t again = 0;      // tiles in which the lane has a NaN, left for later
     const auto tile = [&](int t, const Packed<Y, V> *yv) {
         v4f d[NT];
 #pragma unroll
@@ -348,6 +367,13 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
         }
         const bool on = t + r < tokens;
         if (t + r >= (in_place ? tokens : a.len)) return;
+        bool odd = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) odd |= __builtin_isunordered(d[n][0], d[n][1]) || __builtin_isunordered(d[n][2], d[n][3]);
+        if (on && odd) {
+            again |= 1u << (t - t0) / 16;
+            return;
+        }
         Y *p = static_cast<Y *>(a.out) + (b * a.bso + (t + r) * a.ldo);
 #pragma unroll
         for (int h = 0; h < NT / PAIR; ++h) {
@@ -381,6 +407,23 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
         turn(t, y[0]);
         load(t + 32 * UT, y[0]);
         turn(t + 16 * UT, y[1]);
+    }
+    // (in the loop above it took 31 to 50 registers more)
+    const int64_t part = (int64_t)a.batch * a.len * a.ranks;
+    for (; again; again &= again - 1) {
+        const int t = t0 + 16 * __builtin_ctz(again) + r;
+        const bf16_t *tr = static_cast<const bf16_t *>(a.t) + ((int64_t)b * a.len + t) * a.ranks;
+#pragma unroll 1
+        for (int e = 0; e < 4 * NT; ++e) {
+            const int col = column(e / V) + e % V;
+            if (col >= a.n) continue;
+            const W *wp = static_cast<const W *>(a.b) + ((int64_t)id * a.n + col) * a.rank;
+            const float sum = sum_again(a.rank, [&](int j, float v) {
+                return __builtin_fmaf((float)tr[j] + (float)tr[j + part] + (float)tr[j + 2 * part], (float)wp[j], v);
+            });
+            const Y yv = (static_cast<const Y *>(a.y) + (b * a.bsy + t * a.ldy))[col];
+            (static_cast<Y *>(a.out) + (b * a.bso + t * a.ldo))[col] = (Y)((float)yv + sum);
+        }
     }
 }
 
