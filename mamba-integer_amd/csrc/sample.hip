@@ -47,17 +47,20 @@ struct SampleArgs {
     int vocab, bits;
     int slices, slice;      // of a row, and tokens of one
     char *workspace;
+    size_t row_bytes;       // of it
 };
 
-// What the kernels of a row pass on, in the workspace.
+// What the kernels of a row pass on, in the workspace; behind it the masses of each slice's bins
+// (top_p alone).
 struct SampleShared {
     uint64_t best[kSampleSlices];            // the first of the order in a slice
     uint64_t slice_mass[kSampleSlices];      // the mass of a slice that is surely kept
-    uint64_t slice_bins[kSampleSlices][kSampleBins];      // top_p alone: a slice's masses
     uint64_t mass[kSampleBins];
     uint32_t count[kSampleBins];
     uint32_t found, unused;
     uint64_t list[kSampleList];              // places of candidates
+    __device__ __forceinline__ uint64_t *slice_bins(int slice) { return reinterpret_cast<uint64_t *>(this + 1) + slice * kSampleBins; }
+    static size_t bytes(int slices) { return sizeof(SampleShared) + (size_t)slices * kSampleBins * sizeof(uint64_t); }
 };
 
 // A logit's place in the order: larger for larger logits, 0 and -0 alike.
@@ -413,7 +416,7 @@ __device__ __forceinline__ void scale_by(SampleRow<T> &r, const SampleArgs &a, u
 // Few rows of many tokens: a row's passes are shared by `slices` blocks, in a kernel each
 // (the first of the order; the bins; what the bins leave), and the last kernel draws.
 __device__ __forceinline__ SampleShared &shared_of(const SampleArgs &a, int64_t row) {
-    return reinterpret_cast<SampleShared *>(a.workspace)[row];
+    return *reinterpret_cast<SampleShared *>(a.workspace + row * a.row_bytes);
 }
 // (a slice's a lane: one after the other they took a load's latency each)
 __device__ __forceinline__ uint64_t best_of(const SampleArgs &a, const SampleShared &g) {
@@ -475,7 +478,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_bins_kernel(SampleArgs 
         if (s.count[i]) atomicAdd(&g.count[i], s.count[i]);
         if (f.by_k) continue;
         if (s.mass[i]) atomicAdd((unsigned long long *)&g.mass[i], (unsigned long long)s.mass[i]);
-        g.slice_bins[slice][i] = s.mass[i];
+        g.slice_bins(slice)[i] = s.mass[i];
     }
 }
 
@@ -543,7 +546,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_gather_kernel(SampleArg
         });
     else if (f.by_p && !(f.least > 0.0f)) {
         // (the bins in front of the cut are kept as they are)
-        for (int i = tid; i < c.bin; i += kSampleThreads) sum += g.slice_bins[slice][i];
+        for (int i = tid; i < c.bin; i += kSampleThreads) sum += g.slice_bins(slice)[i];
         each_logit(r, [&](Logit<T> v, int i) {
             const double d = r.below(v);
             if (SampleRow<T>::bin(d) == c.bin) list(v, i);
@@ -845,7 +848,8 @@ extern "C" mi_status mi_sample_workspace_size(int rows, int vocab, size_t *bytes
     MI_REQUIRE(rows >= 0 && rows < (1 << 22), MI_ERR_BAD_DIM, "mi_sample_workspace_size: rows=%d must be in [0, %d)", rows, 1 << 22);
     MI_REQUIRE(vocab >= 1 && vocab <= kSampleMaxVocab, MI_ERR_BAD_DIM, "mi_sample_workspace_size: vocab=%d must be in [1, %d]", vocab,
                kSampleMaxVocab);
-    *bytes = sample_slices(rows, vocab) > 1 ? (size_t)rows * sizeof(SampleShared) : 0;
+    const int slices = sample_slices(rows, vocab);
+    *bytes = slices > 1 ? rows * SampleShared::bytes(slices) : 0;
     return MI_OK;
 }
 
@@ -868,7 +872,7 @@ extern "C" mi_status mi_sample_tokens(const void *logits, int type, int64_t ld, 
     if (rows == 0) return MI_OK;
     MI_REQUIRE(logits && u && ids, MI_ERR_NULL_POINTER, "mi_sample_tokens: logits, u and ids are required");
     const int slices = sample_slices(rows, vocab);
-    const size_t need = slices > 1 ? (size_t)rows * sizeof(SampleShared) : 0;
+    const size_t need = slices > 1 ? rows * SampleShared::bytes(slices) : 0;
     MI_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), MI_ERR_BAD_ARG,
                "mi_sample_tokens: the workspace has %zu bytes, %zu are needed", workspace_bytes, need);
     MI_REQUIRE(need == 0 || aligned(workspace, 16), MI_ERR_BAD_ALIGNMENT, "mi_sample_tokens: the workspace must be 16-byte aligned");
@@ -877,7 +881,7 @@ extern "C" mi_status mi_sample_tokens(const void *logits, int type, int64_t ld, 
     // the masses of a row sum to 2^62 at most; a slice has whole vectors of 16 bytes
     SampleArgs a{logits, ld, scale, u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all,
                  ids, logprob, vocab, std::min(51, 62 - log2v), slices, ((vocab + slices - 1) / slices + 7) / 8 * 8,
-                 static_cast<char *>(workspace)};
+                 static_cast<char *>(workspace), SampleShared::bytes(slices)};
     a.slices = (vocab + a.slice - 1) / a.slice;      // (none without tokens)
     const hipStream_t st = as_stream(stream);
     const auto launch = [&](auto t) {
