@@ -16,7 +16,7 @@ LIB_PATH = os.environ.get("MAMBA_INT_LIB", os.path.join(PKG_ROOT, "libmamba_int.
 
 MI_OK, MI_ERR_NULL_POINTER, MI_ERR_BAD_DIM, MI_ERR_BAD_ALIGNMENT, MI_ERR_BAD_ARG, MI_ERR_HIP = range(6)
 OUT_INT32, OUT_INT8, OUT_DECAY_MOD, OUT_RESIDUAL, OUT_FLOAT = range(5)
-F32, BF16, F16, I32, I8 = range(5)   # mi_dtype
+F32, BF16, F16, TYPE_I32, TYPE_I8 = range(5)     # mi_dtype (I32 is an argument's type below)
 
 P = ctypes.c_void_p
 I = ctypes.c_int
