@@ -97,3 +97,43 @@ def test_lowest_integers_next_to_each_other(program, tmp_path, V, below):
     logits = (LOWEST + np.random.default_rng(below).integers(0, 5_000_000, (4, V))).astype(np.int32)
     check(program, tmp_path, [(logits, U, dict(scale=1e-12, top_k=V - below)),
                               (logits, U, dict(scale=1e-12, top_p=1 - (below + 0.5) / V))])
+
+
+def mixed(B, seed):
+    """Parameters of B rows: every kind of filter, none, and the first of the order, in turn."""
+    g = np.random.default_rng(seed)
+    kinds = [dict(), dict(temperature=0.0), dict(top_k=20), dict(top_k=700), dict(top_p=0.8), dict(top_k=3000, top_p=0.7), dict(min_p=0.05),
+             dict(top_p=0.9, min_p=0.01), dict(top_k=40, top_p=0.9, min_p=0.02), dict(temperature=2.5, top_p=0.95), dict(top_k=1),
+             dict(temperature=float("nan"))]
+    rows = [kinds[(b + seed) % len(kinds)] for b in range(B)]
+    par = {n: np.array([r.get(n, d) for r in rows], np.int32 if n == "top_k" else np.float32)
+           for n, d in (("temperature", 1.0), ("top_p", 1.0), ("min_p", 0.0), ("top_k", 0))}
+    return par, g
+
+
+@pytest.mark.parametrize("V", [777, 9001, 20000])
+@pytest.mark.parametrize("dtype", [np.float32, np.int32])
+def test_rows_of_every_kind(program, tmp_path, V, dtype):
+    par, g = mixed(12, V)
+    logits = 2.0 * g.standard_normal((12, V)) - np.log1p(np.arange(V))[g.permutation(V)]
+    if dtype == np.int32:
+        logits, par = np.round(logits * 1024), dict(par, scale=1.0 / 1024)
+    check(program, tmp_path, [(logits.astype(dtype), g.random(12).astype(np.float32), par)])
+
+
+@pytest.mark.parametrize("V", [777, 9001, 20000])
+@pytest.mark.parametrize("par", [dict(), dict(top_k=20), dict(top_p=0.8), dict(top_k=600, top_p=0.7, min_p=0.01), dict(temperature=0.0),
+                                 dict(temperature=float("inf"))])
+def test_masked_rows(program, tmp_path, V, par):
+    """Rows, and whole slices of them, of -inf, NaN and the lowest value; infinities; u out of range."""
+    g = np.random.default_rng(V)
+    low, inf, nan = np.finfo(np.float32).min, np.inf, np.nan
+    logits = g.standard_normal((10, V)).astype(np.float32)
+    for b, v in enumerate((-inf, low, nan)):
+        logits[b, : V - 300] = v
+        logits[3 + b] = v
+    logits[6, 100], logits[6, V - 5] = inf, inf
+    logits[7], logits[7, V // 2] = -inf, low
+    logits[8, ::2], logits[8, 1::2] = 0.0, -0.0
+    u = np.array([0.3, 0.6, 0.9, 0.5, 0.5, 0.5, 0.75, 0.5, 0.4, 1.0], np.float32)
+    check(program, tmp_path, [(logits, u, par)])
