@@ -23,7 +23,7 @@ class Sampling:
 
     def draw(self, logits: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
         """Tokens int64 [B] from logits [B, V] (int32 ones count in ``scale``); a row without a
-        token to draw gives -1."""
+        token to draw gives -1, which is no token to go on with."""
         u = torch.rand(logits.shape[0], device=logits.device, generator=self.generator)
         return ops.sample_tokens(logits, u, temperature=self.temperature, top_k=self.top_k, top_p=self.top_p, min_p=self.min_p,
                                  scale=scale)

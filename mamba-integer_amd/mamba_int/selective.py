@@ -235,13 +235,20 @@ class SelectiveRunner:
     def generate(self, ids: torch.Tensor, steps: int, lens: Optional[torch.Tensor] = None, sampling: Optional[Sampling] = None,
                  adapters: Optional[Adapters] = None) -> torch.Tensor:
         """Tokens int64 [B, steps] after the prompts: the largest logit's, or drawn as ``sampling``
-        says."""
+        says.  A sequence whose logits hold nothing to draw (NaN and -inf alone) ends: it has -1
+        from there on."""
         state = self.new_state(ids.shape[0])
         out, logits = [], self.forward(ids, state, lens, adapters)
         for i in range(steps):
-            out.append((sampling.draw(logits) if sampling is not None else logits.argmax(-1)).unsqueeze(-1))
+            if sampling is None:
+                tok = logits.argmax(-1, keepdim=True)
+                out.append(tok)
+            else:
+                tok = sampling.draw(logits).unsqueeze(-1)
+                out.append(torch.where(out[-1] < 0, -1, tok) if out else tok)
+                tok = out[-1].clamp(min=0)      # (what an ended sequence goes on with is dropped)
             if i + 1 < steps:
-                logits = self.forward(out[-1], state, adapters=adapters)
+                logits = self.forward(tok, state, adapters=adapters)
         return torch.cat(out, 1) if out else ids.new_empty((ids.shape[0], 0))
 
 
