@@ -124,10 +124,11 @@ def test_two_graphs_and_a_stream(cuda):
     from mamba_int import ops
     B, V = 8, 40000
     side = [torch.cuda.Stream() for _ in range(2)]
-    graphs, got, want = [], [], []
+    graphs, got, want, inputs = [], [], [], []
     for i in range(2):
         logits, _, u = make(B, V, torch.float32, 50 + i)
         logits, u = logits.to(cuda), u.to(cuda)
+        inputs.append((logits, u))      # (a graph reads them at every replay)
         want.append(ops.sample_tokens(logits, u, top_p=0.9 - 0.2 * i))
         torch.cuda.synchronize()
         graphs.append(torch.cuda.CUDAGraph())
