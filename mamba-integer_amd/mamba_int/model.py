@@ -5,7 +5,8 @@ Orchestrates the per-layer kernels in the block order of
 model order of ``MambaIntegerModel.forward`` (``:486-495``).  Adds what the
 reference lacks: a recurrent decode step with per-layer conv and scan state
 (the reference recomputes the whole prefix per token,
-``scripts/inference.py:147-161``), and a HIP-graph-captured greedy decode loop.
+``scripts/inference.py:147-161``), and a HIP-graph-captured decode loop, greedy or
+with drawn tokens.
 
 Activations live in preallocated int8/int32 workspaces sized for one
 (batch, length); the int32 residual is updated in place by the out_proj
@@ -20,6 +21,7 @@ import torch
 
 from . import ops
 from .params import LayerParams, ModelParams
+from .sampling import Sampling
 
 
 @dataclass
@@ -411,27 +413,33 @@ class IntegerMambaRunner:
 
     @torch.no_grad()
     def decode_loop(self, logits: torch.Tensor, state: DecodeState, n_new: int,
-                    use_graph: bool = True) -> torch.Tensor:
-        """Greedy continuation from last-position logits [B, V] and `state`."""
+                    use_graph: bool = True, sampling: Optional[Sampling] = None, scale: float = 1.0) -> torch.Tensor:
+        """Continuation from last-position logits [B, V] and `state`: greedy, or drawn as
+        `sampling` says from logits that count in `scale` (with graphs each step is the replay of
+        a whole step and the draw behind it)."""
         B = logits.shape[0]
         out = torch.empty((B, n_new), dtype=torch.int64, device=self.device)
         if n_new == 0:
             return out
-        tok = ops.argmax(logits)
+        tok = ops.argmax(logits) if sampling is None else sampling.draw(logits, scale)
         out[:, 0] = tok
         if not use_graph:
             for i in range(1, n_new):
                 logits = self.decode_step(tok, state)
-                tok = ops.argmax(logits)
+                tok = ops.argmax(logits) if sampling is None else sampling.draw(logits, scale)
                 out[:, i] = tok
             return out
-        if self._chain_ok(B):
+        if n_new == 1:
+            return out
+        if sampling is None and self._chain_ok(B):
             self._decode_chain_loop(tok, state, out)
             return out
         step = self._decode_graph(B, state)
         step.tok_in.copy_(tok)
         for i in range(1, n_new):
             step.graph.replay()          # embed(tok) ... argmax -> tok
+            if sampling is not None:
+                sampling.draw(step.logits, scale, out=step.tok_in)
             out[:, i] = step.tok_in
         # hand the state back to the caller's tensors
         for i in range(len(self.layers)):
@@ -565,7 +573,7 @@ class IntegerMambaRunner:
             class _G:
                 pass
             g = _G()
-            g.graph, g.tok_in, g.tok_out, g.state = graph, tok_in, tok_out, gstate
+            g.graph, g.tok_in, g.tok_out, g.logits, g.state = graph, tok_in, tok_out, logits, gstate
             self._graphs[B] = g
         for i in range(len(self.layers)):
             g.state.conv[i].copy_(state.conv[i])

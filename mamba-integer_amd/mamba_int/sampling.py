@@ -21,9 +21,9 @@ class Sampling:
     min_p: Union[float, torch.Tensor] = 0.0
     generator: Optional[torch.Generator] = None
 
-    def draw(self, logits: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
-        """Tokens int64 [B] from logits [B, V] (int32 ones count in ``scale``); a row without a
-        token to draw gives -1, which is no token to go on with."""
+    def draw(self, logits: torch.Tensor, scale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Tokens int64 [B] (in ``out``) from logits [B, V] (int32 ones count in ``scale``); a row
+        without a token to draw gives -1, which is no token to go on with."""
         u = torch.rand(logits.shape[0], device=logits.device, generator=self.generator)
         return ops.sample_tokens(logits, u, temperature=self.temperature, top_k=self.top_k, top_p=self.top_p, min_p=self.min_p,
-                                 scale=scale)
+                                 scale=scale, out=out)

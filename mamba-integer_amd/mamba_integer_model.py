@@ -281,16 +281,12 @@ class MambaIntegerModel(nn.Module):
                  sampling: Optional[Sampling] = None) -> torch.Tensor:
         """Returns input_ids extended by max_new_tokens ids: the largest logits', or drawn from the
         logits as ``sampling`` says, step by step (the reference draws at a temperature of 0.8,
-        ``scripts/inference.py:157-158``)."""
+        ``scripts/inference.py:157-158``).  ``use_graph``: the steps are replayed from HIP graphs,
+        drawn ones too."""
         runner = self.runner(input_ids.device)
-        if sampling is None or max_new_tokens == 0:
-            new = runner.generate(input_ids, max_new_tokens, use_graph=use_graph)
-            return torch.cat([input_ids, new], dim=1)
         logits, state = runner.prefill(input_ids)
-        new = [sampling.draw(logits, self.logit_scale)]
-        while len(new) < max_new_tokens:
-            new.append(sampling.draw(runner.decode_step(new[-1], state), self.logit_scale))
-        return torch.cat([input_ids, torch.stack(new, dim=1)], dim=1)
+        new = runner.decode_loop(logits, state, max_new_tokens, use_graph=use_graph, sampling=sampling, scale=self.logit_scale)
+        return torch.cat([input_ids, new], dim=1)
 
 
 __all__ = ["MambaIntegerModel", "MambaIntegerBlock", "MambaIntegerBlockV2", "BitShiftNorm", "BitShiftNormV2",
