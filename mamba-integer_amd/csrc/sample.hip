@@ -57,7 +57,7 @@ struct SampleShared {
     uint64_t slice_mass[kSampleSlices];      // the mass of a slice that is surely kept
     uint64_t mass[kSampleBins];
     uint32_t count[kSampleBins];
-    uint32_t found, unused;
+    uint32_t found, unused[63];      // (256 bytes)
     uint64_t list[kSampleList];              // places of candidates
     __device__ __forceinline__ uint64_t *slice_bins(int slice) { return reinterpret_cast<uint64_t *>(this + 1) + slice * kSampleBins; }
     static size_t bytes(int slices) { return sizeof(SampleShared) + (size_t)slices * kSampleBins * sizeof(uint64_t); }
