@@ -33,5 +33,5 @@ def program(tmp_path_factory):
 
 @pytest.mark.parametrize("cus", [1, 3, 256])
 def test_addresses_in_bounds(program, cus):
-    out = subprocess.run([program, str(cus), "24", "1"], capture_output=True, text=True, timeout=300)
+    out = subprocess.run([program, str(cus), "12", "1"], capture_output=True, text=True, timeout=300)
     assert out.returncode == 0, (out.stdout + out.stderr)[-6000:]
