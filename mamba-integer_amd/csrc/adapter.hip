@@ -5,9 +5,10 @@
 // in two kernels: t = x A^T (with the scales) into the workspace, then out = y + t B^T, the
 // sum rounded once to out's type.  Sequences of up to 7 tokens (decode steps) go row by row
 // on the vector units, where the adapters' bytes are the work; longer ones in tiles of 16
-// tokens on the matrix units, where x and y are.  16384 x 4096 -> 2048 of rank 32 in bf16: 31.6
-// and 33.6 us, 4.2 and 4.0 TB/s, bound by HBM; 64 x 1 x 2048 -> 8192 of rank 16: 4.0 and 4.6 us,
-// the second's B at 3.7 TB/s, and a call 10 us with its host side.
+// tokens on the matrix units, where x and y are.  16384 x 4096 -> 2048 of rank 32 in bf16: 40.1
+// and 37.5 us, 3.3 and 3.6 TB/s, bound by HBM (31.4 and 33.2 where the same rows come again and
+// the last-level cache has some of them); 64 x 1 x 2048 -> 8192 of rank 16: 4.2 and 4.8 us, the
+// second's B at 3.5 TB/s, and a call 10 us with its host side.
 #include <algorithm>
 #include <type_traits>
 

@@ -22,7 +22,7 @@ namespace mi {
 // bf16 68.6 us, 1 x 16384 x 1536 in float32 86.6; 8 waves 69.7 and 88.3, 4 waves 93 and 111, waves
 // of 8 steps with two channels a lane 78 and 101.  A wave takes 73 registers, so a CU has one
 // block; held to 64 for two of them it spills: 77.6 and 90.5.  What bounds it is that block's
-// chain of load, join and store (the vector units work in 37 us), in float32 HBM (4.8 TB/s).  Backwards 4 waves of 16, since a wave there
+// chain of load, join and store (the vector units work in 38 us), in float32 HBM (4.8 TB/s).  Backwards 4 waves of 16, since a wave there
 // takes 160 registers and a block of 8 leaves no room for a second one: 133 us against 166.
 constexpr int kSteps = 16, kWaves = 16;
 constexpr int kStepsBack = 16, kWavesBack = 4;

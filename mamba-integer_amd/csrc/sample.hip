@@ -16,7 +16,9 @@
 // Rows in slices, a launch each for the first of the order, the bins, the candidates and the
 // draw.  1 x 32000 takes 24 us, 64 x 131072 in bf16 76 (first 7, bins 18, candidates 24, draw
 // 29), where its bytes take 3: what bounds it is the chain of loads, barriers and sums over
-// lanes in each launch, and the exponentials (11 us of the bins).
+// lanes in each launch, and the exponentials (11 us of the bins).  Where more than 8192 tokens
+// are candidates (flat logits, a large top_k) a block goes over the whole row: 64 x 32000 within
+// 0.01 of each other 102 us with top_k 50, 164 by top_p.
 #include <algorithm>
 #include <type_traits>
 
@@ -832,7 +834,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
 }
 
 // Slices of a row: of 8192 tokens or so (each block has the row's bins to read first: 64 rows
-// of 32000 in slices of 4000 49 us, of 8000 42), 512 blocks at most.
+// of 32000 in slices of 4000 49 us, of 8000 42), 512 blocks at most.  So from 257 rows on a block
+// has a whole row: of 32000 with top_k 50 and top_p 0.9 79 us instead of the 44 of 256 rows, by
+// top_p alone 101 and 74; of 131072 269 and 91, 438 and 161.
 inline int sample_slices(int rows, int vocab) {
     const int n = std::min((vocab + 8191) / 8192, kSampleSlices);
     return std::max(1, std::min(n, kSampleBlocks / std::max(rows, 1)));

@@ -613,7 +613,7 @@ def adapter_add(y, x, a, b, ids, scales=None, x_scale=None, lens=None, out=None)
     [bank, N, rank] of one float type, rank up to 128; ids int32 [B] (outside [0, bank): no
     adapter), scales float32 [bank] (None: 1), lens int32 [B]: tokens of each sequence, the
     rows past them are y's.  ``out`` may be y: rows without an adapter are not touched then.
-    Forward only."""
+    Infinite values give what the formula gives.  Forward only."""
     return _calls().adapter_add(_here(), y, x, a, b, ids, scales, x_scale, lens, out)
 
 
@@ -623,6 +623,8 @@ def gated_scan(x, r, i, decay, z=None, rate: float = 8.0, h_in=None, h_out=None,
     x, r, i, z [B, L, D] of one float type; decay float32 [D]; h_in / h_out float32 [B, D]
     (None: zeros; may be the same tensor); L = 1 is a decode step.  lens int32 [B]: tokens of
     each sequence (h_out: the state after them; rows of the output past them are zero).
+    Infinite values give what the formula gives, but a state may become a NaN at a step whose a is
+    below 2^-126, and an infinite rate * softplus(decay) is the largest float.
 
     Differentiable, once, in x, r, i, decay, z and h_in; while autograd records one of them,
     out and h_out cannot be given.  In a graph's capture no other live graph may hold such a
